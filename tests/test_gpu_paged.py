@@ -1,0 +1,418 @@
+"""Paged-cache operators on the GPU against the 64-bit restatement in paged_reference.py, whose
+bounds are derived there.  Every cache has NaN in all slots that hold no token and table entries out
+of range behind each sequence, so anything read from there shows."""
+import pytest
+import torch
+
+import usagi_b200 as ub
+from usagi_b200 import _lib
+from paged_reference import Cache, attention, check_attention, rotate
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _setup():
+    ub.setup(device="cuda:0")
+    yield
+    ub.check_errors(DEV)
+
+
+def _q(B, Hq, Tq, dtype, seed, gain=2.0):
+    return (gain * torch.randn(B, Hq, Tq, 128,
+                               generator=torch.Generator().manual_seed(seed))).to(dtype)
+
+
+def _ql(q_lens):
+    return None if q_lens is None else torch.tensor(q_lens, dtype=torch.int32, device=DEV)
+
+
+# (lens, Hq, Hkv, Tq, q_lens, page, dtype, layout)
+DECODE = {
+    "one_token": ([1], 4, 4, 1, None, 16, F16, "hnd"),
+    "empty_and_short": ([0, 1, 2, 15, 16, 17, 127, 128, 129], 8, 2, 1, None, 16, BF16, "hnd"),
+    "odd_group": ([333, 40, 700], 6, 2, 1, None, 32, F16, "nhd"),
+    "group7": ([513, 255], 28, 4, 1, None, 64, BF16, "hnd"),
+    "group16": ([1000, 1], 32, 2, 1, None, 128, F16, "hnd"),
+    "group9_over_eight_rows": ([600], 9, 1, 1, None, 256, BF16, "nhd"),
+    "long_split": ([20011], 2, 1, 1, None, 64, F16, "hnd"),
+    "many_sequences": (list(range(0, 600, 2)), 2, 1, 1, None, 16, F16, "hnd"),
+    "page1024": ([3000, 1024], 4, 2, 1, None, 1024, BF16, "hnd"),
+    "drafts": ([5, 300, 4099], 8, 4, 5, None, 32, F16, "hnd"),
+    "drafts_ragged": ([700, 300, 40, 9], 14, 2, 4, [4, 0, 3, 1], 16, BF16, "nhd"),
+    "more_rows_than_tokens": ([3, 0], 4, 2, 6, None, 16, F16, "hnd"),
+    "group32_rows": ([300, 77], 32, 1, 1, None, 16, BF16, "hnd"),
+    "chunk": ([900, 130], 4, 2, 130, [130, 77], 64, F16, "hnd"),
+    "chunk_odd": ([700, 333], 6, 2, 100, [100, 99], 32, BF16, "nhd"),
+    "chunk_group5": ([513], 5, 1, 257, None, 128, F16, "hnd"),
+    "rows17": ([200, 1111], 17, 1, 1, None, 16, F16, "hnd"),
+    "group_over_128_rows_per_token": ([300], 130, 1, 1, None, 64, BF16, "hnd"),
+}
+
+
+@pytest.mark.parametrize("name", list(DECODE))
+def test_attention_over_the_cache(name):
+    lens, Hq, Hkv, Tq, q_lens, page, dtype, layout = DECODE[name]
+    c = Cache(lens, Hkv, page, dtype, 11, DEV, layout)
+    q = _q(len(lens), Hq, Tq, dtype, 12)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV), q_lens=_ql(q_lens))
+    ub.check_errors(DEV)
+    assert o.dtype == dtype and o.shape == q.shape
+    check_attention(o, lse, attention(q, c, q_lens))
+
+
+@pytest.mark.parametrize("window,glob", [(1, 0), (2, 1), (3, 4), (64, 2)])
+@pytest.mark.parametrize("Tq,Hq", [(1, 8), (5, 4), (200, 2)])
+def test_window_and_global_blocks(window, glob, Tq, Hq):
+    lens = [200, 640, 1283, 2000]
+    c = Cache(lens, 2, 32, F16, 21, DEV)
+    q = _q(4, Hq, Tq, F16, 22)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV), window=window, global_blocks=glob)
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c, None, window, glob))
+
+
+# (prefix, own lens, Hq, Hkv, Tq, q_lens, page, dtype, layout)
+SHARED = {
+    "small": (64, [1, 7, 30], 8, 2, 1, None, 16, F16, "hnd"),
+    "no_prefix": (0, [100, 40], 4, 2, 1, None, 32, BF16, "hnd"),
+    "ends_inside_a_tile": (336, [1, 200, 129], 8, 2, 1, None, 16, BF16, "nhd"),
+    "whole_tiles": (512, [3] * 9, 16, 2, 1, None, 128, F16, "hnd"),
+    "odd_group_many": (272, list(range(1, 60)), 6, 2, 1, None, 16, F16, "hnd"),
+    "group7": (400, list(range(1, 40)), 7, 1, 1, None, 16, BF16, "hnd"),
+    "drafts": (320, [5, 6, 70, 9, 33], 8, 2, 5, [5, 2, 0, 4, 5], 64, F16, "nhd"),
+    "chunks": (256, [70, 200], 4, 2, 70, [70, 33], 32, BF16, "hnd"),
+    "long_chunks": (256, [300], 2, 1, 300, None, 64, F16, "hnd"),
+    "one_sequence": (1280, [1], 4, 4, 1, None, 64, F16, "hnd"),
+    "wide": (2048, [1 + b % 17 for b in range(130)], 4, 1, 1, None, 64, BF16, "hnd"),
+    "shorter_than_the_prefix": (256, [-256, -100, -1, 0, 1, 40], 8, 2, 1, None, 64, F16, "hnd"),
+    "rows_end_inside_the_prefix": (256, [-100, 3, 2], 4, 2, 8, [8, 8, 1], 64, BF16, "hnd"),
+}
+
+
+@pytest.mark.parametrize("name", list(SHARED))
+def test_shared_prefix(name):
+    prefix, own, Hq, Hkv, Tq, q_lens, page, dtype, layout = SHARED[name]
+    lens = [prefix + n for n in own]
+    c = Cache(lens + [prefix], Hkv, page, dtype, 31, DEV, layout, prefix=prefix)
+    c.table, c.lens = c.table[:-1], c.lens[:-1]  # the last one only holds the whole prefix
+    q = _q(len(lens), Hq, Tq, dtype, 32)
+    o, lse = ub.shared_prefix_attn_fwd(q.to(DEV), *c.to(DEV), prefix_len=prefix,
+                                       q_lens=_ql(q_lens))
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c, q_lens))
+
+
+def test_scores_far_apart():
+    """Key blocks of growing size raise the running maximum again and again; a huge score makes
+    every other weight vanish."""
+    c = Cache([1500, 700], 2, 32, F16, 41, DEV)
+    k = c.pages[0]
+    for b, n in enumerate(c.lens):
+        for j in range(n):
+            k[c.table[b, j // 32], :, j % 32] *= 0.2 + j / 150
+    q = _q(2, 8, 1, F16, 42, gain=4.0)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV))
+    check_attention(o, lse, attention(q, c))
+    o2, lse2 = ub.shared_prefix_attn_fwd(q[:1].to(DEV).contiguous(), *[
+        x[:1] if i > 1 else x for i, x in enumerate(c.to(DEV))], prefix_len=1024)
+    check_attention(o2, lse2, [x[:1] for x in attention(q, c)])
+    ub.check_errors(DEV)
+
+
+@pytest.mark.parametrize("prefix", [0, 256])
+def test_options(prefix):
+    """Scale, output type, given outputs, no lse, int64 metadata, a strided table and q."""
+    c = Cache([300, 500], 2, 64, BF16, 51, DEV, prefix=prefix)
+    q = _q(2, 4, 3, BF16, 52)
+    kp, vp, table, lens = c.to(DEV)
+    kw = dict(prefix_len=prefix) if prefix else {}
+    fn = ub.shared_prefix_attn_fwd if prefix else ub.paged_attn_fwd
+    qs = q.transpose(1, 2).contiguous().to(DEV).transpose(1, 2)
+    wide = torch.full((2, 2 * table.shape[1]), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    out = torch.empty(2, 4, 3, 128, device=DEV, dtype=F16)
+    lse = torch.empty(2, 4, 3, device=DEV)
+    o, l2 = fn(qs, kp, vp, wide[:, :table.shape[1]], lens.long(), scale=0.05, out_dtype=F16,
+               out=out, lse_out=lse, **kw)
+    assert o is out and l2 is lse
+    check_attention(o, lse, attention(q, c, scale=0.05, out_dtype=F16))
+    o, none = fn(q.to(DEV), kp, vp, table, lens, return_lse=False, **kw)
+    assert none is None
+    want = attention(q, c)
+    check_attention(o, want[1], want)
+    ub.check_errors(DEV)
+
+
+APPEND = {
+    # lens, q_lens, Hq, Hkv, Tq, page, dtype, layout, rot, interleaved
+    "one": ([1], None, 4, 4, 1, 16, F16, "hnd", 128, False),
+    "batch": ([17, 1, 33, 500, 64], None, 8, 2, 1, 16, BF16, "nhd", 128, False),
+    "ragged_interleaved": ([40, 7, 300], [5, 0, 3], 6, 3, 5, 32, F16, "hnd", 64, True),
+    "prompt": ([130, 129], [130, 100], 2, 1, 130, 64, BF16, "hnd", 32, False),
+    "no_rotation": ([20, 19], None, 4, 2, 3, 16, F16, "nhd", 0, False),
+    "odd_rot": ([1000, 999], None, 3, 3, 2, 256, F16, "hnd", 48, False),
+    "full_interleaved": ([1000, 64], None, 3, 1, 2, 1024, BF16, "hnd", 128, True),
+    "no_q": ([90, 3], [2, 3], 0, 2, 3, 16, BF16, "hnd", 128, False),
+}
+
+
+@pytest.mark.parametrize("name", list(APPEND))
+def test_append(name):
+    lens, q_lens, Hq, Hkv, Tq, page, dtype, layout, rot, inter = APPEND[name]
+    c = Cache(lens, Hkv, page, dtype, 61, DEV, layout)
+    B = len(lens)
+    g = torch.Generator().manual_seed(62)
+    qkv = torch.randn(B, Tq, Hq + 2 * Hkv, 128, generator=g).to(dtype)
+    dev = qkv.to(DEV)
+    q, k, v = [x.transpose(1, 2) for x in dev.split([Hq, Hkv, Hkv], 2)]
+    inv = ub.rope_inv_freq(rot, 10000.0, DEV) if rot else None
+    kp, vp, table, sl = c.to(DEV)
+    out = ub.paged_kv_append(kp, vp, table, sl, k, v, q=q if Hq else None, q_lens=_ql(q_lens),
+                             inv_freq=inv, interleaved=inter)
+    ub.check_errors(DEV)
+    u = torch.finfo(dtype).eps / 2
+    want_k, want_v = [x.clone() for x in c.pages]
+    close = torch.zeros_like(want_k, dtype=torch.bool)
+    hq, hk, hv = [x.transpose(1, 2) for x in qkv.split([Hq, Hkv, Hkv], 2)]
+
+    def near(got, exact, pair):
+        """One rounding, after 32-bit products of values no larger than the pair's length."""
+        return (got.double().cpu() - exact).abs() <= u * exact.abs() + 2.0 ** -21 * pair + 2.0 ** -25
+
+    for b, L in enumerate(lens):
+        n = Tq if q_lens is None else q_lens[b]
+        pos = torch.arange(L - n, L)
+        turn = (lambda x: rotate(x, pos, inv.cpu(), inter)) if rot else (lambda x: x.double())
+        big = (lambda x: x.double().abs().amax(-1, keepdim=True)) if rot else (lambda x: 0.0)
+        if Hq:
+            assert near(out[b, :, :n], turn(hq[b, :, :n]), big(hq[b, :, :n])).all()
+            assert (out[b, :, n:] == 0).all()
+        page_of, slot = c.table[b, pos // page].long(), pos % page
+        got = kp.cpu()[page_of, :, slot].transpose(0, 1)
+        assert near(got, turn(hk[b, :, :n]), big(hk[b, :, :n])).all()
+        want_k[page_of, :, slot] = got.transpose(0, 1)
+        want_v[page_of, :, slot] = hv[b, :, :n].transpose(0, 1)
+    if not Hq:
+        assert out is None
+    # every other slot, and all of v, bit for bit
+    for got, want in ((kp, want_k), (vp, want_v)):
+        assert torch.equal(got.cpu().contiguous().view(torch.int16),
+                           want.contiguous().view(torch.int16))
+
+
+def test_append_far_positions():
+    """At position two million the angle has to be formed in 64 bits."""
+    page, n = 1024, 2_000_003
+    table = torch.full((1, n // page + 1), 0, dtype=torch.int32, device=DEV)
+    kp, vp = [torch.zeros(1, 1, page, 128, dtype=F16, device=DEV) for _ in range(2)]
+    x = torch.randn(1, 1, 1, 128, generator=torch.Generator().manual_seed(63)).half()
+    inv = ub.rope_inv_freq(128, 500000.0, DEV)
+    q = ub.paged_kv_append(kp, vp, table, torch.tensor([n], device=DEV), x.to(DEV), x.to(DEV),
+                           q=x.to(DEV), inv_freq=inv)
+    want = rotate(x, torch.tensor([n - 1]), inv, False)
+    bound = 2.0 ** -11 * want.abs() + 2.0 ** -20 * x.double().abs().max()
+    assert ((q.double().cpu() - want).abs() <= bound).all()
+    ub.check_errors(DEV)
+
+
+def test_append_in_place_and_unaligned():
+    c = Cache([100, 30], 2, 16, BF16, 71, DEV)
+    g = torch.Generator().manual_seed(72)
+    q, k, v = [torch.randn(2, h, 4, 128, generator=g).to(BF16).to(DEV) for h in (4, 2, 2)]
+    inv = ub.rope_inv_freq(128, device=DEV)
+    a, b = c.to(DEV), c.to(DEV)
+    want = ub.paged_kv_append(*a, k, v, q=q, inv_freq=inv)
+    odd = torch.empty(q.numel() + 1, dtype=BF16, device=DEV)[1:].view(q.shape)
+    odd.copy_(q)
+    same = q.clone()
+    got = ub.paged_kv_append(*b, k, v, q=same, inv_freq=inv, q_out=same)
+    assert got is same and torch.equal(got, want)
+    assert torch.equal(ub.paged_kv_append(*b, k, v, q=odd, inv_freq=inv), want)
+    for x, y in zip(a[:2], b[:2]):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+    ub.check_errors(DEV)
+
+
+def _expect_page_error():
+    with pytest.raises(ub.BsattnError) as err:
+        ub.check_errors(DEV)
+    assert err.value.code == _lib.E_PAGE
+    ub.check_errors(DEV)  # cleared
+
+
+@pytest.mark.parametrize("prefix", [0, 128])
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_bad_pages_and_lengths_are_reported(prefix, Tq):
+    """Out-of-range table entries, lengths and row counts are found and reported; the sequences
+    that are in order keep their results."""
+    c = Cache([200, 190, 180], 2, 16, F16, 81, DEV, prefix=prefix)
+    q = _q(3, 4, Tq, F16, 82).to(DEV)
+    kp, vp, table, lens = c.to(DEV)
+    fn = (lambda *a, **k: ub.shared_prefix_attn_fwd(*a, prefix_len=prefix, **k)) if prefix \
+        else ub.paged_attn_fwd
+    ref = fn(q, kp, vp, table, lens)
+    ub.check_errors(DEV)
+    want = attention(q.cpu(), c)
+
+    def in_order(o, lse, *which):
+        for b in which:
+            check_attention(o[b:b + 1], lse[b:b + 1], [x[b:b + 1] for x in want])
+
+    for value in (-1, kp.shape[0], 2 ** 31 - 1):
+        bad = table.clone()
+        bad[1, 9] = value
+        o, lse = fn(q, kp, vp, bad, lens)
+        _expect_page_error()
+        for b in (0, 2):
+            assert torch.equal(o[b], ref[0][b]) and torch.equal(lse[b], ref[1][b])
+    for value in (-5, table.shape[1] * 16 + 1, 2 ** 31 - 1):
+        bad = lens.clone()
+        bad[0] = value
+        # the pages a longer length reaches exist in the table's width only
+        ok = table.clamp(min=0)
+        o, lse = fn(q, kp.nan_to_num(), vp.nan_to_num(), ok, bad)
+        _expect_page_error()
+        in_order(o, lse, 1, 2)
+    for value in (-1, Tq + 1, 2 ** 31 - 1):
+        ql = torch.tensor([Tq, value, Tq], dtype=torch.int32, device=DEV)
+        o, lse = fn(q, kp, vp, table, lens, q_lens=ql)
+        _expect_page_error()
+        in_order(o, lse, 0, 2)
+
+
+def test_append_reports_bad_pages_and_writes_nothing_there():
+    c = Cache([40, 40], 1, 16, F16, 83, DEV)
+    kp, vp, table, lens = c.to(DEV)
+    x = torch.ones(2, 1, 1, 128, dtype=F16, device=DEV)
+    before = kp.clone()
+    for value in (-1, kp.shape[0], 2 ** 31 - 1):
+        bad = table.clone()
+        bad[0, 2] = value
+        ub.paged_kv_append(kp, vp, bad, lens, x, x)
+        _expect_page_error()
+    want = before.clone()
+    want[table[1, 2].item(), :, 39 % 16] = 1
+    assert torch.equal(kp.view(torch.int16), want.view(torch.int16))
+    ub.paged_kv_append(kp, vp, table, torch.tensor([10 ** 6, 40], device=DEV), x, x)
+    _expect_page_error()
+
+
+def test_results_do_not_depend_on_the_run():
+    c = Cache([5000, 3, 777, 1200], 2, 32, BF16, 91, DEV)
+    q = _q(4, 8, 1, BF16, 92).to(DEV)
+    args = c.to(DEV)
+    first = ub.paged_attn_fwd(q, *args)
+    shared = ub.shared_prefix_attn_fwd(q[:1].contiguous(), *args[:2], args[2][:1], args[3][:1],
+                                       prefix_len=4096)
+    for _ in range(5):
+        o, lse = ub.paged_attn_fwd(q, *args)
+        assert torch.equal(o, first[0]) and torch.equal(lse, first[1])
+        o, lse = ub.shared_prefix_attn_fwd(q[:1].contiguous(), *args[:2], args[2][:1], args[3][:1],
+                                           prefix_len=4096)
+        assert torch.equal(o, shared[0]) and torch.equal(lse, shared[1])
+    ub.check_errors(DEV)
+
+
+def test_two_graphs_side_by_side():
+    """Two graphs captured on one stream and replayed at once on two: nothing is shared."""
+    side = torch.cuda.Stream(DEV)
+    sets = []
+    for s in range(2):
+        c = Cache([4000 + 100 * s, 900], 2, 32, F16, 101 + s, DEV, prefix=512)
+        q = _q(2, 4, 1, F16, 103 + s).to(DEV)
+        sets.append((q, c.to(DEV)))
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    want, outs, graphs = [], [], []
+    with torch.cuda.stream(side):
+        for q, a in sets:
+            want.append([*ub.paged_attn_fwd(q, *a), *ub.shared_prefix_attn_fwd(q, *a, prefix_len=512)])
+        side.synchronize()
+        for q, a in sets:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                outs.append([*ub.paged_attn_fwd(q, *a),
+                             *ub.shared_prefix_attn_fwd(q, *a, prefix_len=512)])
+            graphs.append(graph)
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    for rep in range(20):
+        for o in outs:
+            for x in o:
+                x.zero_()
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(x, y) for x, y in zip(o, w)), rep
+    with torch.cuda.stream(side):
+        ub.check_errors(DEV)
+    del graphs
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^32 bytes per tensor whose tokens sit at its end."""
+    Hkv, page = 8, 64
+    n_pages = (1 << 32) // (Hkv * page * 128 * 2) + 40
+    kp, vp = [torch.zeros(n_pages, Hkv, page, 128, dtype=F16, device=DEV) for _ in range(2)]
+    L = 20 * page - 5
+    c = Cache([L], Hkv, page, F16, 111, DEV, extra_pages=0, width_extra=0)
+    first = n_pages - c.pages[0].shape[0]
+    kp[first:], vp[first:] = c.pages[0].to(DEV), c.pages[1].to(DEV)
+    table = c.table.to(DEV) + first
+    lens = torch.tensor([L], dtype=torch.int32, device=DEV)
+    q = _q(1, 16, 1, F16, 112)
+    want = attention(q, c)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), kp, vp, table, lens)
+    check_attention(o, lse, want)
+    o, lse = ub.shared_prefix_attn_fwd(q.to(DEV), kp, vp, table, lens, prefix_len=18 * page)
+    check_attention(o, lse, want)
+    x = torch.randn(1, Hkv, 1, 128, generator=torch.Generator().manual_seed(113)).half().to(DEV)
+    ub.paged_kv_append(kp, vp, table, lens, x, x)
+    at = table[0, (L - 1) // page].item(), (L - 1) % page
+    assert torch.equal(kp[at[0], :, at[1]], x[0, :, 0])
+    assert torch.equal(vp[at[0], :, at[1]], x[0, :, 0])
+    ub.check_errors(DEV)
+
+
+@pytest.mark.parametrize("window,glob", [(None, 0), (2, 1)])
+def test_prefill_then_decode(window, glob):
+    """The operators together, as a serving loop uses them: a prompt is appended (rotated) and
+    prefilled with the framework's window kernel, then tokens are added one by one and attend over
+    the cache.  Every step has to agree with the prefill kernel run over the whole sequence."""
+    B, H, page, T, steps = 2, 2, 64, 1024, 3
+    g = torch.Generator(device=DEV).manual_seed(121)
+    q, k, v = [torch.randn(B, H, T, 128, generator=g, device=DEV).half() for _ in range(3)]
+    inv = ub.rope_inv_freq(128, 10000.0, DEV)
+    kp, vp = [torch.full((B * T // page, H, page, 128), float("nan"), dtype=F16, device=DEV)
+              for _ in range(2)]
+    table = torch.randperm(B * T // page, generator=torch.Generator().manual_seed(1)).view(B, -1)
+    table = table.to(DEV, torch.int32)
+    # the whole sequence at once: rotated q, and k read back from the cache
+    full = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    rq = ub.paged_kv_append(kp, vp, table, full, k, v, q=q, inv_freq=inv)
+    rk = kp[table.long()].transpose(1, 2).reshape(B, H, T, 128)
+    o_ref, lse_ref = ub.block_sparse_attn_fwd_window(rq, rk, v, window=window or T // 128,
+                                                     global_blocks=glob)
+    # again: a prompt, then single tokens
+    kp.fill_(float("nan"))
+    vp.fill_(float("nan"))
+    n = T - steps
+    lens = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    ub.paged_kv_append(kp, vp, table, lens, k[:, :, :n], v[:, :, :n], inv_freq=inv)
+    for i in range(n, T):
+        lens += 1
+        qi = ub.paged_kv_append(kp, vp, table, lens, k[:, :, i:i + 1], v[:, :, i:i + 1],
+                                q=q[:, :, i:i + 1], inv_freq=inv)
+        assert torch.equal(qi, rq[:, :, i:i + 1])
+        o, lse = ub.paged_attn_fwd(qi, kp, vp, table, lens, window=window, global_blocks=glob)
+        # both kernels round P and o once each: 2 (u A + u |o|), with A <= max |v|
+        bound = 4 * 2.0 ** -11 * v.abs().max().item()
+        assert (o - o_ref[:, :, i:i + 1]).abs().max().item() <= bound
+        assert (lse - lse_ref[:, :, i:i + 1]).abs().max().item() <= 2e-4
+    assert torch.equal(kp[table.long()].transpose(1, 2).reshape(B, H, T, 128), rk)
+    ub.check_errors(DEV)

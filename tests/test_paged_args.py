@@ -1,0 +1,103 @@
+"""Refusals of the paged-cache entry points that need no GPU: the C ABI's argument checks run before
+any device access, and the Python side checks shapes before it asks for the device."""
+import ctypes
+
+import pytest
+import torch
+
+import usagi_b200 as ub
+from usagi_b200 import _lib
+
+S6 = (ctypes.c_int64 * 6)(*([128] * 6))
+
+
+def _fwd(**kw):
+    a = dict(q=16, kp=16, vp=16, st=S6, table=16, ts=4, mp=4, np=8, ps=16, sl=16, ql=None, o=16,
+             lse=None, B=1, Hq=2, Hkv=1, Tq=1, window=0, glob=0, prefix=0, flags=0, ws=16, wsb=256)
+    a.update(kw)
+    return _lib.load().bsattn_paged_fwd(
+        a["q"], a["kp"], a["vp"], a["st"], a["table"], a["ts"], a["mp"], a["np"], a["ps"], a["sl"],
+        a["ql"], a["o"], a["lse"], a["B"], a["Hq"], a["Hkv"], a["Tq"], a["window"], a["glob"],
+        a["prefix"], 0.0, a["flags"], 16, 1 << 20, a["ws"], a["wsb"], None)
+
+
+def _append(**kw):
+    a = dict(kp=16, vp=16, st=S6, table=16, ts=4, mp=4, np=8, ps=16, sl=16, ql=None, q=16, k=16,
+             v=16, ins=(ctypes.c_int64 * 9)(*([128] * 9)), qo=16, inv=16, rot=128, B=1, Hq=2, Hkv=1,
+             Tq=1, flags=0, ws=16, wsb=256)
+    a.update(kw)
+    return _lib.load().bsattn_paged_append(
+        a["kp"], a["vp"], a["st"], a["table"], a["ts"], a["mp"], a["np"], a["ps"], a["sl"], a["ql"],
+        a["q"], a["k"], a["v"], a["ins"], a["qo"], a["inv"], a["rot"], 0, a["B"], a["Hq"], a["Hkv"],
+        a["Tq"], a["flags"], a["ws"], a["wsb"], None)
+
+
+@pytest.mark.parametrize("call", [_fwd, _append])
+def test_cache_arguments(call):
+    for name in ("kp", "vp", "st", "table", "sl", "q"):
+        assert call(**{name: None}) == _lib.E_NULL, name
+    for kw in (dict(B=0), dict(Hkv=0), dict(Tq=0), dict(mp=0), dict(np=0), dict(ts=-1),
+               dict(ps=8), dict(ps=48), dict(ps=2048), dict(mp=1 << 27)):
+        assert call(**kw) == _lib.E_SHAPE, kw
+    assert call(kp=24) == _lib.E_ALIGN
+    assert call(st=(ctypes.c_int64 * 6)(128, 128, 132, 128, 128, 128)) == _lib.E_ALIGN
+    assert call(ws=None) == _lib.E_WORKSPACE
+    assert call(wsb=4) == _lib.E_WORKSPACE
+
+
+def test_attention_arguments():
+    for kw in (dict(window=-1), dict(glob=-1, window=1), dict(glob=1), dict(window=1 << 25),
+               dict(prefix=-16), dict(prefix=24), dict(prefix=80), dict(prefix=16, window=1)):
+        assert _fwd(**kw) == _lib.E_SHAPE, kw
+    assert _fwd(o=None) == _lib.E_NULL
+    assert _fwd(flags=4) == _lib.E_DTYPE
+    assert _fwd(q=24) == _lib.E_ALIGN
+    assert _fwd(o=24) == _lib.E_ALIGN
+
+
+def test_append_arguments():
+    assert _append(k=None) == _lib.E_NULL
+    assert _append(ins=None) == _lib.E_NULL
+    assert _append(qo=None) == _lib.E_NULL
+    assert _append(flags=1) == _lib.E_DTYPE
+    for rot in (0, 8, 24, 144, -16):
+        assert _append(rot=rot) == _lib.E_SHAPE, rot
+    assert _append(k=24) == _lib.E_ALIGN
+    assert _append(ins=(ctypes.c_int64 * 9)(*([128] * 8 + [100]))) == _lib.E_ALIGN
+
+
+def test_error_code_has_a_text():
+    assert "page" in _lib.strerror(_lib.E_PAGE)
+
+
+def test_python_side():
+    kp = torch.zeros(4, 2, 16, 128, dtype=torch.float16)
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    lens = torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 4, 1, 128, dtype=torch.float16)
+    k = torch.zeros(1, 2, 1, 128, dtype=torch.float16)
+    for call in (lambda: ub.paged_attn_fwd(q, kp, kp, table, lens),
+                 lambda: ub.shared_prefix_attn_fwd(q, kp, kp, table, lens, prefix_len=16),
+                 lambda: ub.paged_kv_append(kp, kp, table, lens, k, k)):
+        with pytest.raises(ValueError, match="no CPU path"):
+            call()
+    with pytest.raises(TypeError):
+        ub.paged_attn_fwd(q.float(), kp.float(), kp.float(), table, lens)
+    with pytest.raises(ValueError):
+        ub.paged_attn_fwd(q, kp[..., :64], kp[..., :64], table, lens)
+    with pytest.raises(ValueError):
+        ub.paged_attn_fwd(q[0], kp, kp, table, lens)
+    with pytest.raises(ValueError, match="window"):
+        ub.paged_attn_fwd(q, kp, kp, table, lens, window=0)
+    with pytest.raises(ValueError, match="window"):
+        ub.paged_attn_fwd(q, kp, kp, table, lens, global_blocks=1)
+    with pytest.raises(ValueError, match="whole pages"):
+        ub.shared_prefix_attn_fwd(q, kp, kp, table, lens, prefix_len=24)
+    with pytest.raises(ValueError, match="holds"):
+        ub.shared_prefix_attn_fwd(q, kp, kp, table, lens, prefix_len=80)
+
+
+def test_inv_freq():
+    f = ub.rope_inv_freq(64, 10000.0, "cpu")
+    assert f.dtype == torch.float64 and f.shape == (32,)
+    assert f[0] == 1.0 and abs(f[16].item() - 0.01) < 1e-15

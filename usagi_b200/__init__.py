@@ -17,6 +17,12 @@ from .api import (  # noqa: F401
     set_timeout_ns,
     setup,
 )
+from .paged import (  # noqa: F401
+    paged_attn_fwd,
+    paged_kv_append,
+    rope_inv_freq,
+    shared_prefix_attn_fwd,
+)
 from . import patterns  # noqa: F401
 
 __version__ = "0.1.0"

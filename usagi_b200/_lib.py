@@ -63,6 +63,31 @@ SIGNATURES = {
     "bsattn_ipc_open": (_c_int, [_c_void_p, ctypes.c_uint64, ctypes.POINTER(_c_void_p)]),
     "bsattn_ipc_close": (_c_int, [_c_void_p, ctypes.c_uint64]),
     "bsattn_peer_copy": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    "bsattn_paged_append": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p,          # k_pages, v_pages, page_strides (host int64[6])
+        _c_void_p, ctypes.c_int64, _c_int,        # block_table, table_stride, max_pages
+        _c_int, _c_int,                           # n_pages, page_size
+        _c_void_p, _c_void_p,                     # seq_lens, q_lens
+        _c_void_p, _c_void_p, _c_void_p,          # q, k, v
+        _c_void_p, _c_void_p,                     # in_strides (host int64[9]), q_out
+        _c_void_p, _c_int, _c_int,                # inv_freq, rot_dim, interleaved
+        _c_int, _c_int, _c_int, _c_int, _c_int,   # B, Hq, Hkv, Tq, dtype_flags
+        _c_void_p, _c_size_t, _c_void_p,          # workspace, bytes, stream
+    ]),
+    "bsattn_paged_scratch_bytes": (_c_int, [_c_int] * 7 + [ctypes.POINTER(_c_size_t)]),
+    "bsattn_paged_fwd": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p,          # q, k_pages, v_pages
+        _c_void_p,                                # page_strides (host int64[6])
+        _c_void_p, ctypes.c_int64, _c_int,        # block_table, table_stride, max_pages
+        _c_int, _c_int,                           # n_pages, page_size
+        _c_void_p, _c_void_p,                     # seq_lens, q_lens
+        _c_void_p, _c_void_p,                     # o, lse
+        _c_int, _c_int, _c_int, _c_int,           # B, Hq, Hkv, Tq
+        _c_int, _c_int, _c_int,                   # window, global_blocks, prefix_len
+        ctypes.c_float, _c_int,                   # scale, dtype_flags
+        _c_void_p, _c_size_t,                     # scratch, bytes
+        _c_void_p, _c_size_t, _c_void_p,          # workspace, bytes, stream
+    ]),
     "bsattn_fwd_noalloc": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p,          # q, k, v
         _c_void_p, _c_void_p,                     # o, lse
@@ -78,7 +103,7 @@ SIGNATURES = {
 OK = 0
 E_SHAPE, E_ALIGN, E_NULL, E_WORKSPACE, E_CUDA, E_TMA, E_DEVICE, E_CSR, E_TIMEOUT, E_DTYPE = (
     -1, -2, -3, -4, -5, -6, -7, -8, -9, -10)
-E_PLAN = -11
+E_PLAN, E_PAGE = -11, -12
 OUT_F16, OUT_BF16, IN_BF16 = 0, 1, 2
 CSR_WINDOW, CSR_PREFIX_WINDOW, CSR_RETRIEVAL = 0, 1, 2
 

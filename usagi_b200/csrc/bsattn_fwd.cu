@@ -1139,6 +1139,7 @@ const char* bsattn_strerror(int code) {
     case BSATTN_E_TIMEOUT: return "kernel pipeline wait timed out";
     case BSATTN_E_DTYPE: return "unsupported dtype flags";
     case BSATTN_E_PLAN: return "work list does not match this call";
+    case BSATTN_E_PAGE: return "page table entry, sequence length or live row count out of range";
     default: return "unknown error";
   }
 }

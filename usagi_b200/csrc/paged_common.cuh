@@ -1,0 +1,193 @@
+// paged_common.cuh -- what the paged-cache kernels share: the view of the cache and the batch,
+// the rule that turns a sequence's lengths into tiles, and thin wrappers of the warp-level
+// instructions (cp.async, ldmatrix, mma.sync, programmatic launch).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/bsattn.h"
+
+namespace bsattn {
+namespace paged {
+
+constexpr int kHeadDim = 128;
+constexpr int kTileKeys = 128;  // keys of one tile: the block size of the window rule
+
+// The cache and the batch as the kernels see them.  Strides are in bytes; the last dimension of
+// the pages is contiguous.
+struct Cache {
+  const char* k;
+  const char* v;
+  long long k_page, k_head, k_tok;
+  long long v_page, v_head, v_tok;
+  const int32_t* table;
+  long long table_stride;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;  // null: every sequence has Tq live rows
+  int max_pages, n_pages, page_shift;
+  int B, Hkv, Tq;
+  int* err;
+};
+
+__device__ __forceinline__ void raise(int* err, int code) { atomicCAS(err, 0, code); }
+
+// Length of sequence b and its live rows, both forced into what the table and the call can hold;
+// a value outside is reported and never used to form an address.
+struct SeqLen {
+  int len, rows;
+};
+__device__ __forceinline__ SeqLen seq_len(const Cache& c, int b) {
+  SeqLen s;
+  const int cap = c.max_pages << c.page_shift;
+  const int len = __ldg(c.seq_lens + b);
+  const int rows = c.q_lens != nullptr ? __ldg(c.q_lens + b) : c.Tq;
+  s.len = min(max(len, 0), cap);
+  s.rows = min(max(rows, 0), c.Tq);
+  if (s.len != len || s.rows != rows) raise(c.err, BSATTN_E_PAGE);
+  return s;
+}
+
+// Page of key position `pos` of sequence b, or -1 (reported) when the table entry is no page.
+__device__ __forceinline__ int page_checked(const Cache& c, int page) {
+  if (static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages)) return page;
+  raise(c.err, BSATTN_E_PAGE);
+  return -1;
+}
+
+// The key tiles of one sequence.  Row t is the token at position first + t and sees keys j <= its
+// position; with a window it sees blocks j / 128 < glob and j / 128 > position / 128 - window.
+// Tiles are the blocks any live row sees, in ascending order: n_glob leading ones, then those from
+// lo_block on.  Without a window the tiles start at key k0 (the end of a shared prefix, or 0).  A
+// sequence with no key still gets one tile, so that every row is written by the same path.
+struct Tiles {
+  int len, rows, first;
+  int n, n_glob, lo_block;
+};
+struct Rule {
+  int k0, window, glob;  // window == 0: every key
+};
+__device__ __forceinline__ Tiles tiles_of(const Cache& c, const Rule& r, int b) {
+  const SeqLen s = seq_len(c, b);
+  Tiles t;
+  t.len = s.len;
+  t.rows = s.rows;
+  t.first = s.len - s.rows;
+  t.n_glob = 0;
+  t.lo_block = 0;
+  int n = 0;
+  if (s.rows > 0 && s.len > r.k0) {
+    if (r.window == 0) {
+      n = (s.len - r.k0 + kTileKeys - 1) / kTileKeys;
+    } else {
+      t.lo_block = max(0, max(t.first, 0) / kTileKeys - r.window + 1);
+      t.n_glob = min(r.glob, t.lo_block);
+      n = t.n_glob + (s.len - 1) / kTileKeys - t.lo_block + 1;
+    }
+  }
+  t.n = max(n, 1);
+  return t;
+}
+__device__ __forceinline__ int tile_key(const Tiles& t, const Rule& r, int tile) {
+  return r.k0 + (tile < t.n_glob ? tile : t.lo_block + tile - t.n_glob) * kTileKeys;
+}
+
+// The keys one row sees: j < limit, and j >= lo or j < glob_end.  limit == 0: none.
+struct RowKeys {
+  int limit, lo;
+};
+__device__ __forceinline__ RowKeys row_keys(const Tiles& t, const Rule& r, int row_t) {
+  RowKeys k;
+  const int pos = t.first + row_t;
+  k.limit = (row_t < t.rows && pos >= 0) ? pos + 1 : 0;
+  k.lo = r.window == 0 ? 0 : max(0, pos / kTileKeys - r.window + 1) * kTileKeys;
+  return k;
+}
+
+// ---------------------------------------------------------------- instructions
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// Transposes an 8x8 matrix of 16-bit values held two per lane (row = lane / 4).
+__device__ __forceinline__ uint32_t movm_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, const uint32_t* b) {
+  if constexpr (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi, int bf16) {
+  return bf16 ? pack16<true>(lo, hi) : pack16<false>(lo, hi);
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t v) {
+  if constexpr (BF16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+// Programmatic launch: the next kernel of the stream may start its own setup; it waits for this
+// one's results with pdl_wait.
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ---------------------------------------------------------------- host
+// Number of SMs of the current device (checked to be sm_100).
+int device_sms(int* sms);
+
+// Checks and fills the cache view of a call (paged_attn.cu).
+int fill_cache(Cache* c, const void* k_pages, const void* v_pages, const int64_t* page_strides,
+               const int32_t* block_table, int64_t table_stride, int max_pages, int n_pages,
+               int page_size, const int32_t* seq_lens, const int32_t* q_lens, int B, int Hkv,
+               int Tq, void* workspace, size_t workspace_bytes);
+
+}  // namespace paged
+}  // namespace bsattn

@@ -1,0 +1,290 @@
+"""Paged K/V cache: new tokens into it, and attention over it (Python side of the C ABI).
+
+The prefill entry points (:func:`usagi_b200.block_sparse_attn_fwd`) answer one pass over a prompt.
+These continue it token by token: :func:`paged_kv_append` puts the keys and values of new tokens
+into the cache, rotated to their positions, and :func:`paged_attn_fwd` is the attention of the new
+tokens over everything held, with the same window + global-blocks rows as
+:func:`usagi_b200.block_sparse_attn_fwd_window`; :func:`shared_prefix_attn_fwd` is the same for a
+batch whose sequences begin with the same pages.  Serving only: there is no backward pass here, as
+there is none for the prefill.
+
+The cache is plain tensors that the caller owns:
+
+* ``k_pages``, ``v_pages``: fp16 or bf16 ``[n_pages, Hkv, page_size, 128]``, page_size a power of two
+  from 16 to 1024.  Any strides that are multiples of 8 with a contiguous last dimension: a
+  ``[n_pages, page_size, Hkv, 128]`` cache is passed as ``pages.transpose(1, 2)``.
+* ``block_table``: int ``[B, max_pages]``, the pages of each sequence in order.  Entries behind a
+  sequence's length are not read and may be anything.
+* ``seq_lens``: int ``[B]``, tokens of each sequence, the new ones of this call included.
+* ``q_lens``: int ``[B]`` or None, how many of the Tq rows of each sequence are live (None: all).
+  Row t < q_lens[b] is the token at position ``seq_lens[b] - q_lens[b] + t``; the rows behind them are
+  padding.
+
+A page table entry, a length or a row count out of range is found on the device, never used as an
+address, and raised by :func:`usagi_b200.check_errors` (code ``E_PAGE``).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .api import HEAD_DIM, BsattnError, _workspace
+
+__all__ = ["paged_kv_append", "paged_attn_fwd", "shared_prefix_attn_fwd", "rope_inv_freq"]
+
+_Strides6 = ctypes.c_int64 * 6
+_Strides9 = ctypes.c_int64 * 9
+
+
+def rope_inv_freq(rot_dim: int = HEAD_DIM, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """``base ** (-2 i / rot_dim)`` for i < rot_dim / 2 in 64 bits, for :func:`paged_kv_append`."""
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    return (float(base) ** (-2.0 * i / rot_dim)).to(device)
+
+
+def _index(t: torch.Tensor, name: str, dev, shape) -> torch.Tensor:
+    """``t`` as int32 on ``dev``; ``shape`` is its expected shape (-1: any)."""
+    if t.dim() != len(shape) or any(n not in (-1, m) for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != torch.int32 or t.device != dev:
+        t = t.to(device=dev, dtype=torch.int32)
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t
+
+
+def _rows(t: torch.Tensor, name: str, dev, dtype) -> torch.Tensor:
+    """A [B, H, T, 128] input as the kernels read it in place: 16-byte rows and strides."""
+    if t.dim() != 4 or t.shape[3] != HEAD_DIM:
+        raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}], got {tuple(t.shape)}")
+    if t.dtype != dtype or t.device != dev:
+        raise TypeError(f"{name} must be {dtype} on {dev} like the pages, got {t.dtype} on "
+                        f"{t.device}")
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+class _Call:
+    """The checked cache arguments of one call, in the order of the C ABI."""
+
+    __slots__ = ("dev", "dtype", "B", "Hkv", "head", "lens", "keep", "max_pages", "page_size")
+
+    def __init__(self, k_pages, v_pages, block_table, seq_lens, q_lens, B):
+        if k_pages.dim() != 4 or k_pages.shape[3] != HEAD_DIM or v_pages.shape != k_pages.shape:
+            raise ValueError(f"k_pages and v_pages must be [n_pages, Hkv, page_size, {HEAD_DIM}] of "
+                             f"one shape, got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
+        dev, dtype = k_pages.device, k_pages.dtype
+        if dtype not in (torch.float16, torch.bfloat16) or v_pages.dtype != dtype:
+            raise TypeError("k_pages and v_pages must both be float16 or both bfloat16, got "
+                            f"{dtype}, {v_pages.dtype}")
+        if not k_pages.is_cuda or v_pages.device != dev:
+            raise ValueError("the paged cache needs CUDA tensors on one device (there is no CPU "
+                             "path)")
+        n_pages, Hkv, page_size, _ = k_pages.shape
+        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+        ks, vs = k_pages.stride(), v_pages.stride()
+        if ks[3] != 1 or vs[3] != 1 or any(s % 8 for s in ks[:3] + vs[:3]) \
+                or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
+            raise ValueError("k_pages and v_pages must be 16-byte aligned, with a contiguous last "
+                             "dimension and strides that are multiples of 8")
+        table = _index(block_table, "block_table", dev, (B, -1))
+        sl = _index(seq_lens, "seq_lens", dev, (B,))
+        ql = None if q_lens is None else _index(q_lens, "q_lens", dev, (B,))
+        self.dev, self.dtype, self.B, self.Hkv = dev, dtype, B, Hkv
+        self.max_pages, self.page_size = table.shape[1], page_size
+        self.keep = (table, sl, ql)
+        self.head = (k_pages.data_ptr(), v_pages.data_ptr(), _Strides6(*ks[:3], *vs[:3]),
+                     table.data_ptr(), table.stride(0), table.shape[1], n_pages, page_size,
+                     sl.data_ptr(), ql.data_ptr() if ql is not None else None)
+
+
+class _on:
+    """``torch.cuda.device`` without its cost when ``dev`` is current already."""
+
+    __slots__ = ("ctx",)
+
+    def __init__(self, dev):
+        self.ctx = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                    q: Optional[torch.Tensor] = None, q_lens: Optional[torch.Tensor] = None,
+                    inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
+                    q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Put the keys and values of new tokens into the cache (``bsattn_paged_append``).
+
+    k, v: ``[B, Hkv, Tq, 128]``, q: ``[B, Hq, Tq, 128]`` or None, all of the pages' dtype and with any
+    strides (the slices of a fused projection are read in place).  With ``inv_freq`` (float64
+    ``[rot_dim / 2]``, rot_dim a multiple of 16 up to 128; see :func:`rope_inv_freq`) the first
+    rot_dim values of every row of k and q are turned by position * inv_freq[i], pairs
+    (x_i, x_{i + rot_dim/2}) or, ``interleaved``, (x_2i, x_{2i+1}); angles are formed in 64 bits.  Only
+    the slots of live rows are written.  Returns the rotated q, contiguous, with zeros in padding
+    rows (``q_out`` when given; it may be q itself if that is contiguous), or None without q.
+    """
+    lib = _lib.load()
+    if k.dim() != 4:
+        raise ValueError(f"k must be [B, Hkv, Tq, {HEAD_DIM}], got {tuple(k.shape)}")
+    B, _, Tq, _ = k.shape
+    c = _Call(k_pages, v_pages, block_table, seq_lens, q_lens, B)
+    dev, dtype = c.dev, c.dtype
+    k, v = _rows(k, "k", dev, dtype), _rows(v, "v", dev, dtype)
+    if k.shape[1] != c.Hkv or v.shape != k.shape:
+        raise ValueError(f"k and v must be [{B}, {c.Hkv}, {Tq}, {HEAD_DIM}], got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    Hq = 0
+    if q is not None:
+        Hq = q.shape[1] if q.dim() == 4 else 0
+        if tuple(q.shape) != (B, Hq, Tq, HEAD_DIM) or Hq == 0:
+            raise ValueError(f"q must be [{B}, Hq, {Tq}, {HEAD_DIM}], got {tuple(q.shape)}")
+        q = _rows(q, "q", dev, dtype)
+        if q_out is None:
+            q_out = torch.empty((B, Hq, Tq, HEAD_DIM), device=dev, dtype=dtype)
+        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.device != dev \
+                or not q_out.is_contiguous():
+            raise ValueError("q_out has the wrong shape, dtype, device or layout")
+    elif q_out is not None:
+        raise ValueError("q_out needs q")
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != dev:
+            raise TypeError("inv_freq must be float64 [rot_dim / 2] on the device of the pages")
+        rot = 2 * inv_freq.shape[0]
+        if rot % 16 or not 0 < rot <= HEAD_DIM:
+            raise ValueError(f"rot_dim must be a multiple of 16 up to {HEAD_DIM}, got {rot}")
+        inv_freq = inv_freq.contiguous()
+    if B == 0 or Tq == 0:
+        return q_out
+    strides = _Strides9(*(q.stride()[:3] if q is not None else (0, 0, 0)), *k.stride()[:3],
+                        *v.stride()[:3])
+    with _on(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        ws = _workspace(dev, stream)
+        rc = lib.bsattn_paged_append(
+            *c.head, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), strides,
+            q_out.data_ptr() if q is not None else None,
+            inv_freq.data_ptr() if inv_freq is not None else None, rot, int(bool(interleaved)), B,
+            Hq, c.Hkv, Tq, _lib.IN_BF16 if dtype == torch.bfloat16 else 0, ws.data_ptr(),
+            ws.numel() * 4, stream)
+    if rc != 0:
+        raise BsattnError(rc, "bsattn_paged_append")
+    return q_out
+
+
+def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   block_table: torch.Tensor, seq_lens: torch.Tensor, *,
+                   q_lens: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                   global_blocks: int = 0, scale: Optional[float] = None,
+                   out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+                   lse_out: Optional[torch.Tensor] = None, return_lse: bool = True
+                   ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Attention of the new tokens over the paged cache (``bsattn_paged_fwd``).
+
+    q: ``[B, Hq, Tq, 128]`` of the pages' dtype, Hq a multiple of Hkv; Tq = 1 is the usual decode
+    step, more rows check drafted tokens or process a chunk of a prompt.  The new tokens' keys are
+    in the cache already (:func:`paged_kv_append`); each row sees the keys up to its own position.
+    ``window`` (in blocks of 128) keeps, for a row in block i, the blocks > i - window and the first
+    ``global_blocks``: the rows of :func:`usagi_b200.block_sparse_attn_fwd_window`.  Returns
+    ``(o, lse)`` like the prefill calls: o ``[B, Hq, Tq, 128]`` in ``out_dtype`` (default: q's),
+    lse fp32 ``[B, Hq, Tq]`` (None if ``return_lse=False``); rows without a key, padding among them,
+    get o = 0, lse = -inf.
+    """
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1 block, got {window}")
+    if global_blocks < 0 or (global_blocks and window is None):
+        raise ValueError("global_blocks must not be negative and needs a window")
+    return _attn(q, k_pages, v_pages, block_table, seq_lens, q_lens, window or 0, global_blocks, 0,
+                 scale, out_dtype, out, lse_out, return_lse)
+
+
+def shared_prefix_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                           block_table: torch.Tensor, seq_lens: torch.Tensor, *, prefix_len: int,
+                           q_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                           out_dtype: Optional[torch.dtype] = None,
+                           out: Optional[torch.Tensor] = None,
+                           lse_out: Optional[torch.Tensor] = None, return_lse: bool = True
+                           ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """:func:`paged_attn_fwd` for a batch whose sequences all begin with the same ``prefix_len``
+    tokens (a system prompt, a document): whole pages, at the front of every row of ``block_table``,
+    read through the row of sequence 0 and once for the whole batch.  Same arguments and same
+    result; a sequence may also be shorter than the prefix.
+    """
+    page = k_pages.shape[2] if k_pages.dim() == 4 else 1
+    if prefix_len < 0 or prefix_len % page:
+        raise ValueError(f"prefix_len must be whole pages (multiples of {page}), got {prefix_len}")
+    if block_table.dim() == 2 and prefix_len > block_table.shape[1] * page:
+        raise ValueError("prefix_len is more than block_table holds")
+    return _attn(q, k_pages, v_pages, block_table, seq_lens, q_lens, 0, 0, int(prefix_len), scale,
+                 out_dtype, out, lse_out, return_lse)
+
+
+def _attn(q, k_pages, v_pages, block_table, seq_lens, q_lens, window, global_blocks, prefix_len,
+          scale, out_dtype, out, lse_out, return_lse):
+    lib = _lib.load()
+    if q.dim() != 4 or q.shape[3] != HEAD_DIM:
+        raise ValueError(f"q must be [B, Hq, Tq, {HEAD_DIM}], got {tuple(q.shape)}")
+    B, Hq, Tq, _ = q.shape
+    c = _Call(k_pages, v_pages, block_table, seq_lens, q_lens, B)
+    dev = c.dev
+    if q.dtype != c.dtype or q.device != dev:
+        raise TypeError(f"q must be {c.dtype} on {dev} like the pages, got {q.dtype} on {q.device}")
+    if c.Hkv == 0 or Hq == 0 or Hq % c.Hkv:
+        raise ValueError(f"Hq must be a multiple of Hkv, got {Hq} and {c.Hkv}")
+    if out_dtype is None:
+        out_dtype = q.dtype
+    if out_dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"out_dtype must be float16 or bfloat16, got {out_dtype}")
+    if not q.is_contiguous():
+        q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    if out is None:
+        out = torch.empty(q.shape, device=dev, dtype=out_dtype)
+    elif out.shape != q.shape or out.dtype != out_dtype or out.device != dev \
+            or not out.is_contiguous():
+        raise ValueError("out has the wrong shape, dtype, device or layout")
+    lse = None
+    if return_lse:
+        lse = lse_out
+        if lse is None:
+            lse = torch.empty((B, Hq, Tq), device=dev, dtype=torch.float32)
+        elif lse.shape != (B, Hq, Tq) or lse.dtype != torch.float32 or lse.device != dev \
+                or not lse.is_contiguous():
+            raise ValueError("lse_out has the wrong shape, dtype, device or layout")
+    if B == 0 or Tq == 0:
+        return out, lse
+    flags = (_lib.IN_BF16 if c.dtype == torch.bfloat16 else 0) | \
+        (_lib.OUT_BF16 if out_dtype == torch.bfloat16 else 0)
+    with _on(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        ws = _workspace(dev, stream)
+        need = ctypes.c_size_t(0)
+        rc = lib.bsattn_paged_scratch_bytes(B, Hq, c.Hkv, Tq, c.max_pages, c.page_size, prefix_len,
+                                            ctypes.byref(need))
+        if rc != 0:
+            raise BsattnError(rc, "bsattn_paged_scratch_bytes")
+        # From the caching allocator: in a captured graph it belongs to the graph.
+        scratch = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        rc = lib.bsattn_paged_fwd(
+            q.data_ptr(), *c.head, out.data_ptr(), lse.data_ptr() if lse is not None else None, B,
+            Hq, c.Hkv, Tq, window, global_blocks, prefix_len,
+            float(scale) if scale is not None else 0.0, flags, scratch.data_ptr(), need.value,
+            ws.data_ptr(), ws.numel() * 4, stream)
+    if rc != 0:
+        raise BsattnError(rc, "bsattn_paged_fwd")
+    return out, lse
