@@ -416,3 +416,30 @@ def test_prefill_then_decode(window, glob):
         assert (lse - lse_ref[:, :, i:i + 1]).abs().max().item() <= 2e-4
     assert torch.equal(kp[table.long()].transpose(1, 2).reshape(B, H, T, 128), rk)
     ub.check_errors(DEV)
+
+
+def test_wait_timeout_is_reported_and_context_survives():
+    """The many-row kernel's waits are bounded: with the test hook its Q K^T issuers wait on a barrier
+    that nothing signals, the bound runs out on every SM, and the host reads the status."""
+    c = Cache([900, 500], 2, 32, F16, 131, DEV, prefix=256)
+    args = c.to(DEV)
+    calls = [lambda q=_q(2, 4, 40, F16, 132).to(DEV): ub.paged_attn_fwd(q, *args),
+             lambda q=_q(2, 4, 1, F16, 133).to(DEV): ub.shared_prefix_attn_fwd(q, *args,
+                                                                            prefix_len=256)]
+    want = [f() for f in calls]
+    ub.check_errors(DEV)
+    lib = _lib.load()
+    for f, w in zip(calls, want):
+        try:
+            ub.set_timeout_ns(10_000_000)
+            lib.bsattn_test_unsignalled_wait(1)
+            f()
+            with pytest.raises(ub.BsattnError) as err:
+                ub.check_errors(DEV)
+            assert err.value.code == _lib.E_TIMEOUT
+        finally:
+            lib.bsattn_test_unsignalled_wait(0)
+            ub.set_timeout_ns(2_000_000_000)
+        o, lse = f()
+        ub.check_errors(DEV)
+        assert torch.equal(o, w[0]) and torch.equal(lse, w[1])

@@ -1020,6 +1020,10 @@ static DeviceInfo g_dev[64];
 static unsigned long long g_timeout_ns = 2000000000ull;
 static int g_test_unsignalled_wait = 0;
 
+// The same bound and test hook for the library's other pipelined kernels.
+unsigned long long launch_timeout_ns() { return g_timeout_ns; }
+int launch_test_wait() { return g_test_unsignalled_wait; }
+
 static size_t smem_bytes() { return sizeof(SharedStorage) + 1024; }
 
 // Heads per item group: K and V of one head take 2 * T * 128 * 2 bytes; keep a group's worth near

@@ -32,6 +32,7 @@
 #include <mutex>
 
 #include "paged_common.cuh"
+#include "paged_tile.cuh"
 #include "sm100_ptx.cuh"
 
 namespace bsattn {
@@ -52,9 +53,10 @@ struct AttnParams {
   const void* q;
   void* o;
   float* lse;
-  int G, rows, row_tiles;  // rows = G * Tq; row_tiles = ceil(rows / R)
+  int rows, row_tiles;  // rows = G * Tq; row_tiles = ceil(rows / R)
   float scale_log2;
   int out_bf16;
+  int all_partial;  // behind a shared prefix: no piece is a whole result
   // Scratch: prefix sums of the tiles per sequence [B + 1], partial outputs and their log2 sums.
   int* cum;
   float* part_o;
@@ -69,6 +71,13 @@ struct DecodeSmem {
   int warp_sum[kWarps];
   int found[3];
 };
+
+// Where a piece of item `item` that CTA `cta` holds leaves its partial output.  A CTA holds at most
+// one piece that begins its item and one other; when whole items are partial too, item + cta
+// numbers all pieces, since along the line one of the two always grows.
+__device__ __forceinline__ long long part_slot(int all_partial, long long item, int cta, bool head) {
+  return all_partial ? item + cta : 2ll * cta + (head ? 1 : 0);
+}
 
 // A position on the line of tiles.
 struct Cursor {
@@ -123,7 +132,10 @@ __global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_const
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) p.cum[p.c.B] = total;
   __syncthreads();
-  if (begin >= end) return;
+  if (begin >= end) {
+    pdl_wait();
+    return;
+  }
 
   auto seek = [&](Cursor& x) {
     x.b = sh.found[0];
@@ -338,8 +350,9 @@ __global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_const
             sh.l[warp][nb * 8 + 2 * t4 + c] = l[nb][c];
           }
         }
-      const bool whole = seg_tile0 == 0 && cx.tile + 1 == cx.t.n;
-      const long long slot = (static_cast<long long>(cx.b) * per_seq + cx.h) + blockIdx.x;
+      const bool whole = !p.all_partial && seg_tile0 == 0 && cx.tile + 1 == cx.t.n;
+      const long long slot = part_slot(p.all_partial, static_cast<long long>(cx.b) * per_seq + cx.h,
+                                       static_cast<int>(blockIdx.x), seg_tile0 == 0);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         __syncthreads();
@@ -397,35 +410,88 @@ __global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_const
     if (i + 1 < n_tiles) advance(cx);
   }
   cp_async_wait<0>();
+  // Behind a shared prefix this kernel starts while the prefix's still runs, and must not end
+  // before it: the join waits for this kernel only.
+  pdl_wait();
 }
 
-// Joins the pieces of the items that were split: o = sum_i o_i 2^(l_i - l), l = log2 sum 2^l_i.
-// One block per row; its four warps take every fourth piece and meet in shared memory.
+// Joins the pieces of a row: o = sum_i o_i 2^(l_i - l), l = log2 sum 2^l_i, over the pieces of its
+// item in the order of the line, then over those of the shared prefix.  A row whose item is one
+// piece is written already.  One block per row; its four warps take every fourth piece and meet in
+// shared memory.
 constexpr int kJoinWarps = 4;
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttnParams p,
-                                                               int pieces, int R) {
+struct JoinParams {
+  int Hkv, G, Tq;
+  void* o;
+  float* lse;
+  int out_bf16;
+  // Own keys: virtual sequence = b * v_per_seq + t / v_tok, item = it * heads + head tile, where a
+  // K/V head's rows are in tiles of R (few-row kernel) or already one tile (n_t tokens each).
+  const int* cum;
+  const float* part_o;
+  const float* part_l;
+  int count, pieces, R, row_tiles, all_partial;
+  int n_t, per_seq;  // many-row kernel: tokens per tile of rows; 0: few-row kernel
+  // Prefix: n_b sequences per tile of rows, each item tiles_p tiles, pieces_p CTAs.
+  const float* pre_o;
+  const float* pre_l;
+  int n_b, tiles_p, quota_p;
+};
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ JoinParams p) {
   __shared__ float4 so[kJoinWarps][32];
   __shared__ float sl[kJoinWarps], sm[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per_seq = p.c.Hkv * p.row_tiles;
-  const int row = blockIdx.x % p.rows;
-  const int bh = blockIdx.x / p.rows;
-  const int b = bh / p.c.Hkv;
-  const int hr = (bh - b * p.c.Hkv) * p.row_tiles + row / R;
+  const int t = blockIdx.x % p.Tq;
+  const int bh = blockIdx.x / p.Tq;
+  const int Hq = p.Hkv * p.G;
+  const int b = bh / Hq, hq = bh - b * Hq;
+  const int h = hq / p.G, g = hq - h * p.G;
+  int v, hr, r;
+  if (p.n_t > 0) {
+    v = b * p.per_seq + t / p.n_t;
+    hr = h;
+    r = g * p.n_t + t % p.n_t;
+  } else {
+    const int row = g * p.Tq + t;
+    v = b;
+    hr = h * p.row_tiles + row / p.R;
+    r = row % p.R;
+  }
+  const int heads = p.Hkv * p.row_tiles;
   pdl_wait();
-  const int c0 = p.cum[b], n = p.cum[b + 1] - c0;
-  const int line = p.cum[p.c.B] * per_seq;
-  const int quota = (line + pieces - 1) / pieces;
-  const int s = c0 * per_seq + hr * n;
+  const int c0 = p.cum[v], n = p.cum[v + 1] - c0;
+  const int line = p.cum[p.count] * heads;
+  const int quota = (line + p.pieces - 1) / p.pieces;
+  const int s = c0 * heads + hr * n;
   const int first = s / quota, last = (s + n - 1) / quota;
-  if (first == last) return;  // written whole
-  const long long slot0 = static_cast<long long>(b) * per_seq + hr;
-  const int r = row % R;
+  if (first == last && !p.all_partial) return;
+  const long long item = static_cast<long long>(v) * heads + hr;
+  int first_p = 0, pre = 0;  // pieces of the prefix
+  long long item_p = 0;
+  int rp = 0;
+  if (p.tiles_p > 0) {
+    item_p = static_cast<long long>(b / p.n_b) * p.Hkv + h;
+    rp = ((b % p.n_b) * p.G + g) * p.Tq + t;
+    const long long sp = item_p * p.tiles_p;
+    first_p = static_cast<int>(sp / p.quota_p);
+    pre = static_cast<int>((sp + p.tiles_p - 1) / p.quota_p) - first_p + 1;
+  }
+  const int own = last - first + 1;
   float mx = -INFINITY, sum = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int c = first + warp; c <= last; c += kJoinWarps) {
-    const float lg = p.part_l[(slot0 + c) * R + r];
-    const float4 y = reinterpret_cast<const float4*>(p.part_o)[((slot0 + c) * R + r) * (kHeadDim / 4) + lane];
+  for (int i = warp; i < own + pre; i += kJoinWarps) {
+    const float *po, *pl;
+    if (i < own) {
+      const long long row = part_slot(p.all_partial, item, first + i, i == 0) * p.R + r;
+      po = p.part_o + row * kHeadDim;
+      pl = p.part_l + row;
+    } else {
+      const long long row = (item_p + first_p + i - own) * 128 + rp;
+      po = p.pre_o + row * kHeadDim;
+      pl = p.pre_l + row;
+    }
+    const float lg = *pl;
+    const float4 y = reinterpret_cast<const float4*>(po)[lane];
     if (lg == -INFINITY) continue;
     const float mn = fmaxf(mx, lg);
     const float fa = ptx::ex2(mx - mn), fb = ptx::ex2(lg - mn);
@@ -460,11 +526,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     out.w += y.w * f;
   }
   const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-  const long long g = static_cast<long long>(bh) * p.rows + row;
-  reinterpret_cast<uint2*>(p.o)[g * (kHeadDim / 4) + lane] =
+  const long long row = blockIdx.x;
+  reinterpret_cast<uint2*>(p.o)[row * (kHeadDim / 4) + lane] =
       make_uint2(pack_out(out.x * inv, out.y * inv, p.out_bf16), pack_out(out.z * inv, out.w * inv, p.out_bf16));
   if (p.lse != nullptr && lane == 0)
-    p.lse[g] = total > 0.0f ? (top + log2f(total)) * 0.69314718055994531f : -INFINITY;
+    p.lse[row] = total > 0.0f ? (top + log2f(total)) * 0.69314718055994531f : -INFINITY;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -492,6 +558,8 @@ int device_sms(int* sms) {
                                static_cast<int>(i < 2 ? sizeof(DecodeSmem<1>)
                                                       : sizeof(DecodeSmem<2>))) != cudaSuccess)
         return BSATTN_E_CUDA;
+    const int rt = tile_setup();
+    if (rt != BSATTN_OK) return rt;
     known[dev] = n;
   }
   *sms = known[dev];
@@ -538,36 +606,110 @@ int fill_cache(Cache* c, const void* k_pages, const void* v_pages, const int64_t
   return BSATTN_OK;
 }
 
-// The launch of one call: rows of q per tile of rows, pieces of the line, scratch.
+// The launches of one call and their scratch.
 struct Shape {
-  int rows, R, row_tiles, pieces;
-  long long items, slots;
-  size_t cum_bytes, bytes;
+  int rows;         // G * Tq
+  bool few;         // own keys by the few-row kernel
+  bool prefix;      // prefix keys by the many-row kernel, stacked over the batch
+  int k0;           // first own key
+  int R, row_tiles, pieces, count;
+  bool all_partial;
+  RowTiles rt;      // of the many-row kernel's launch
+  int tiles_p, pieces_p;
+  long long slots, slots_p;
+  size_t cum, part_o, part_l, cum_p, pre_o, pre_l, bytes;  // offsets into the scratch
 };
 
-static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size, int sms,
-                    Shape* s) {
+constexpr int kFewRows = 16;     // rows of one tile of the few-row kernel
+constexpr int kStackedRows = 64; // more rows of one sequence fill a tile without its neighbours
+
+static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size, int prefix_len,
+                    int sms, Shape* s) {
   if (B < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv != 0 || Tq < 1) return BSATTN_E_SHAPE;
-  const long long rows = static_cast<long long>(Hq / Hkv) * Tq;
+  const int G = Hq / Hkv;
+  const long long rows = static_cast<long long>(G) * Tq;
   if (rows * B * Hkv > (1ll << 31) - 1) return BSATTN_E_SHAPE;
   s->rows = static_cast<int>(rows);
-  s->R = rows <= 8 ? 8 : 16;
-  s->row_tiles = static_cast<int>((rows + s->R - 1) / s->R);
-  s->items = static_cast<long long>(B) * Hkv * s->row_tiles;
-  // Most tiles a sequence can have; the line is never longer than that for every item.
+  s->prefix = prefix_len > 0 && rows <= kStackedRows;
+  s->few = s->prefix || rows <= kFewRows || G > 128;
+  s->k0 = s->prefix ? prefix_len : 0;
+  s->all_partial = s->prefix;
+  // Most tiles one item can have.
   const long long tiles = (static_cast<long long>(max_pages) * page_size + kTileKeys - 1) / kTileKeys + 1;
-  if (s->items * tiles > (1ll << 30)) return BSATTN_E_SHAPE;
-  s->pieces = static_cast<int>(std::min<long long>(sms, s->items * tiles));
-  // A piece of an item is numbered item + CTA: along the line one of the two always grows.
-  s->slots = s->items + s->pieces;
-  s->cum_bytes = (static_cast<size_t>(B + 1) * sizeof(int) + 255) / 256 * 256;
-  s->bytes = s->cum_bytes + static_cast<size_t>(s->slots) * s->R * (kHeadDim + 1) * sizeof(float);
+  long long items;
+  if (s->few) {
+    s->R = rows <= 8 ? 8 : kFewRows;
+    s->row_tiles = static_cast<int>((rows + s->R - 1) / s->R);
+    s->count = B;
+    items = static_cast<long long>(B) * Hkv * s->row_tiles;
+  } else {
+    s->R = 128;
+    s->row_tiles = 1;
+    s->rt.G = G;
+    s->rt.n_t = std::min(Tq, 128 / G);
+    s->rt.n_b = 1;
+    s->rt.per_seq = (Tq + s->rt.n_t - 1) / s->rt.n_t;
+    const long long count = static_cast<long long>(B) * s->rt.per_seq;
+    items = count * Hkv;
+    if (items * tiles > (1ll << 30)) return BSATTN_E_SHAPE;
+    s->rt.count = s->count = static_cast<int>(count);
+  }
+  if (items * tiles > (1ll << 30)) return BSATTN_E_SHAPE;
+  s->pieces = static_cast<int>(std::min<long long>(sms, items * tiles));
+  s->slots = s->all_partial ? items + s->pieces : 2ll * s->pieces;
+  s->tiles_p = s->pieces_p = 0;
+  s->slots_p = 0;
+  if (s->prefix) {
+    s->rt.G = G;
+    s->rt.n_t = Tq;
+    s->rt.n_b = std::min(B, 128 / s->rows);
+    s->rt.per_seq = 1;
+    s->rt.count = (B + s->rt.n_b - 1) / s->rt.n_b;
+    s->tiles_p = (prefix_len + kTileKeys - 1) / kTileKeys;
+    const long long items_p = static_cast<long long>(s->rt.count) * Hkv;
+    if (items_p * s->tiles_p > (1ll << 30)) return BSATTN_E_SHAPE;
+    s->pieces_p = static_cast<int>(std::min<long long>(sms, items_p * s->tiles_p));
+    s->slots_p = items_p + s->pieces_p;
+  }
+  if (s->slots * s->R > (1ll << 31) - 1 || s->slots_p * 128 > (1ll << 31) - 1) return BSATTN_E_SHAPE;
+  size_t at = 0;
+  auto take = [&](long long n) {
+    const size_t here = at;
+    at += (static_cast<size_t>(n) * sizeof(float) + 255) / 256 * 256;
+    return here;
+  };
+  s->cum = take(s->count + 1);
+  s->part_o = take(s->slots * s->R * kHeadDim);
+  s->part_l = take(s->slots * s->R);
+  s->cum_p = take(s->prefix ? s->rt.count + 1 : 0);
+  s->pre_o = take(s->slots_p * 128 * kHeadDim);
+  s->pre_l = take(s->slots_p * 128);
+  s->bytes = at;
   return BSATTN_OK;
 }
 
-static int launch_paged(const void* q, const Cache& cache, const Rule& rule, int Hq, float scale,
-                        int dtype_flags, int page_size, void* o, float* lse, void* scratch,
-                        size_t scratch_bytes, cudaStream_t stream) {
+// A launch that may start while its predecessor still runs.
+template <class P>
+static bool launch_overlapped(void (*kernel)(P), unsigned grid, int threads, size_t smem,
+                              cudaStream_t stream, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess) return true;
+  cudaGetLastError();
+  return false;
+}
+
+static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix_len, int Hq,
+                        float scale, int dtype_flags, int page_size, void* o, float* lse,
+                        void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   if (!q || !o) return BSATTN_E_NULL;
   if ((dtype_flags & ~(BSATTN_OUT_BF16 | BSATTN_IN_BF16)) != 0) return BSATTN_E_DTYPE;
   if ((reinterpret_cast<uintptr_t>(q) & 15u) != 0 || (reinterpret_cast<uintptr_t>(o) & 15u) != 0 ||
@@ -577,47 +719,91 @@ static int launch_paged(const void* q, const Cache& cache, const Rule& rule, int
   int rc = device_sms(&sms);
   if (rc != BSATTN_OK) return rc;
   Shape s;
-  rc = shape_of(cache.B, Hq, cache.Hkv, cache.Tq, cache.max_pages, page_size, sms, &s);
+  rc = shape_of(cache.B, Hq, cache.Hkv, cache.Tq, cache.max_pages, page_size, prefix_len, sms, &s);
   if (rc != BSATTN_OK) return rc;
   if (!scratch || scratch_bytes < s.bytes) return BSATTN_E_WORKSPACE;
-  AttnParams p;
-  p.c = cache;
-  p.rule = rule;
-  p.q = q;
-  p.o = o;
-  p.lse = lse;
-  p.G = Hq / cache.Hkv;
-  p.rows = s.rows;
-  p.row_tiles = s.row_tiles;
+  char* const base = static_cast<char*>(scratch);
   const double sc = scale > 0.0f ? static_cast<double>(scale) : 0.08838834764831845;
-  p.scale_log2 = static_cast<float>(sc * 1.4426950408889634);
-  p.out_bf16 = (dtype_flags & BSATTN_OUT_BF16) != 0;
-  p.cum = static_cast<int*>(scratch);
-  p.part_o = reinterpret_cast<float*>(static_cast<char*>(scratch) + s.cum_bytes);
-  p.part_l = p.part_o + s.slots * s.R * kHeadDim;
   const bool bf16 = (dtype_flags & BSATTN_IN_BF16) != 0;
-  const unsigned grid = static_cast<unsigned>(s.pieces);
-  if (s.R == 8) {
-    if (bf16) decode_kernel<true, 1><<<grid, kThreadsD, sizeof(DecodeSmem<1>), stream>>>(p);
-    else decode_kernel<false, 1><<<grid, kThreadsD, sizeof(DecodeSmem<1>), stream>>>(p);
-  } else {
-    if (bf16) decode_kernel<true, 2><<<grid, kThreadsD, sizeof(DecodeSmem<2>), stream>>>(p);
-    else decode_kernel<false, 2><<<grid, kThreadsD, sizeof(DecodeSmem<2>), stream>>>(p);
+  const int out_bf16 = (dtype_flags & BSATTN_OUT_BF16) != 0;
+  const float scale_log2 = static_cast<float>(sc * 1.4426950408889634);
+  rule.k0 = s.k0;
+
+  if (s.prefix || !s.few) {
+    TileCall t;
+    t.c = cache;
+    t.rule = rule;
+    t.rule.k0 = 0;
+    t.rt = s.rt;
+    t.prefix_len = s.prefix ? prefix_len : 0;
+    t.q = q;
+    t.o = o;
+    t.lse = lse;
+    t.Hq = Hq;
+    t.scale_log2 = scale_log2;
+    t.in_bf16 = bf16;
+    t.out_bf16 = out_bf16;
+    t.pieces = s.prefix ? s.pieces_p : s.pieces;
+    t.slots = s.prefix ? s.slots_p : s.slots;
+    t.cum = reinterpret_cast<int*>(base + (s.prefix ? s.cum_p : s.cum));
+    t.part_o = reinterpret_cast<float*>(base + (s.prefix ? s.pre_o : s.part_o));
+    t.part_l = reinterpret_cast<float*>(base + (s.prefix ? s.pre_l : s.part_l));
+    if ((rc = tile_launch(t, page_size, stream)) != BSATTN_OK) return rc;
   }
-  if (cudaGetLastError() != cudaSuccess) return BSATTN_E_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long long>(cache.B) * cache.Hkv * s.rows));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, join_kernel, p, s.pieces, s.R) != cudaSuccess) {
-    cudaGetLastError();
-    return BSATTN_E_CUDA;
+  if (s.few) {
+    AttnParams p;
+    p.c = cache;
+    p.rule = rule;
+    p.q = q;
+    p.o = o;
+    p.lse = lse;
+    p.rows = s.rows;
+    p.row_tiles = s.row_tiles;
+    p.scale_log2 = scale_log2;
+    p.out_bf16 = out_bf16;
+    p.all_partial = s.all_partial;
+    p.cum = reinterpret_cast<int*>(base + s.cum);
+    p.part_o = reinterpret_cast<float*>(base + s.part_o);
+    p.part_l = reinterpret_cast<float*>(base + s.part_l);
+    const unsigned grid = static_cast<unsigned>(s.pieces);
+    void (*kernel)(AttnParams) = s.R == 8 ? (bf16 ? decode_kernel<true, 1> : decode_kernel<false, 1>)
+                                          : (bf16 ? decode_kernel<true, 2> : decode_kernel<false, 2>);
+    const size_t smem = s.R == 8 ? sizeof(DecodeSmem<1>) : sizeof(DecodeSmem<2>);
+    if (s.prefix) {
+      if (!launch_overlapped(kernel, grid, kThreadsD, smem, stream, p)) return BSATTN_E_CUDA;
+    } else {
+      kernel<<<grid, kThreadsD, smem, stream>>>(p);
+      if (cudaGetLastError() != cudaSuccess) return BSATTN_E_CUDA;
+    }
   }
+  JoinParams j;
+  j.Hkv = cache.Hkv;
+  j.G = Hq / cache.Hkv;
+  j.Tq = cache.Tq;
+  j.o = o;
+  j.lse = lse;
+  j.out_bf16 = out_bf16;
+  j.cum = reinterpret_cast<const int*>(base + s.cum);
+  j.part_o = reinterpret_cast<const float*>(base + s.part_o);
+  j.part_l = reinterpret_cast<const float*>(base + s.part_l);
+  j.count = s.count;
+  j.pieces = s.pieces;
+  j.R = s.R;
+  j.row_tiles = s.row_tiles;
+  j.all_partial = s.all_partial;
+  j.n_t = s.few ? 0 : s.rt.n_t;
+  j.per_seq = s.few ? 1 : s.rt.per_seq;
+  j.pre_o = reinterpret_cast<const float*>(base + s.pre_o);
+  j.pre_l = reinterpret_cast<const float*>(base + s.pre_l);
+  j.n_b = s.prefix ? s.rt.n_b : 1;
+  j.tiles_p = s.tiles_p;
+  j.quota_p = 1;
+  if (s.prefix) {
+    const long long line = static_cast<long long>(s.rt.count) * cache.Hkv * s.tiles_p;
+    j.quota_p = static_cast<int>((line + s.pieces_p - 1) / s.pieces_p);
+  }
+  const unsigned rows = static_cast<unsigned>(static_cast<long long>(cache.B) * Hq * cache.Tq);
+  if (!launch_overlapped(join_kernel, rows, kJoinWarps * 32, 0, stream, j)) return BSATTN_E_CUDA;
   return BSATTN_OK;
 }
 
@@ -639,7 +825,7 @@ int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages, in
   int rc = device_sms(&sms);
   if (rc != BSATTN_OK) return rc;
   Shape s;
-  rc = shape_of(B, Hq, Hkv, Tq, max_pages, page_size, sms, &s);
+  rc = shape_of(B, Hq, Hkv, Tq, max_pages, page_size, prefix_len, sms, &s);
   if (rc != BSATTN_OK) return rc;
   *bytes = s.bytes;
   return BSATTN_OK;
@@ -669,7 +855,7 @@ int bsattn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
   rule.k0 = 0;
   rule.window = window;
   rule.glob = global_blocks;
-  return launch_paged(q, c, rule, Hq, scale, dtype_flags, page_size, o, lse, scratch,
+  return launch_paged(q, c, rule, prefix_len, Hq, scale, dtype_flags, page_size, o, lse, scratch,
                       scratch_bytes, static_cast<cudaStream_t>(stream));
 }
 

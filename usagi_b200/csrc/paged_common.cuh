@@ -11,6 +11,10 @@
 #include "../../include/bsattn.h"
 
 namespace bsattn {
+
+unsigned long long launch_timeout_ns();  // bsattn_set_timeout_ns
+int launch_test_wait();                  // bsattn_test_unsignalled_wait
+
 namespace paged {
 
 constexpr int kHeadDim = 128;
