@@ -207,58 +207,59 @@ BSATTN_API int bsattn_peer_copy(void* dst, const void* src, size_t bytes, void* 
 
 /* ---- Paged K/V cache: new tokens into it, and their attention over it -------------------------
  * No counterpart in the reference, which stops at prefill.  A cache holds the keys and values of B
- * sequences in pages of page_size tokens (a power of two, 16 .. 1024):
- *   k_pages, v_pages  fp16 or bf16 [n_pages, Hkv, page_size, 128]; page_strides[6] = elements
- *                     between pages, heads and tokens of k_pages, then of v_pages (multiples of 8;
- *                     16-byte aligned bases; the 128 values of a token and head are contiguous)
- *   block_table       int32, sequence b's page of tokens n * page_size .. is
- *                     block_table[b * table_stride + n], n < max_pages; entries behind a sequence's
- *                     length are not read
- *   seq_lens          int32 [B]: tokens of each sequence, the new ones of this call included
- *   q_lens            int32 [B] or NULL: live rows of each sequence, 0 .. Tq; NULL: Tq for all
- * Row t < q_lens[b] of sequence b is the token at position seq_lens[b] - q_lens[b] + t; rows behind
- * them are padding, and a row whose position is negative is dead like them.
+ * sequences in pages of page_size tokens.  Row t < q_lens[b] of sequence b is the token at position
+ * seq_lens[b] - q_lens[b] + t; the rows behind them are padding, and a row whose position is negative
+ * is dead like them.
  * A page table entry outside [0, n_pages), a length outside the table or a live row count outside
  * [0, Tq] is reported as BSATTN_E_PAGE through bsattn_check_error and never used as an address:
  * the length or count is forced into range, the entry's tokens are not written, and are read as
- * zeros.  Slots that hold no token of a sequence are never used, whatever their bits are.
- *
- * bsattn_paged_append writes the live rows of k and v [B, Hkv, Tq, 128] into their slots and leaves
- * every other slot as it was.  With inv_freq (rot_dim / 2 doubles on the device, rot_dim a multiple
- * of 16 up to 128) the first rot_dim values of each row of k, and of q [B, Hq, Tq, 128] on its way
- * to q_out (contiguous; zero in padding rows), are turned: pair i = (x_i, x_{i + rot_dim/2}), or
- * (x_2i, x_{2i+1}) when interleaved, by position * inv_freq[i].  inv_freq NULL: no rotation.  Hq == 0:
- * no q.  q_out may be q itself when q is contiguous.  in_strides[9] = elements between batches, heads
- * and tokens of q, k, v.  dtype_flags: BSATTN_IN_BF16 or 0, the type of everything.  Two rows of one
- * call in the same slot (a page in two places of the table) leave one of them there.
- *
- * bsattn_paged_fwd is the attention of the live rows over the cache, the new tokens included:
- * o [B, Hq, Tq, 128] (contiguous, like q) and lse [B, Hq, Tq] (or NULL), each group of Hq / Hkv query
- * heads on one K/V head, keys at positions up to the row's own.  window > 0 keeps, for a row in block
- * i = position / 128, the keys of blocks < global_blocks and > i - window: the rows that
- * bsattn_fwd_window computes.  prefix_len > 0 (a multiple of page_size; without a window) says that the
- * first prefix_len tokens of every sequence are the same pages, those of sequence 0: they are read
- * once for the whole batch.  The result is that of prefix_len == 0.  Dead rows and rows without keys
- * get o = 0 and lse = -inf.  scratch: bsattn_paged_scratch_bytes bytes of device memory, 16-byte
- * aligned, any content, used by this call only. */
-BSATTN_API int bsattn_paged_append(void* k_pages, void* v_pages, const int64_t* page_strides,
-                                   const int32_t* block_table, int64_t table_stride, int max_pages,
-                                   int n_pages, int page_size, const int32_t* seq_lens,
-                                   const int32_t* q_lens, const void* q, const void* k,
+ * zeros.  Slots that hold no token of a sequence are never used, whatever their bits are. */
+typedef struct bsattn_paged_call {
+  void* k_pages;              /* fp16 or bf16 [n_pages, Hkv, page_size, 128], 16-byte aligned      */
+  void* v_pages;
+  int64_t page_strides[6];    /* elements between pages, heads, tokens of k_pages, then of v_pages:
+                                 multiples of 8, positive where the dimension is not 1; the 128
+                                 values of a token and head are contiguous                         */
+  const int32_t* block_table; /* tokens n * page_size .. of sequence b: page [b * table_stride + n];
+                                 entries behind a sequence's length are not read                   */
+  int64_t table_stride;
+  const int32_t* seq_lens;    /* [B] tokens of each sequence, the new ones of this call included   */
+  const int32_t* q_lens;      /* [B] live rows of each sequence, 0 .. Tq; NULL: Tq for all         */
+  int32_t max_pages;          /* entries of a table row                                            */
+  int32_t n_pages;
+  int32_t page_size;          /* a power of two, 16 .. 1024                                        */
+  int32_t B, Hq, Hkv, Tq;
+  int32_t dtype_flags;        /* BSATTN_IN_BF16: pages and rows are bf16; BSATTN_OUT_BF16: o       */
+  void* workspace;            /* as for bsattn_fwd                                                 */
+  size_t workspace_bytes;
+  void* stream;
+} bsattn_paged_call;
+
+/* Writes the live rows of k and v [B, Hkv, Tq, 128] into their slots and leaves every other slot as it
+ * was.  With inv_freq (rot_dim / 2 doubles on the device, rot_dim a multiple of 16 up to 128) the first
+ * rot_dim values of each row of k, and of q [B, Hq, Tq, 128] on its way to q_out (contiguous; zero in
+ * padding rows), are turned: pair i = (x_i, x_{i + rot_dim/2}), or (x_2i, x_{2i+1}) when interleaved, by
+ * position * inv_freq[i].  inv_freq NULL: no rotation.  Hq == 0: no q.  q_out may be q itself when q is
+ * contiguous.  in_strides[9] (host) = elements between batches, heads and tokens of q, k, v.  Two rows
+ * of one call in the same slot (a page in two places of the table) leave one of them there. */
+BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q, const void* k,
                                    const void* v, const int64_t* in_strides, void* q_out,
-                                   const double* inv_freq, int rot_dim, int interleaved, int B,
-                                   int Hq, int Hkv, int Tq, int dtype_flags, void* workspace,
-                                   size_t workspace_bytes, void* stream);
+                                   const double* inv_freq, int rot_dim, int interleaved);
+
+/* Attention of the live rows over the cache, the new tokens included: o [B, Hq, Tq, 128] (contiguous,
+ * like q) and lse [B, Hq, Tq] (or NULL), each group of Hq / Hkv query heads on one K/V head, keys at
+ * positions up to the row's own.  window > 0 keeps, for a row in block i = position / 128, the keys of
+ * blocks < global_blocks and > i - window: the rows that bsattn_fwd_window computes.  prefix_len > 0 (a
+ * multiple of page_size; without a window) says that the first prefix_len tokens of every sequence are
+ * the same pages, those of sequence 0's table row: they may be read once for the whole batch.  The
+ * result is that of prefix_len == 0.  Dead rows and rows without keys get o = 0 and lse = -inf.
+ * scratch: bsattn_paged_scratch_bytes bytes of device memory, 16-byte aligned, any content, used by
+ * this call only. */
 BSATTN_API int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages,
                                           int page_size, int prefix_len, size_t* bytes);
-BSATTN_API int bsattn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
-                                const int64_t* page_strides, const int32_t* block_table,
-                                int64_t table_stride, int max_pages, int n_pages, int page_size,
-                                const int32_t* seq_lens, const int32_t* q_lens, void* o, float* lse,
-                                int B, int Hq, int Hkv, int Tq, int window, int global_blocks,
-                                int prefix_len, float scale, int dtype_flags, void* scratch,
-                                size_t scratch_bytes, void* workspace, size_t workspace_bytes,
-                                void* stream);
+BSATTN_API int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, float* lse,
+                                int window, int global_blocks, int prefix_len, float scale,
+                                void* scratch, size_t scratch_bytes);
 
 /* Human-readable text for a BSATTN_E* code. */
 BSATTN_API const char* bsattn_strerror(int code);

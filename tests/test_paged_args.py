@@ -8,40 +8,43 @@ import torch
 import usagi_b200 as ub
 from usagi_b200 import _lib
 
-S6 = (ctypes.c_int64 * 6)(*([128] * 6))
+def _record(a):
+    return _lib.PAGED_CALL.pack(a["kp"], a["vp"], *a["st"], a["table"], a["ts"], a["sl"], a["ql"],
+                                a["mp"], a["np"], a["ps"], a["B"], a["Hq"], a["Hkv"], a["Tq"],
+                                a["flags"], a["ws"], a["wsb"], 0)
+
+
+CACHE = dict(kp=16, vp=16, st=[128] * 6, table=16, ts=4, mp=4, np=8, ps=16, sl=16, ql=0, B=1, Hq=2,
+             Hkv=1, Tq=1, flags=0, ws=16, wsb=256)
 
 
 def _fwd(**kw):
-    a = dict(q=16, kp=16, vp=16, st=S6, table=16, ts=4, mp=4, np=8, ps=16, sl=16, ql=None, o=16,
-             lse=None, B=1, Hq=2, Hkv=1, Tq=1, window=0, glob=0, prefix=0, flags=0, ws=16, wsb=256)
+    a = dict(CACHE, q=16, o=16, lse=None, window=0, glob=0, prefix=0)
     a.update(kw)
-    return _lib.load().bsattn_paged_fwd(
-        a["q"], a["kp"], a["vp"], a["st"], a["table"], a["ts"], a["mp"], a["np"], a["ps"], a["sl"],
-        a["ql"], a["o"], a["lse"], a["B"], a["Hq"], a["Hkv"], a["Tq"], a["window"], a["glob"],
-        a["prefix"], 0.0, a["flags"], 16, 1 << 20, a["ws"], a["wsb"], None)
+    return _lib.load().bsattn_paged_fwd(_record(a), a["q"], a["o"], a["lse"], a["window"],
+                                        a["glob"], a["prefix"], 0.0, 16, 1 << 20)
 
 
 def _append(**kw):
-    a = dict(kp=16, vp=16, st=S6, table=16, ts=4, mp=4, np=8, ps=16, sl=16, ql=None, q=16, k=16,
-             v=16, ins=(ctypes.c_int64 * 9)(*([128] * 9)), qo=16, inv=16, rot=128, B=1, Hq=2, Hkv=1,
-             Tq=1, flags=0, ws=16, wsb=256)
+    a = dict(CACHE, q=16, k=16, v=16, ins=[128] * 9, qo=16, inv=16, rot=128)
     a.update(kw)
-    return _lib.load().bsattn_paged_append(
-        a["kp"], a["vp"], a["st"], a["table"], a["ts"], a["mp"], a["np"], a["ps"], a["sl"], a["ql"],
-        a["q"], a["k"], a["v"], a["ins"], a["qo"], a["inv"], a["rot"], 0, a["B"], a["Hq"], a["Hkv"],
-        a["Tq"], a["flags"], a["ws"], a["wsb"], None)
+    ins = None if a["ins"] is None else bytes((ctypes.c_int64 * 9)(*a["ins"]))
+    return _lib.load().bsattn_paged_append(_record(a), a["q"], a["k"], a["v"], ins, a["qo"],
+                                           a["inv"], a["rot"], 0)
 
 
 @pytest.mark.parametrize("call", [_fwd, _append])
 def test_cache_arguments(call):
-    for name in ("kp", "vp", "st", "table", "sl", "q"):
-        assert call(**{name: None}) == _lib.E_NULL, name
+    for name in ("kp", "vp", "table", "sl"):
+        assert call(**{name: 0}) == _lib.E_NULL, name
+    assert call(q=None) == _lib.E_NULL
     for kw in (dict(B=0), dict(Hkv=0), dict(Tq=0), dict(mp=0), dict(np=0), dict(ts=-1),
                dict(ps=8), dict(ps=48), dict(ps=2048), dict(mp=1 << 27)):
         assert call(**kw) == _lib.E_SHAPE, kw
     assert call(kp=24) == _lib.E_ALIGN
-    assert call(st=(ctypes.c_int64 * 6)(128, 128, 132, 128, 128, 128)) == _lib.E_ALIGN
-    assert call(ws=None) == _lib.E_WORKSPACE
+    for bad in (132, 0, -128):
+        assert call(st=[128, 128, bad, 128, 128, 128]) == _lib.E_ALIGN
+    assert call(ws=0) == _lib.E_WORKSPACE
     assert call(wsb=4) == _lib.E_WORKSPACE
 
 
@@ -63,7 +66,13 @@ def test_append_arguments():
     for rot in (0, 8, 24, 144, -16):
         assert _append(rot=rot) == _lib.E_SHAPE, rot
     assert _append(k=24) == _lib.E_ALIGN
-    assert _append(ins=(ctypes.c_int64 * 9)(*([128] * 8 + [100]))) == _lib.E_ALIGN
+    assert _append(ins=[128] * 8 + [100]) == _lib.E_ALIGN
+
+
+def test_null_call_record():
+    lib = _lib.load()
+    assert lib.bsattn_paged_fwd(None, 16, 16, None, 0, 0, 0, 0.0, 16, 1 << 20) == _lib.E_NULL
+    assert lib.bsattn_paged_append(None, 16, 16, 16, bytes(72), 16, None, 0, 0) == _lib.E_NULL
 
 
 def test_error_code_has_a_text():

@@ -5,6 +5,7 @@ There is no fallback: if the library is missing or does not export the ABI, load
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -64,29 +65,17 @@ SIGNATURES = {
     "bsattn_ipc_close": (_c_int, [_c_void_p, ctypes.c_uint64]),
     "bsattn_peer_copy": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),
     "bsattn_paged_append": (_c_int, [
-        _c_void_p, _c_void_p, _c_void_p,          # k_pages, v_pages, page_strides (host int64[6])
-        _c_void_p, ctypes.c_int64, _c_int,        # block_table, table_stride, max_pages
-        _c_int, _c_int,                           # n_pages, page_size
-        _c_void_p, _c_void_p,                     # seq_lens, q_lens
+        ctypes.c_char_p,                          # PAGED_CALL
         _c_void_p, _c_void_p, _c_void_p,          # q, k, v
-        _c_void_p, _c_void_p,                     # in_strides (host int64[9]), q_out
+        ctypes.c_char_p, _c_void_p,               # in_strides (host int64[9]), q_out
         _c_void_p, _c_int, _c_int,                # inv_freq, rot_dim, interleaved
-        _c_int, _c_int, _c_int, _c_int, _c_int,   # B, Hq, Hkv, Tq, dtype_flags
-        _c_void_p, _c_size_t, _c_void_p,          # workspace, bytes, stream
     ]),
     "bsattn_paged_scratch_bytes": (_c_int, [_c_int] * 7 + [ctypes.POINTER(_c_size_t)]),
     "bsattn_paged_fwd": (_c_int, [
-        _c_void_p, _c_void_p, _c_void_p,          # q, k_pages, v_pages
-        _c_void_p,                                # page_strides (host int64[6])
-        _c_void_p, ctypes.c_int64, _c_int,        # block_table, table_stride, max_pages
-        _c_int, _c_int,                           # n_pages, page_size
-        _c_void_p, _c_void_p,                     # seq_lens, q_lens
-        _c_void_p, _c_void_p,                     # o, lse
-        _c_int, _c_int, _c_int, _c_int,           # B, Hq, Hkv, Tq
-        _c_int, _c_int, _c_int,                   # window, global_blocks, prefix_len
-        ctypes.c_float, _c_int,                   # scale, dtype_flags
+        ctypes.c_char_p,                          # PAGED_CALL
+        _c_void_p, _c_void_p, _c_void_p,          # q, o, lse
+        _c_int, _c_int, _c_int, ctypes.c_float,   # window, global_blocks, prefix_len, scale
         _c_void_p, _c_size_t,                     # scratch, bytes
-        _c_void_p, _c_size_t, _c_void_p,          # workspace, bytes, stream
     ]),
     "bsattn_fwd_noalloc": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p,          # q, k, v
@@ -98,6 +87,10 @@ SIGNATURES = {
         _c_void_p, _c_void_p,                     # status (device or pinned host int*), stream
     ]),
 }
+
+# bsattn_paged_call: k_pages, v_pages, page_strides[6], block_table, table_stride, seq_lens, q_lens,
+# max_pages, n_pages, page_size, B, Hq, Hkv, Tq, dtype_flags, workspace, workspace_bytes, stream
+PAGED_CALL = struct.Struct("@PP6qPqPP8iPNP")
 
 # error codes (include/bsattn.h)
 OK = 0

@@ -167,21 +167,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 using namespace bsattn;
 using namespace bsattn::paged;
 
-extern "C" int bsattn_paged_append(void* k_pages, void* v_pages, const int64_t* page_strides,
-                                   const int32_t* block_table, int64_t table_stride, int max_pages,
-                                   int n_pages, int page_size, const int32_t* seq_lens,
-                                   const int32_t* q_lens, const void* q, const void* k,
+extern "C" int bsattn_paged_append(const bsattn_paged_call* call, const void* q, const void* k,
                                    const void* v, const int64_t* in_strides, void* q_out,
-                                   const double* inv_freq, int rot_dim, int interleaved, int B,
-                                   int Hq, int Hkv, int Tq, int dtype_flags, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+                                   const double* inv_freq, int rot_dim, int interleaved) {
   AppendParams p;
-  int rc = fill_cache(&p.c, k_pages, v_pages, page_strides, block_table, table_stride, max_pages,
-                      n_pages, page_size, seq_lens, q_lens, B, Hkv, Tq, workspace,
-                      workspace_bytes);
+  int rc = fill_cache(&p.c, call);
   if (rc != BSATTN_OK) return rc;
-  if (!k || !v || !in_strides || Hq < 0 || (Hq > 0 && (!q || !q_out))) return BSATTN_E_NULL;
-  if ((dtype_flags & ~BSATTN_IN_BF16) != 0) return BSATTN_E_DTYPE;
+  const int B = call->B, Hq = call->Hq, Hkv = call->Hkv, Tq = call->Tq;
+  if (Hq < 0) return BSATTN_E_SHAPE;
+  if (!k || !v || !in_strides || (Hq > 0 && (!q || !q_out))) return BSATTN_E_NULL;
+  if ((call->dtype_flags & ~BSATTN_IN_BF16) != 0) return BSATTN_E_DTYPE;
   if (inv_freq == nullptr) rot_dim = 0;
   if (rot_dim < 0 || rot_dim > kHeadDim || rot_dim % 16 != 0 || (inv_freq && rot_dim == 0) ||
       (reinterpret_cast<uintptr_t>(inv_freq) & 7u) != 0)
@@ -199,8 +194,8 @@ extern "C" int bsattn_paged_append(void* k_pages, void* v_pages, const int64_t* 
   if (heads > 65535 || tokens > (1ll << 31) - 2) return BSATTN_E_SHAPE;
   int sms = 0;
   if ((rc = device_sms(&sms)) != BSATTN_OK) return rc;
-  p.k_pages = static_cast<char*>(k_pages);
-  p.v_pages = static_cast<char*>(v_pages);
+  p.k_pages = static_cast<char*>(call->k_pages);
+  p.v_pages = static_cast<char*>(call->v_pages);
   p.q = static_cast<const char*>(q);
   p.k = static_cast<const char*>(k);
   p.v = static_cast<const char*>(v);
@@ -216,8 +211,8 @@ extern "C" int bsattn_paged_append(void* k_pages, void* v_pages, const int64_t* 
   p.heads_per_block = static_cast<int>((heads + split - 1) / split);
   const dim3 grid(static_cast<unsigned>(bx),
                   static_cast<unsigned>((heads + p.heads_per_block - 1) / p.heads_per_block));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype_flags & BSATTN_IN_BF16)
+  cudaStream_t s = static_cast<cudaStream_t>(call->stream);
+  if (call->dtype_flags & BSATTN_IN_BF16)
     append_kernel<true><<<grid, kAppendThreads, 0, s>>>(p);
   else
     append_kernel<false><<<grid, kAppendThreads, 0, s>>>(p);

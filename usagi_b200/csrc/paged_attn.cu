@@ -566,43 +566,43 @@ int device_sms(int* sms) {
   return BSATTN_OK;
 }
 
-int fill_cache(Cache* c, const void* k_pages, const void* v_pages, const int64_t* page_strides,
-               const int32_t* block_table, int64_t table_stride, int max_pages, int n_pages,
-               int page_size, const int32_t* seq_lens, const int32_t* q_lens, int B, int Hkv,
-               int Tq, void* workspace, size_t workspace_bytes) {
-  if (!k_pages || !v_pages || !page_strides || !block_table || !seq_lens) return BSATTN_E_NULL;
-  if (B < 1 || Hkv < 1 || Tq < 1 || max_pages < 1 || n_pages < 1 || table_stride < 0)
+int fill_cache(Cache* c, const bsattn_paged_call* a) {
+  if (!a || !a->k_pages || !a->v_pages || !a->block_table || !a->seq_lens) return BSATTN_E_NULL;
+  if (a->B < 1 || a->Hkv < 1 || a->Tq < 1 || a->max_pages < 1 || a->n_pages < 1 || a->table_stride < 0)
     return BSATTN_E_SHAPE;
-  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0)
+  if (a->page_size < 16 || a->page_size > 1024 || (a->page_size & (a->page_size - 1)) != 0)
     return BSATTN_E_SHAPE;
-  if (static_cast<long long>(max_pages) * page_size > (1ll << 31) - 2 * kTileKeys)
+  if (static_cast<long long>(a->max_pages) * a->page_size > (1ll << 31) - 2 * kTileKeys)
     return BSATTN_E_SHAPE;
-  if (!workspace || workspace_bytes < bsattn_workspace_bytes()) return BSATTN_E_WORKSPACE;
-  if ((reinterpret_cast<uintptr_t>(k_pages) & 15u) != 0 ||
-      (reinterpret_cast<uintptr_t>(v_pages) & 15u) != 0)
+  if (!a->workspace || a->workspace_bytes < bsattn_workspace_bytes()) return BSATTN_E_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(a->k_pages) & 15u) != 0 ||
+      (reinterpret_cast<uintptr_t>(a->v_pages) & 15u) != 0)
     return BSATTN_E_ALIGN;
-  for (int i = 0; i < 6; ++i)
-    if (page_strides[i] < 0 || page_strides[i] % 8 != 0) return BSATTN_E_ALIGN;
-  c->k = static_cast<const char*>(k_pages);
-  c->v = static_cast<const char*>(v_pages);
-  c->k_page = page_strides[0] * 2;
-  c->k_head = page_strides[1] * 2;
-  c->k_tok = page_strides[2] * 2;
-  c->v_page = page_strides[3] * 2;
-  c->v_head = page_strides[4] * 2;
-  c->v_tok = page_strides[5] * 2;
-  c->table = block_table;
-  c->table_stride = table_stride;
-  c->seq_lens = seq_lens;
-  c->q_lens = q_lens;
-  c->max_pages = max_pages;
-  c->n_pages = n_pages;
+  const int dims[3] = {a->n_pages, a->Hkv, a->page_size};
+  for (int i = 0; i < 6; ++i) {
+    const int64_t st = a->page_strides[i];
+    if (st < 0 || st % 8 != 0 || (st == 0 && dims[i % 3] > 1)) return BSATTN_E_ALIGN;
+  }
+  c->k = static_cast<const char*>(a->k_pages);
+  c->v = static_cast<const char*>(a->v_pages);
+  c->k_page = a->page_strides[0] * 2;
+  c->k_head = a->page_strides[1] * 2;
+  c->k_tok = a->page_strides[2] * 2;
+  c->v_page = a->page_strides[3] * 2;
+  c->v_head = a->page_strides[4] * 2;
+  c->v_tok = a->page_strides[5] * 2;
+  c->table = a->block_table;
+  c->table_stride = a->table_stride;
+  c->seq_lens = a->seq_lens;
+  c->q_lens = a->q_lens;
+  c->max_pages = a->max_pages;
+  c->n_pages = a->n_pages;
   c->page_shift = 0;
-  while ((1 << c->page_shift) < page_size) ++c->page_shift;
-  c->B = B;
-  c->Hkv = Hkv;
-  c->Tq = Tq;
-  c->err = static_cast<int*>(workspace);
+  while ((1 << c->page_shift) < a->page_size) ++c->page_shift;
+  c->B = a->B;
+  c->Hkv = a->Hkv;
+  c->Tq = a->Tq;
+  c->err = static_cast<int*>(a->workspace);
   return BSATTN_OK;
 }
 
@@ -831,32 +831,23 @@ int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages, in
   return BSATTN_OK;
 }
 
-int bsattn_paged_fwd(const void* q, const void* k_pages, const void* v_pages,
-                     const int64_t* page_strides, const int32_t* block_table, int64_t table_stride,
-                     int max_pages, int n_pages, int page_size, const int32_t* seq_lens,
-                     const int32_t* q_lens, void* o, float* lse, int B, int Hq, int Hkv, int Tq,
-                     int window, int global_blocks, int prefix_len, float scale, int dtype_flags,
-                     void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes,
-                     void* stream) {
+int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, float* lse, int window,
+                     int global_blocks, int prefix_len, float scale, void* scratch,
+                     size_t scratch_bytes) {
   Cache c;
-  const int rc = fill_cache(&c, k_pages, v_pages, page_strides, block_table, table_stride,
-                            max_pages, n_pages, page_size, seq_lens, q_lens, B, Hkv, Tq, workspace,
-                            workspace_bytes);
+  const int rc = fill_cache(&c, call);
   if (rc != BSATTN_OK) return rc;
   constexpr int kMaxWindow = 1 << 24;
   if (window < 0 || window > kMaxWindow || global_blocks < 0 || global_blocks > kMaxWindow ||
       (window == 0 && global_blocks != 0))
     return BSATTN_E_SHAPE;
-  if (prefix_len < 0 || prefix_len % page_size != 0 ||
-      static_cast<long long>(prefix_len) > static_cast<long long>(max_pages) * page_size ||
+  if (prefix_len < 0 || prefix_len % call->page_size != 0 ||
+      prefix_len > static_cast<long long>(call->max_pages) * call->page_size ||
       (prefix_len > 0 && window > 0))
     return BSATTN_E_SHAPE;
-  Rule rule;
-  rule.k0 = 0;
-  rule.window = window;
-  rule.glob = global_blocks;
-  return launch_paged(q, c, rule, prefix_len, Hq, scale, dtype_flags, page_size, o, lse, scratch,
-                      scratch_bytes, static_cast<cudaStream_t>(stream));
+  const Rule rule{0, window, global_blocks};
+  return launch_paged(q, c, rule, prefix_len, call->Hq, scale, call->dtype_flags, call->page_size, o,
+                      lse, scratch, scratch_bytes, static_cast<cudaStream_t>(call->stream));
 }
 
 }  // extern "C"

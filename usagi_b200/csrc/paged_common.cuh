@@ -187,11 +187,8 @@ __device__ __forceinline__ void pdl_wait() {
 // Number of SMs of the current device (checked to be sm_100).
 int device_sms(int* sms);
 
-// Checks and fills the cache view of a call (paged_attn.cu).
-int fill_cache(Cache* c, const void* k_pages, const void* v_pages, const int64_t* page_strides,
-               const int32_t* block_table, int64_t table_stride, int max_pages, int n_pages,
-               int page_size, const int32_t* seq_lens, const int32_t* q_lens, int B, int Hkv,
-               int Tq, void* workspace, size_t workspace_bytes);
+// Checks a call and fills the kernels' view of its cache (paged_attn.cu).
+int fill_cache(Cache* c, const bsattn_paged_call* call);
 
 }  // namespace paged
 }  // namespace bsattn

@@ -26,6 +26,8 @@ address, and raised by :func:`usagi_b200.check_errors` (code ``E_PAGE``).
 from __future__ import annotations
 
 import ctypes
+import struct
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -35,8 +37,11 @@ from .api import HEAD_DIM, BsattnError, _workspace
 
 __all__ = ["paged_kv_append", "paged_attn_fwd", "shared_prefix_attn_fwd", "rope_inv_freq"]
 
-_Strides6 = ctypes.c_int64 * 6
-_Strides9 = ctypes.c_int64 * 9
+# A decode step is a few microseconds of GPU time, so the host side is kept short: the call record
+# is packed in one go, and the current device and stream are asked for without wrapper objects.
+_PACK = _lib.PAGED_CALL.pack
+_STRIDES9 = struct.Struct("@9q").pack
+_HALF = (torch.float16, torch.bfloat16)
 
 
 def rope_inv_freq(rot_dim: int = HEAD_DIM, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -46,80 +51,77 @@ def rope_inv_freq(rot_dim: int = HEAD_DIM, base: float = 10000.0, device="cuda")
 
 
 def _index(t: torch.Tensor, name: str, dev, shape) -> torch.Tensor:
-    """``t`` as int32 on ``dev``; ``shape`` is its expected shape (-1: any)."""
-    if t.dim() != len(shape) or any(n not in (-1, m) for n, m in zip(shape, t.shape)):
+    """``t`` as int32 on ``dev`` with a contiguous last dimension."""
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != torch.int32 or t.device != dev:
         t = t.to(device=dev, dtype=torch.int32)
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         t = t.contiguous()
     return t
 
 
-def _rows(t: torch.Tensor, name: str, dev, dtype) -> torch.Tensor:
-    """A [B, H, T, 128] input as the kernels read it in place: 16-byte rows and strides."""
-    if t.dim() != 4 or t.shape[3] != HEAD_DIM:
-        raise ValueError(f"{name} must be [B, H, T, {HEAD_DIM}], got {tuple(t.shape)}")
+def _rows(t: torch.Tensor, name: str, dev, dtype, shape):
+    """A [B, H, T, 128] input as the kernels read it in place (16-byte rows and strides), and its
+    strides."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype != dtype or t.device != dev:
         raise TypeError(f"{name} must be {dtype} on {dev} like the pages, got {t.dtype} on "
                         f"{t.device}")
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
+    st = t.stride()
+    if st[3] != 1 or (st[0] | st[1] | st[2]) & 7 or t.data_ptr() & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
-    return t
+        st = t.stride()
+    return t, st
 
 
-class _Call:
-    """The checked cache arguments of one call, in the order of the C ABI."""
+def _cache(k_pages, v_pages, block_table, seq_lens, q_lens, B):
+    """Checks of the cache arguments: (device, dtype, Hkv, max_pages, page_size, first fields of the
+    call record, tensors to keep until the launch)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM or v_pages.shape != shape:
+        raise ValueError(f"k_pages and v_pages must be [n_pages, Hkv, page_size, {HEAD_DIM}] of one "
+                         f"shape, got {tuple(shape)}, {tuple(v_pages.shape)}")
+    dev, dtype = k_pages.device, k_pages.dtype
+    if dtype not in _HALF or v_pages.dtype != dtype:
+        raise TypeError("k_pages and v_pages must both be float16 or both bfloat16, got "
+                        f"{dtype}, {v_pages.dtype}")
+    if dev.type != "cuda" or v_pages.device != dev:
+        raise ValueError("the paged cache needs CUDA tensors on one device (there is no CPU path)")
+    n_pages, Hkv, page_size, _ = shape
+    if n_pages == 0 or Hkv == 0:
+        raise ValueError(f"the cache has no pages or no heads: {tuple(shape)}")
+    if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if k3 != 1 or v3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & 7 or (kp | vp) & 15:
+        raise ValueError("k_pages and v_pages must be 16-byte aligned, with a contiguous last "
+                         "dimension and strides that are multiples of 8")
+    if block_table.dim() != 2 or block_table.shape[1] == 0:
+        raise ValueError(f"block_table must be [B, max_pages], got {tuple(block_table.shape)}")
+    max_pages = block_table.shape[1]
+    table = _index(block_table, "block_table", dev, (B, max_pages))
+    sl = _index(seq_lens, "seq_lens", dev, (B,))
+    ql = None if q_lens is None else _index(q_lens, "q_lens", dev, (B,))
+    head = (kp, vp, k0, k1, k2, v0, v1, v2, table.data_ptr(), table.stride(0), sl.data_ptr(),
+            0 if ql is None else ql.data_ptr(), max_pages, n_pages, page_size, B)
+    return dev, dtype, Hkv, max_pages, page_size, head, (table, sl, ql)
 
-    __slots__ = ("dev", "dtype", "B", "Hkv", "head", "lens", "keep", "max_pages", "page_size")
 
-    def __init__(self, k_pages, v_pages, block_table, seq_lens, q_lens, B):
-        if k_pages.dim() != 4 or k_pages.shape[3] != HEAD_DIM or v_pages.shape != k_pages.shape:
-            raise ValueError(f"k_pages and v_pages must be [n_pages, Hkv, page_size, {HEAD_DIM}] of "
-                             f"one shape, got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
-        dev, dtype = k_pages.device, k_pages.dtype
-        if dtype not in (torch.float16, torch.bfloat16) or v_pages.dtype != dtype:
-            raise TypeError("k_pages and v_pages must both be float16 or both bfloat16, got "
-                            f"{dtype}, {v_pages.dtype}")
-        if not k_pages.is_cuda or v_pages.device != dev:
-            raise ValueError("the paged cache needs CUDA tensors on one device (there is no CPU "
-                             "path)")
-        n_pages, Hkv, page_size, _ = k_pages.shape
-        if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
-            raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
-        ks, vs = k_pages.stride(), v_pages.stride()
-        if ks[3] != 1 or vs[3] != 1 or any(s % 8 for s in ks[:3] + vs[:3]) \
-                or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16:
-            raise ValueError("k_pages and v_pages must be 16-byte aligned, with a contiguous last "
-                             "dimension and strides that are multiples of 8")
-        table = _index(block_table, "block_table", dev, (B, -1))
-        sl = _index(seq_lens, "seq_lens", dev, (B,))
-        ql = None if q_lens is None else _index(q_lens, "q_lens", dev, (B,))
-        self.dev, self.dtype, self.B, self.Hkv = dev, dtype, B, Hkv
-        self.max_pages, self.page_size = table.shape[1], page_size
-        self.keep = (table, sl, ql)
-        self.head = (k_pages.data_ptr(), v_pages.data_ptr(), _Strides6(*ks[:3], *vs[:3]),
-                     table.data_ptr(), table.stride(0), table.shape[1], n_pages, page_size,
-                     sl.data_ptr(), ql.data_ptr() if ql is not None else None)
-
-
-class _on:
-    """``torch.cuda.device`` without its cost when ``dev`` is current already."""
-
-    __slots__ = ("ctx",)
-
-    def __init__(self, dev):
-        self.ctx = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+@lru_cache(maxsize=4096)
+def _scratch_bytes(device_index, B, Hq, Hkv, Tq, max_pages, page_size, prefix_len) -> int:
+    """``bsattn_paged_scratch_bytes`` on the current device: a function of the sizes alone."""
+    need = ctypes.c_size_t(0)
+    rc = _lib.load().bsattn_paged_scratch_bytes(B, Hq, Hkv, Tq, max_pages, page_size, prefix_len,
+                                                ctypes.byref(need))
+    if rc != 0:
+        raise BsattnError(rc, "bsattn_paged_scratch_bytes")
+    return need.value
 
 
 def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -137,30 +139,30 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     the slots of live rows are written.  Returns the rotated q, contiguous, with zeros in padding
     rows (``q_out`` when given; it may be q itself if that is contiguous), or None without q.
     """
-    lib = _lib.load()
-    if k.dim() != 4:
-        raise ValueError(f"k must be [B, Hkv, Tq, {HEAD_DIM}], got {tuple(k.shape)}")
-    B, _, Tq, _ = k.shape
-    c = _Call(k_pages, v_pages, block_table, seq_lens, q_lens, B)
-    dev, dtype = c.dev, c.dtype
-    k, v = _rows(k, "k", dev, dtype), _rows(v, "v", dev, dtype)
-    if k.shape[1] != c.Hkv or v.shape != k.shape:
-        raise ValueError(f"k and v must be [{B}, {c.Hkv}, {Tq}, {HEAD_DIM}], got {tuple(k.shape)}, "
-                         f"{tuple(v.shape)}")
-    Hq = 0
+    shape = k.shape
+    if len(shape) != 4:
+        raise ValueError(f"k must be [B, Hkv, Tq, {HEAD_DIM}], got {tuple(shape)}")
+    B, _, Tq, _ = shape
+    dev, dtype, Hkv, _, _, head, keep = _cache(k_pages, v_pages, block_table, seq_lens, q_lens, B)
+    rows = (B, Hkv, Tq, HEAD_DIM)
+    k, ks = _rows(k, "k", dev, dtype, rows)
+    v, vs = _rows(v, "v", dev, dtype, rows)
+    Hq, qs, qp, qo = 0, (0, 0, 0), None, None
     if q is not None:
         Hq = q.shape[1] if q.dim() == 4 else 0
-        if tuple(q.shape) != (B, Hq, Tq, HEAD_DIM) or Hq == 0:
+        if Hq == 0:
             raise ValueError(f"q must be [{B}, Hq, {Tq}, {HEAD_DIM}], got {tuple(q.shape)}")
-        q = _rows(q, "q", dev, dtype)
+        q, qs = _rows(q, "q", dev, dtype, (B, Hq, Tq, HEAD_DIM))
+        qp = q.data_ptr()
         if q_out is None:
-            q_out = torch.empty((B, Hq, Tq, HEAD_DIM), device=dev, dtype=dtype)
+            q_out = q.new_empty((B, Hq, Tq, HEAD_DIM))
         elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.device != dev \
-                or not q_out.is_contiguous():
-            raise ValueError("q_out has the wrong shape, dtype, device or layout")
+                or not q_out.is_contiguous() or q_out.data_ptr() & 15:
+            raise ValueError("q_out has the wrong shape, dtype, device, layout or alignment")
+        qo = q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out needs q")
-    rot = 0
+    rot, inv = 0, None
     if inv_freq is not None:
         if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != dev:
             raise TypeError("inv_freq must be float64 [rot_dim / 2] on the device of the pages")
@@ -168,19 +170,26 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
         if rot % 16 or not 0 < rot <= HEAD_DIM:
             raise ValueError(f"rot_dim must be a multiple of 16 up to {HEAD_DIM}, got {rot}")
         inv_freq = inv_freq.contiguous()
+        inv = inv_freq.data_ptr()
     if B == 0 or Tq == 0:
         return q_out
-    strides = _Strides9(*(q.stride()[:3] if q is not None else (0, 0, 0)), *k.stride()[:3],
-                        *v.stride()[:3])
-    with _on(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        ws = _workspace(dev, stream)
-        rc = lib.bsattn_paged_append(
-            *c.head, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), strides,
-            q_out.data_ptr() if q is not None else None,
-            inv_freq.data_ptr() if inv_freq is not None else None, rot, int(bool(interleaved)), B,
-            Hq, c.Hkv, Tq, _lib.IN_BF16 if dtype == torch.bfloat16 else 0, ws.data_ptr(),
-            ws.numel() * 4, stream)
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _append(dev, dtype, head, Hq, Hkv, Tq, qp, k, v, qs, ks, vs, qo, inv, rot,
+                           interleaved, q_out)
+    return _append(dev, dtype, head, Hq, Hkv, Tq, qp, k, v, qs, ks, vs, qo, inv, rot, interleaved,
+                   q_out)
+
+
+def _append(dev, dtype, head, Hq, Hkv, Tq, qp, k, v, qs, ks, vs, qo, inv, rot, interleaved, q_out):
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    ws = _workspace(dev, stream)
+    call = _PACK(*head, Hq, Hkv, Tq, _lib.IN_BF16 if dtype == torch.bfloat16 else 0, ws.data_ptr(),
+                 4 * ws.numel(), stream)
+    rc = _lib.load().bsattn_paged_append(
+        call, qp, k.data_ptr(), v.data_ptr(),
+        _STRIDES9(qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), qo, inv, rot,
+        1 if interleaved else 0)
     if rc != 0:
         raise BsattnError(rc, "bsattn_paged_append")
     return q_out
@@ -235,56 +244,59 @@ def shared_prefix_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 
 def _attn(q, k_pages, v_pages, block_table, seq_lens, q_lens, window, global_blocks, prefix_len,
           scale, out_dtype, out, lse_out, return_lse):
-    lib = _lib.load()
-    if q.dim() != 4 or q.shape[3] != HEAD_DIM:
-        raise ValueError(f"q must be [B, Hq, Tq, {HEAD_DIM}], got {tuple(q.shape)}")
-    B, Hq, Tq, _ = q.shape
-    c = _Call(k_pages, v_pages, block_table, seq_lens, q_lens, B)
-    dev = c.dev
-    if q.dtype != c.dtype or q.device != dev:
-        raise TypeError(f"q must be {c.dtype} on {dev} like the pages, got {q.dtype} on {q.device}")
-    if c.Hkv == 0 or Hq == 0 or Hq % c.Hkv:
-        raise ValueError(f"Hq must be a multiple of Hkv, got {Hq} and {c.Hkv}")
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM:
+        raise ValueError(f"q must be [B, Hq, Tq, {HEAD_DIM}], got {tuple(shape)}")
+    B, Hq, Tq, _ = shape
+    dev, dtype, Hkv, max_pages, page_size, head, keep = _cache(k_pages, v_pages, block_table,
+                                                               seq_lens, q_lens, B)
+    if q.dtype != dtype or q.device != dev:
+        raise TypeError(f"q must be {dtype} on {dev} like the pages, got {q.dtype} on {q.device}")
+    if Hq == 0 or Hq % Hkv:
+        raise ValueError(f"Hq must be a multiple of Hkv, got {Hq} and {Hkv}")
     if out_dtype is None:
-        out_dtype = q.dtype
-    if out_dtype not in (torch.float16, torch.bfloat16):
+        out_dtype = dtype
+    elif out_dtype not in _HALF:
         raise TypeError(f"out_dtype must be float16 or bfloat16, got {out_dtype}")
-    if not q.is_contiguous():
-        q = q.contiguous()
-    if q.data_ptr() % 16:
+    q = q.contiguous()
+    if q.data_ptr() & 15:
         q = q.clone()
     if out is None:
-        out = torch.empty(q.shape, device=dev, dtype=out_dtype)
-    elif out.shape != q.shape or out.dtype != out_dtype or out.device != dev \
-            or not out.is_contiguous():
-        raise ValueError("out has the wrong shape, dtype, device or layout")
+        out = torch.empty_like(q, dtype=out_dtype)
+    elif out.shape != shape or out.dtype != out_dtype or out.device != dev \
+            or not out.is_contiguous() or out.data_ptr() & 15:
+        raise ValueError("out has the wrong shape, dtype, device, layout or alignment")
     lse = None
     if return_lse:
         lse = lse_out
         if lse is None:
-            lse = torch.empty((B, Hq, Tq), device=dev, dtype=torch.float32)
+            lse = q.new_empty((B, Hq, Tq), dtype=torch.float32)
         elif lse.shape != (B, Hq, Tq) or lse.dtype != torch.float32 or lse.device != dev \
                 or not lse.is_contiguous():
             raise ValueError("lse_out has the wrong shape, dtype, device or layout")
     if B == 0 or Tq == 0:
         return out, lse
-    flags = (_lib.IN_BF16 if c.dtype == torch.bfloat16 else 0) | \
+    flags = (_lib.IN_BF16 if dtype == torch.bfloat16 else 0) | \
         (_lib.OUT_BF16 if out_dtype == torch.bfloat16 else 0)
-    with _on(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        ws = _workspace(dev, stream)
-        need = ctypes.c_size_t(0)
-        rc = lib.bsattn_paged_scratch_bytes(B, Hq, c.Hkv, Tq, c.max_pages, c.page_size, prefix_len,
-                                            ctypes.byref(need))
-        if rc != 0:
-            raise BsattnError(rc, "bsattn_paged_scratch_bytes")
-        # From the caching allocator: in a captured graph it belongs to the graph.
-        scratch = torch.empty(need.value, device=dev, dtype=torch.uint8)
-        rc = lib.bsattn_paged_fwd(
-            q.data_ptr(), *c.head, out.data_ptr(), lse.data_ptr() if lse is not None else None, B,
-            Hq, c.Hkv, Tq, window, global_blocks, prefix_len,
-            float(scale) if scale is not None else 0.0, flags, scratch.data_ptr(), need.value,
-            ws.data_ptr(), ws.numel() * 4, stream)
+    rule = (window, global_blocks, prefix_len, 0.0 if scale is None else float(scale))
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags, rule)
+    else:
+        _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags, rule)
+    return out, lse
+
+
+def _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags, rule):
+    index = dev.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    ws = _workspace(dev, stream)
+    need = _scratch_bytes(index, B, Hq, Hkv, Tq, max_pages, page_size, rule[2])
+    # From the caching allocator, for this call only: in a captured graph it belongs to the graph.
+    scratch = q.new_empty(need, dtype=torch.uint8)
+    call = _PACK(*head, Hq, Hkv, Tq, flags, ws.data_ptr(), 4 * ws.numel(), stream)
+    rc = _lib.load().bsattn_paged_fwd(call, q.data_ptr(), out.data_ptr(),
+                                      None if lse is None else lse.data_ptr(), *rule,
+                                      scratch.data_ptr(), need)
     if rc != 0:
         raise BsattnError(rc, "bsattn_paged_fwd")
-    return out, lse
