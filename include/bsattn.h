@@ -254,12 +254,14 @@ BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q,
  * the same pages, those of sequence 0's table row: they may be read once for the whole batch.  The
  * result is that of prefix_len == 0.  Dead rows and rows without keys get o = 0 and lse = -inf.
  * scratch: bsattn_paged_scratch_bytes bytes of device memory, 16-byte aligned, any content, used by
- * this call only. */
+ * this call only.  counters: bsattn_paged_counters() ints of device memory, zero before their first
+ * use; every call leaves them zero, and calls that may run at the same time need their own. */
+BSATTN_API int bsattn_paged_counters(void);
 BSATTN_API int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages,
                                           int page_size, int prefix_len, size_t* bytes);
 BSATTN_API int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, float* lse,
                                 int window, int global_blocks, int prefix_len, float scale,
-                                void* scratch, size_t scratch_bytes);
+                                void* scratch, size_t scratch_bytes, int32_t* counters);
 
 /* Human-readable text for a BSATTN_E* code. */
 BSATTN_API const char* bsattn_strerror(int code);

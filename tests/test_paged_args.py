@@ -19,10 +19,10 @@ CACHE = dict(kp=16, vp=16, st=[128] * 6, table=16, ts=4, mp=4, np=8, ps=16, sl=1
 
 
 def _fwd(**kw):
-    a = dict(CACHE, q=16, o=16, lse=None, window=0, glob=0, prefix=0)
+    a = dict(CACHE, q=16, o=16, lse=None, window=0, glob=0, prefix=0, cnt=16)
     a.update(kw)
     return _lib.load().bsattn_paged_fwd(_record(a), a["q"], a["o"], a["lse"], a["window"],
-                                        a["glob"], a["prefix"], 0.0, 16, 1 << 20)
+                                        a["glob"], a["prefix"], 0.0, 16, 1 << 20, a["cnt"])
 
 
 def _append(**kw):
@@ -53,6 +53,7 @@ def test_attention_arguments():
                dict(prefix=-16), dict(prefix=24), dict(prefix=80), dict(prefix=16, window=1)):
         assert _fwd(**kw) == _lib.E_SHAPE, kw
     assert _fwd(o=None) == _lib.E_NULL
+    assert _fwd(cnt=None) == _lib.E_NULL
     assert _fwd(flags=4) == _lib.E_DTYPE
     assert _fwd(q=24) == _lib.E_ALIGN
     assert _fwd(o=24) == _lib.E_ALIGN
@@ -71,7 +72,7 @@ def test_append_arguments():
 
 def test_null_call_record():
     lib = _lib.load()
-    assert lib.bsattn_paged_fwd(None, 16, 16, None, 0, 0, 0, 0.0, 16, 1 << 20) == _lib.E_NULL
+    assert lib.bsattn_paged_fwd(None, 16, 16, None, 0, 0, 0, 0.0, 16, 1 << 20, 16) == _lib.E_NULL
     assert lib.bsattn_paged_append(None, 16, 16, 16, bytes(72), 16, None, 0, 0) == _lib.E_NULL
 
 

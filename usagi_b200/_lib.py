@@ -75,8 +75,9 @@ SIGNATURES = {
         ctypes.c_char_p,                          # PAGED_CALL
         _c_void_p, _c_void_p, _c_void_p,          # q, o, lse
         _c_int, _c_int, _c_int, ctypes.c_float,   # window, global_blocks, prefix_len, scale
-        _c_void_p, _c_size_t,                     # scratch, bytes
+        _c_void_p, _c_size_t, _c_void_p,          # scratch, bytes, counters
     ]),
+    "bsattn_paged_counters": (_c_int, []),
     "bsattn_fwd_noalloc": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p,          # q, k, v
         _c_void_p, _c_void_p,                     # o, lse

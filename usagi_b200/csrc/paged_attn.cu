@@ -9,12 +9,15 @@
 // Few rows (the decode form).  Every key costs 512 bytes of HBM and G * Tq * 512 operations, so
 // the bound is memory; what matters is that all SMs read all the time and that nothing waits for
 // anything else.
-//   * Work: an item is (sequence, K/V head, tile of rows), a tile is 128 keys.  The tiles of all
-//     items form one line that is cut into equal pieces, one per CTA, so a long sequence is split
-//     over many CTAs and a short one shares a CTA with others.  The lengths are on the device:
-//     each CTA adds them up itself, in a few microseconds at most, and no host copy is needed.
-//   * A CTA is eight warps on their own: warp w owns keys 16w .. 16w+15 of every tile, loads them
-//     with cp.async into a private ring (16-byte pieces swizzled so that ldmatrix reads without
+//   * Work: an item is (sequence, K/V head, tile of rows), a tile is 64 keys.  All items form one
+//     line, measured in units of 16 keys (plus a few per item for what its end costs); it is cut
+//     into equal pieces, and a CTA takes the tiles that begin in its piece.  So a long sequence is
+//     split over many CTAs, a short one shares a CTA with others, and half-empty tiles do not
+//     unbalance them.  The lengths are on the device: each CTA adds them up itself, in a few
+//     microseconds at most, and no host copy is needed.
+//   * A CTA is four warps on their own, and two CTAs share an SM, so that one's item ends are hidden
+//     behind the other's work: warp w owns keys 16w .. 16w+15 of every tile, loads them with cp.async
+//     into a private ring (16-byte pieces swizzled so that ldmatrix reads without
 //     bank conflicts) and keeps its own running maximum, sum and output.  No barrier is met until
 //     a piece of an item ends; the ring runs across item borders.
 //   * Keys are the M dimension of the warp MMAs (m16n8k16): S^T = K Q^T and O^T = V^T P^T, so eight
@@ -22,10 +25,10 @@
 //     the operand layout with movmatrix, in registers.
 //   * The running maximum moves only when a score passes it by more than 2^8 (then P stays within
 //     2^8, far inside fp16 and bf16); the usual step costs one vote instead of a reduction.
-//   * At the end of a piece the eight warps' outputs are merged through shared memory in warp
-//     order.  A piece that is a whole item writes o and lse; others leave (o, log2 sum) in 32 bits
-//     for the join kernel, which adds them in the order of the line: results do not depend on
-//     timing.
+//   * At the end of a piece the warps' outputs are merged through shared memory in warp
+//     order.  A piece that is a whole item writes o and lse; others leave (o, log2 sum) in 32 bits,
+//     and the warp that finds its row's pieces complete adds them, in the order of the line: results
+//     do not depend on timing.
 // Keys past a sequence's end are loaded as zeros, never read: a recycled page may hold anything.
 // P is rounded to the type of V, as the tensor cores take it; its sum is of the unrounded values.
 #include <algorithm>
@@ -38,14 +41,18 @@
 namespace bsattn {
 namespace paged {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
+constexpr int kCtasPerSm = 2;
 constexpr int kThreadsD = kWarps * 32;
 constexpr int kStages = 3;
 constexpr int kSlice = 16;                        // keys of a tile per warp
 constexpr int kSliceBytes = kSlice * kHeadDim * 2;  // 4 KB of K or of V
 constexpr int kOPitch = kHeadDim + 4;             // floats between rows of the merge buffer
 constexpr float kRescaleLog2 = 8.0f;
-static_assert(kWarps * kSlice == kTileKeys, "a tile is one slice per warp");
+constexpr int kMaxSms = 160;     // SMs a call uses at most (a B200 has 148)
+constexpr int kFewRows = 16;     // rows of one tile of the few-row kernel
+constexpr int kStep = kWarps * kSlice;  // keys of a tile
+static_assert(kTileKeys % kStep == 0, "the window rule counts whole tiles");
 
 struct AttnParams {
   Cache c;
@@ -57,19 +64,22 @@ struct AttnParams {
   float scale_log2;
   int out_bf16;
   int all_partial;  // behind a shared prefix: no piece is a whole result
-  // Scratch: prefix sums of the tiles per sequence [B + 1], partial outputs and their log2 sums.
+  // Scratch: for the row join the sequences' places on the line [B + 1], its quota and alignment;
+  // partial outputs and their log2 sums.
   int* cum;
   float* part_o;
   float* part_l;
+  int* counters;  // [pieces, kFewRows], zero between calls: written pieces of a split item, by warp
 };
 
 template <int NB>
 struct DecodeSmem {
   uint8_t ring[kWarps][kStages][2][kSliceBytes];
   float o[kWarps][8][kOPitch];
-  float m[kWarps][8 * NB], l[kWarps][8 * NB];
-  int warp_sum[kWarps];
-  int found[3];
+  float m[kWarps][8], l[kWarps][8];
+  uint64_t o_free;  // all warps have read `o`
+  unsigned long long warp_sum[kWarps];
+  int found[4];
 };
 
 // Where a piece of item `item` that CTA `cta` holds leaves its partial output.  A CTA holds at most
@@ -79,79 +89,253 @@ __device__ __forceinline__ long long part_slot(int all_partial, long long item, 
   return all_partial ? item + cta : 2ll * cta + (head ? 1 : 0);
 }
 
-// A position on the line of tiles.
+// The key tiles of one sequence, those any live row sees, in ascending order: n_glob leading ones,
+// then those from key `lo` on.  A sequence without a key still gets one tile, so that every row is
+// written by the same path.
+struct Tiles {
+  int len;
+  Rows r;
+  int n, n_glob, lo;
+  int last;  // keys of the last tile
+};
+__device__ __forceinline__ int tile_key(const Tiles& t, int tile) {
+  return tile < t.n_glob ? tile * kStep : t.lo + (tile - t.n_glob) * kStep;
+}
+__device__ __forceinline__ Tiles tiles_of(const Cache& c, const Rule& r, int b) {
+  const SeqLen s = seq_len(c, b);
+  Tiles t;
+  t.len = s.len;
+  t.r = Rows{s.rows, s.len - s.rows};
+  t.lo = r.k0;
+  t.n_glob = 0;
+  t.n = 1;
+  t.last = 0;
+  if (s.rows > 0 && s.len > r.k0) {
+    if (r.window > 0) {
+      const int block = max(0, max(t.r.first, 0) / kTileKeys - r.window + 1);
+      t.lo = block * kTileKeys;
+      t.n_glob = min(r.glob, block) * (kTileKeys / kStep);
+    }
+    const int n = (s.len - t.lo + kStep - 1) / kStep;
+    t.last = s.len - t.lo - (n - 1) * kStep;
+    t.n = t.n_glob + n;
+  }
+  return t;
+}
+
+// The line.  Tile k of an item begins kTileUnits k units behind it.  Small calls are cut item by item
+// (align > 0: items are rounded up to pieces of `align` units, so no CTA has two), larger ones in
+// equal pieces wherever that falls.
+constexpr int kTileUnits = kStep / kSlice;
+constexpr int kItemUnits = 2;
+constexpr int kAlign = 16;
+__device__ __forceinline__ int units_of(const Tiles& t, int align) {
+  const int starts = kTileUnits * (t.n - 1);
+  return align > 0 ? (starts / align + 1) * align
+                   : starts + max((t.last + kSlice - 1) / kSlice, 1) + kItemUnits;
+}
+// Pieces of an item of that many units that begins at unit `at`: every CTA from the first one to
+// that of the last tile holds a tile, since a piece is no shorter than one.
+struct Line {
+  int quota, align;
+};
+__device__ __forceinline__ int last_piece(const Line& x, int at, int units) {
+  if (x.align > 0) return (at + units) / x.quota - 1;
+  return (at + (units - kItemUnits - 1) / kTileUnits * kTileUnits) / x.quota;
+}
+
+// A split item of this CTA: the CTAs it lies in, its first row of q and its rows.
+struct Split {
+  int first, last, rows;
+  long long q_row;
+};
+
+// A tile on the line.
 struct Cursor {
   int b, h, tile;  // h counts (K/V head, row tile)
+  int item, u;     // first unit of the item, and of the tile
   Tiles t;
 };
 
+__device__ __forceinline__ void store_row(void* o, float* lse, int out_bf16, long long row, float4 v,
+                                          float lg, int lane) {
+  reinterpret_cast<uint2*>(o)[row * (kHeadDim / 4) + lane] =
+      make_uint2(pack_out(v.x, v.y, out_bf16), pack_out(v.z, v.w, out_bf16));
+  if (lse != nullptr && lane == 0) lse[row] = lg * 0.69314718055994531f;
+}
+
+// A weighted sum of partial rows, which are read past L1: other SMs may have written them while
+// this kernel ran.
+struct PartSum {
+  float4 acc;
+  float sum;
+  __device__ __forceinline__ void add(float4 y, float w) {
+    acc.x += y.x * w;
+    acc.y += y.y * w;
+    acc.z += y.z * w;
+    acc.w += y.w * w;
+    sum += w;
+  }
+};
+__device__ __forceinline__ float4 part_row(const float* po, long long row, int lane) {
+  return __ldcg(reinterpret_cast<const float4*>(po) + row * (kHeadDim / 4) + lane);
+}
+
+// One warp, kRowsPerWarp rows: o = sum_c o_c 2^(l_c - l), l = log2 sum 2^l_c over the pieces of CTAs
+// first .. last, in that order, eight pieces of each row asked for at a time.
+constexpr int kRowsPerWarp = 8 / kWarps;
+__device__ __noinline__ void join_own(const AttnParams& p, long long row, int r, int live, int R,
+                                      int first, int last, int lane) {
+  constexpr int kAtOnce = 8;
+  const int n = last - first + 1;
+  float mx[kRowsPerWarp];
+  PartSum s[kRowsPerWarp];
+#pragma unroll
+  for (int k = 0; k < kRowsPerWarp; ++k) {
+    mx[k] = -INFINITY;
+    s[k] = PartSum{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f};
+  }
+  for (int c0 = 0; c0 < n; c0 += kAtOnce) {
+    float4 y[kRowsPerWarp][kAtOnce];
+    float lg[kRowsPerWarp][kAtOnce];
+#pragma unroll
+    for (int c = 0; c < kAtOnce; ++c)
+#pragma unroll
+      for (int k = 0; k < kRowsPerWarp; ++k) {
+        lg[k][c] = -INFINITY;
+        y[k][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c0 + c < n && k < live) {
+          const long long at = part_slot(0, 0, first + c0 + c, c0 + c == 0) * R + r + k;
+          lg[k][c] = __ldcg(p.part_l + at);
+          y[k][c] = part_row(p.part_o, at, lane);
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < kRowsPerWarp; ++k) {
+      float top = mx[k];
+#pragma unroll
+      for (int c = 0; c < kAtOnce; ++c) top = fmaxf(top, lg[k][c]);
+      if (top == -INFINITY) continue;
+      const float f = ptx::ex2(mx[k] - top);
+      mx[k] = top;
+      s[k].acc = make_float4(s[k].acc.x * f, s[k].acc.y * f, s[k].acc.z * f, s[k].acc.w * f);
+      s[k].sum *= f;
+#pragma unroll
+      for (int c = 0; c < kAtOnce; ++c) s[k].add(y[k][c], ptx::ex2(lg[k][c] - top));
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRowsPerWarp; ++k) {
+    if (k >= live) continue;
+    const float inv = s[k].sum > 0.0f ? 1.0f / s[k].sum : 0.0f;
+    const float4 a = s[k].acc;
+    store_row(p.o, p.lse, p.out_bf16, row + k, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv),
+              s[k].sum > 0.0f ? mx[k] + log2f(s[k].sum) : -INFINITY, lane);
+  }
+}
+
+// The other warps of this CTA are past a __syncthreads and on their way to this arrival: the wait
+// ends within the few hundred cycles that they take to read the buffer.
+__device__ __forceinline__ void wait_merge(uint32_t bar, uint32_t parity) {
+  for (int it = 0; it < (1 << 20) && !ptx::mbar_try_wait(bar, parity); ++it) {
+  }
+}
+
 template <bool BF16, int NB>
-__global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreadsD, kCtasPerSm) decode_kernel(const __grid_constant__ AttnParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   DecodeSmem<NB>& sh = *reinterpret_cast<DecodeSmem<NB>*>(smem_raw);
   constexpr int R = 8 * NB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int per_seq = p.c.Hkv * p.row_tiles;
+  const uint32_t o_free = ptx::smem_u32(&sh.o_free);
   pdl_trigger();
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(o_free, kWarps);
+    ptx::fence_mbar_init();
+    sh.found[0] = -1;
+  }
 
   // Where this CTA's piece of the line starts.
   const int chunk = (p.c.B + kThreadsD - 1) / kThreadsD;
   const int b0 = min(static_cast<int>(threadIdx.x) * chunk, p.c.B);
   const int b1 = min(b0 + chunk, p.c.B);
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(p.c, p.rule, b).n;
-  int incl = mine;
+  unsigned long long mine = 0;  // units, and in the upper half aligned ones
+  for (int b = b0; b < b1; ++b) {
+    const Tiles t = tiles_of(p.c, p.rule, b);
+    mine += static_cast<unsigned>(units_of(t, 0)) +
+            (static_cast<unsigned long long>(units_of(t, kAlign)) << 32);
+  }
+  unsigned long long incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, d);
+    const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += up;
   }
   if (lane == 31) sh.warp_sum[warp] = incl;
   __syncthreads();
-  int total = 0, before = incl - mine;
+  unsigned long long total2 = 0, before2 = incl - mine;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += sh.warp_sum[w];
-    total += sh.warp_sum[w];
+    if (w < warp) before2 += sh.warp_sum[w];
+    total2 += sh.warp_sum[w];
   }
+  const int pieces = static_cast<int>(gridDim.x);
+  Line ln;
+  ln.align = static_cast<long long>(total2 >> 32) * per_seq <= static_cast<long long>(pieces) * kAlign
+                 ? kAlign : 0;
+  const int total = static_cast<int>(ln.align ? total2 >> 32 : total2 & 0xffffffffu);
+  int before = static_cast<int>(ln.align ? before2 >> 32 : before2 & 0xffffffffu);
   const int line = total * per_seq;
-  const int quota = (line + gridDim.x - 1) / gridDim.x;
-  const int begin = min(static_cast<int>(blockIdx.x) * quota, line);
-  const int end = min(begin + quota, line);
+  ln.quota = ln.align ? kAlign : max((line + pieces - 1) / pieces, kTileUnits);
+  const int begin = static_cast<int>(
+      min(static_cast<long long>(blockIdx.x) * ln.quota, static_cast<long long>(line)));
+  const int end = min(begin + ln.quota, line);
   for (int b = b0; b < b1; ++b) {
-    const int n = tiles_of(p.c, p.rule, b).n;
-    if (blockIdx.x == 0) p.cum[b] = before;
+    const Tiles t = tiles_of(p.c, p.rule, b);
+    const int n = units_of(t, ln.align);
+    if (blockIdx.x == 0 && p.all_partial) p.cum[b] = before;
     const int rel = begin - before * per_seq;
     if (rel >= 0 && rel < n * per_seq) {
-      sh.found[0] = b;
-      sh.found[1] = rel / n;
-      sh.found[2] = rel % n;
+      // The first tile that begins at or behind `begin`, maybe of the next item.
+      int h = rel / n, tile = (rel - h * n + kTileUnits - 1) / kTileUnits;
+      if (tile >= t.n) ++h, tile = 0;
+      const bool roll = h == per_seq;
+      sh.found[1] = roll ? 0 : h;
+      sh.found[2] = tile;
+      sh.found[3] = before * per_seq + h * n;
+      sh.found[0] = b + roll;
     }
     before += n;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.cum[p.c.B] = total;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.all_partial) {
+    p.cum[p.c.B] = total;
+    p.cum[p.c.B + 1] = ln.quota;
+    p.cum[p.c.B + 2] = ln.align;
+  }
   __syncthreads();
-  if (begin >= end) {
+  const int b_first = sh.found[0];
+  if (begin >= end || b_first < 0 || b_first >= p.c.B ||
+      sh.found[3] + sh.found[2] * kTileUnits >= end) {
     pdl_wait();
     return;
   }
 
-  auto seek = [&](Cursor& x) {
-    x.b = sh.found[0];
-    x.h = sh.found[1];
-    x.tile = sh.found[2];
-    x.t = tiles_of(p.c, p.rule, x.b);
-  };
   auto advance = [&](Cursor& x) {
-    if (++x.tile < x.t.n) return;
+    if (++x.tile < x.t.n) {
+      x.u += kTileUnits;
+      return;
+    }
     x.tile = 0;
+    x.item += units_of(x.t, ln.align);
+    x.u = x.item;
     if (++x.h < per_seq) return;
     x.h = 0;
     if (++x.b < p.c.B) x.t = tiles_of(p.c, p.rule, x.b);
   };
   // First key of this warp's slice.
-  auto slice_key = [&](const Cursor& x) { return tile_key(x.t, p.rule, x.tile) + warp * kSlice; };
+  auto slice_key = [&](const Cursor& x) { return tile_key(x.t, x.tile) + warp * kSlice; };
   auto page_at = [&](const Cursor& x) {
     const int key = slice_key(x);
     return key < x.t.len ? __ldg(p.c.table + x.b * p.c.table_stride + (key >> p.c.page_shift)) : 0;
@@ -159,16 +343,20 @@ __global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_const
 
   // Loads.  Lane l moves piece l % 16 of rows l / 16, l / 16 + 2, ...; the page of the next slice
   // is asked for one step ahead.
-  const int n_tiles = end - begin;
-  Cursor ld, cx;
-  seek(ld);
-  seek(cx);
+  Cursor ld;
+  ld.b = b_first;
+  ld.h = sh.found[1];
+  ld.tile = sh.found[2];
+  ld.item = sh.found[3];
+  ld.u = ld.item + ld.tile * kTileUnits;
+  ld.t = tiles_of(p.c, p.rule, ld.b);
+  Cursor cx = ld;
   int ld_page = page_at(ld);
   const uint32_t ring = ptx::smem_u32(sh.ring[warp]);
   const int lr = lane >> 4, lc = lane & 15;
   int ld_i = 0;
   auto load_next = [&]() {
-    if (ld_i < n_tiles) {
+    if (ld.u < end) {
       const int key = slice_key(ld);
       if (key < ld.t.len) {
         const int page = page_checked(p.c, ld_page);
@@ -189,10 +377,8 @@ __global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_const
         }
       }
       ++ld_i;
-      if (ld_i < n_tiles) {
-        advance(ld);
-        ld_page = page_at(ld);
-      }
+      advance(ld);
+      if (ld.u < end) ld_page = page_at(ld);
     }
     cp_async_commit();
   };
@@ -207,29 +393,56 @@ __global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_const
   int min_limit = 0, max_lo = 0;
   bool fresh = true;
   int seg_tile0 = 0;
+  uint32_t merges = 0;  // uses of the merge buffer so far
+  Split rest{0, 0, 0, 0}, head{0, 0, 0, 0};
 
-  for (int i = 0; i < n_tiles; ++i) {
+  // First row of q of item (b, h).
+  auto q_row_of = [&](int b, int h) {
+    const int head = h / p.row_tiles;
+    return (static_cast<long long>(b) * p.c.Hkv + head) * p.rows + (h - head * p.row_tiles) * R;
+  };
+  auto load_q = [&](int b, int h, uint32_t(&f)[NB][8][2]) {
+    const int left = p.rows - (h % p.row_tiles) * R;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) +
+                            (q_row_of(b, h) + nb * 8 + g) * (kHeadDim / 2) + t4;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        f[nb][kk][0] = nb * 8 + g < left ? __ldg(src + kk * 8) : 0u;
+        f[nb][kk][1] = nb * 8 + g < left ? __ldg(src + kk * 8 + 4) : 0u;
+      }
+    }
+  };
+  // With registers to spare (NB == 1) the next item's rows are fetched while this one is computed.
+  constexpr bool kAhead = NB == 1;
+  uint32_t qn[kAhead ? NB : 1][8][2];
+  if constexpr (kAhead) load_q(cx.b, cx.h, qn);
+
+  for (int i = 0; cx.u < end; ++i) {
     const int row0 = (cx.h % p.row_tiles) * R;
-    const int head = cx.h / p.row_tiles;
-    const long long q_row = (static_cast<long long>(cx.b) * p.c.Hkv + head) * p.rows + row0;
     if (fresh) {
       fresh = false;
       seg_tile0 = cx.tile;
       min_limit = 0x7fffffff;
       max_lo = 0;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int r = row0 + nb * 8 + g;
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + (q_row + nb * 8 + g) * (kHeadDim / 2);
+      if constexpr (kAhead) {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-          qf[nb][kk][0] = r < p.rows ? __ldg(src + kk * 8 + t4) : 0u;
-          qf[nb][kk][1] = r < p.rows ? __ldg(src + kk * 8 + t4 + 4) : 0u;
+          qf[0][kk][0] = qn[0][kk][0];
+          qf[0][kk][1] = qn[0][kk][1];
         }
+        const bool roll = cx.h + 1 == per_seq;
+        if (cx.item + units_of(cx.t, ln.align) < end) load_q(cx.b + roll, roll ? 0 : cx.h + 1, qn);
+      } else {
+        load_q(cx.b, cx.h, qf);
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int rr = row0 + nb * 8 + 2 * t4 + e;
-          rk[nb][e] = row_keys(cx.t, p.rule, rr % p.c.Tq);
+          rk[nb][e] = row_keys(cx.t.r, p.rule, p.c.Tq == 1 ? 0 : rr % p.c.Tq);
           if (rr >= p.rows) rk[nb][e] = RowKeys{0x7fffffff, 0};
           min_limit = min(min_limit, rk[nb][e].limit);
           max_lo = max(max_lo, rk[nb][e].lo);
@@ -337,200 +550,240 @@ __global__ void __launch_bounds__(kThreadsD, 1) decode_kernel(const __grid_const
       }
     }
 
-    if (cx.tile + 1 == cx.t.n || i + 1 == n_tiles) {
-      // The piece ends: join the warps.
+    if (cx.tile + 1 == cx.t.n || cx.u + kTileUnits >= end) {
+      // The piece ends: join the warps, eight rows at a time.  One barrier: the buffer was read long
+      // ago (o_free), and each warp adds up its share of the rows with everyone's maxima in hand.
+      const bool whole = !p.all_partial && seg_tile0 == 0 && cx.tile + 1 == cx.t.n;
+      const long long q_row = q_row_of(cx.b, cx.h);
+      const long long slot = part_slot(p.all_partial, static_cast<long long>(cx.b) * per_seq + cx.h,
+                                       static_cast<int>(blockIdx.x), seg_tile0 == 0);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int nb = 0; nb < NB; ++nb) {
+        if (merges > 0) wait_merge(o_free, (merges - 1) & 1u);
+        ++merges;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
           if (g == 0) {
-            sh.m[warp][nb * 8 + 2 * t4 + c] = m[nb][c];
-            sh.l[warp][nb * 8 + 2 * t4 + c] = l[nb][c];
+            sh.m[warp][2 * t4 + c] = m[nb][c];
+            sh.l[warp][2 * t4 + c] = l[nb][c];
           }
-        }
-      const bool whole = !p.all_partial && seg_tile0 == 0 && cx.tile + 1 == cx.t.n;
-      const long long slot = part_slot(p.all_partial, static_cast<long long>(cx.b) * per_seq + cx.h,
-                                       static_cast<int>(blockIdx.x), seg_tile0 == 0);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        __syncthreads();
-        // This thread writes row `warp` of the eight; every lane scales two columns.
-        float mx = -INFINITY, sum = 0.0f, f[2];
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sh.m[w][nb * 8 + warp]);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float mw = sh.m[w][nb * 8 + warp];
-          sum += mw == -INFINITY ? 0.0f : sh.l[w][nb * 8 + warp] * ptx::ex2(mw - mx);
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float mc = -INFINITY;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) mc = fmaxf(mc, sh.m[w][nb * 8 + 2 * t4 + c]);
-          f[c] = m[nb][c] == -INFINITY ? 0.0f : ptx::ex2(m[nb][c] - mc);
         }
 #pragma unroll
         for (int a = 0; a < 8; ++a)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            sh.o[warp][2 * t4 + (e & 1)][a * 16 + g + (e >> 1) * 8] = o[nb][a][e] * f[e & 1];
+            sh.o[warp][2 * t4 + (e & 1)][a * 16 + g + (e >> 1) * 8] = o[nb][a][e];
         __syncthreads();
-        const int r = nb * 8 + warp;
-        if (row0 + r < p.rows) {
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const int rb = warp * kRowsPerWarp, r = nb * 8 + rb;
+        const int live = min(max(p.rows - row0 - r, 0), kRowsPerWarp);  // rows of this warp
+        float4 acc[kRowsPerWarp];
+        float mx[kRowsPerWarp], sum[kRowsPerWarp];
+#pragma unroll
+        for (int k = 0; k < kRowsPerWarp; ++k) {
+          mx[k] = -INFINITY;
+          sum[k] = 0.0f;
+          acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (k >= live) continue;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) mx[k] = fmaxf(mx[k], sh.m[w][rb + k]);
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            const float4 y = *reinterpret_cast<const float4*>(&sh.o[w][warp][lane * 4]);
-            acc.x += y.x;
-            acc.y += y.y;
-            acc.z += y.z;
-            acc.w += y.w;
+            const float mw = sh.m[w][rb + k];
+            const float f = mw == -INFINITY ? 0.0f : ptx::ex2(mw - mx[k]);
+            const float4 y = *reinterpret_cast<const float4*>(&sh.o[w][rb + k][lane * 4]);
+            sum[k] += sh.l[w][rb + k] * f;
+            acc[k].x += y.x * f;
+            acc[k].y += y.y * f;
+            acc[k].z += y.z * f;
+            acc[k].w += y.w * f;
           }
-          const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-          const float lg = sum > 0.0f ? mx + log2f(sum) : -INFINITY;
-          acc.x *= inv;
-          acc.y *= inv;
-          acc.z *= inv;
-          acc.w *= inv;
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(o_free);
+#pragma unroll
+        for (int k = 0; k < kRowsPerWarp; ++k) {
+          if (k >= live) continue;
+          const float inv = sum[k] > 0.0f ? 1.0f / sum[k] : 0.0f;
+          const float lg = sum[k] > 0.0f ? mx[k] + log2f(sum[k]) : -INFINITY;
+          const float4 v = make_float4(acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv);
           if (whole) {
-            uint2 w2 = make_uint2(pack_out(acc.x, acc.y, p.out_bf16), pack_out(acc.z, acc.w, p.out_bf16));
-            reinterpret_cast<uint2*>(p.o)[(q_row + r) * (kHeadDim / 4) + lane] = w2;
-            if (p.lse != nullptr && lane == 0) p.lse[q_row + r] = lg * 0.69314718055994531f;
+            store_row(p.o, p.lse, p.out_bf16, q_row + r + k, v, lg, lane);
           } else {
-            reinterpret_cast<float4*>(p.part_o)[(slot * R + r) * (kHeadDim / 4) + lane] = acc;
-            if (lane == 0) p.part_l[slot * R + r] = lg;
+            reinterpret_cast<float4*>(p.part_o)[(slot * R + r + k) * (kHeadDim / 4) + lane] = v;
+            if (lane == 0) p.part_l[slot * R + r + k] = lg;
           }
         }
       }
+      if (!whole) {
+        Split& sp = seg_tile0 == 0 ? head : rest;
+        sp.first = cx.item / ln.quota;
+        sp.last = last_piece(ln, cx.item, units_of(cx.t, ln.align));
+        sp.q_row = q_row;
+        sp.rows = min(p.rows - row0, R);
+      }
       fresh = true;
     }
-    if (i + 1 < n_tiles) advance(cx);
+    advance(cx);
   }
   cp_async_wait<0>();
+  if (!p.all_partial && (head.rows > 0 || rest.rows > 0)) {
+    // The warp that finds its rows' pieces complete adds them up, in the order of the line.  Asked
+    // for once, at the CTA's end: the fence and the counter cost a round trip to L2 each.
+    int done[2][NB];
+    __threadfence();
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const Split& sp = e ? head : rest;
+        const int r = nb * 8 + warp * kRowsPerWarp;
+        done[e][nb] = -1;
+        if (lane == 0 && r < sp.rows)
+          done[e][nb] = atomicAdd(p.counters + sp.first * kFewRows + nb * kWarps + warp, 1);
+      }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const Split& sp = e ? head : rest;
+        const int r = nb * 8 + warp * kRowsPerWarp;
+        if (__shfl_sync(0xffffffffu, done[e][nb], 0) != sp.last - sp.first || r >= sp.rows) continue;
+        __threadfence();
+        if (lane == 0) p.counters[sp.first * kFewRows + nb * kWarps + warp] = 0;
+        join_own(p, sp.q_row + r, r, min(sp.rows - r, kRowsPerWarp), R, sp.first, sp.last, lane);
+      }
+  }
   // Behind a shared prefix this kernel starts while the prefix's still runs, and must not end
   // before it: the join waits for this kernel only.
   pdl_wait();
 }
 
-// Joins the pieces of a row: o = sum_i o_i 2^(l_i - l), l = log2 sum 2^l_i, over the pieces of its
-// item in the order of the line, then over those of the shared prefix.  A row whose item is one
-// piece is written already.  One block per row; its four warps take every fourth piece and meet in
-// shared memory.
-constexpr int kJoinWarps = 4;
-struct JoinParams {
-  int Hkv, G, Tq;
+// Joins behind a shared prefix: every row of the call, W warps a row, over the pieces of its own
+// keys in the order of the line, then over those of the prefix.
+struct RowJoin {
+  int Hkv, rows;         // rows = G * Tq
+  long long total;       // B * Hq * Tq
   void* o;
   float* lse;
   int out_bf16;
-  // Own keys: virtual sequence = b * v_per_seq + t / v_tok, item = it * heads + head tile, where a
-  // K/V head's rows are in tiles of R (few-row kernel) or already one tile (n_t tokens each).
-  const int* cum;
+  const int* cum;        // own keys, by the few-row kernel
   const float* part_o;
   const float* part_l;
-  int count, pieces, R, row_tiles, all_partial;
-  int n_t, per_seq;  // many-row kernel: tokens per tile of rows; 0: few-row kernel
-  // Prefix: n_b sequences per tile of rows, each item tiles_p tiles, pieces_p CTAs.
-  const float* pre_o;
+  int B, R, row_tiles;
+  const float* pre_o;    // prefix: n_b sequences per tile of rows, tiles_p tiles per item
   const float* pre_l;
   int n_b, tiles_p, quota_p;
 };
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ JoinParams p) {
+constexpr int kJoinWarps = 4;
+template <int W>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid_constant__ RowJoin p) {
   __shared__ float4 so[kJoinWarps][32];
-  __shared__ float sl[kJoinWarps], sm[kJoinWarps];
+  __shared__ float sl[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x % p.Tq;
-  const int bh = blockIdx.x / p.Tq;
-  const int Hq = p.Hkv * p.G;
-  const int b = bh / Hq, hq = bh - b * Hq;
-  const int h = hq / p.G, g = hq - h * p.G;
-  int v, hr, r;
-  if (p.n_t > 0) {
-    v = b * p.per_seq + t / p.n_t;
-    hr = h;
-    r = g * p.n_t + t % p.n_t;
-  } else {
-    const int row = g * p.Tq + t;
-    v = b;
-    hr = h * p.row_tiles + row / p.R;
-    r = row % p.R;
-  }
+  const long long row = W == 1 ? static_cast<long long>(blockIdx.x) * kJoinWarps + warp : blockIdx.x;
+  if (row >= p.total) return;
+  const int bh = static_cast<int>(row / p.rows), rr = static_cast<int>(row - static_cast<long long>(bh) * p.rows);
+  const int b = bh / p.Hkv, h = bh - b * p.Hkv;
+  const int hr = h * p.row_tiles + rr / p.R, r = rr % p.R;
   const int heads = p.Hkv * p.row_tiles;
+  const long long item_p = static_cast<long long>(b / p.n_b) * p.Hkv + h;
+  const int rp = (b % p.n_b) * p.rows + rr;
+  const long long sp = item_p * p.tiles_p;
+  const int first_p = static_cast<int>(sp / p.quota_p);
+  const int pre = static_cast<int>((sp + p.tiles_p - 1) / p.quota_p) - first_p + 1;
   pdl_wait();
-  const int c0 = p.cum[v], n = p.cum[v + 1] - c0;
-  const int line = p.cum[p.count] * heads;
-  const int quota = (line + p.pieces - 1) / p.pieces;
+  const int c0 = p.cum[b], n = p.cum[b + 1] - c0;
+  const Line ln{p.cum[p.B + 1], p.cum[p.B + 2]};
   const int s = c0 * heads + hr * n;
-  const int first = s / quota, last = (s + n - 1) / quota;
-  if (first == last && !p.all_partial) return;
-  const long long item = static_cast<long long>(v) * heads + hr;
-  int first_p = 0, pre = 0;  // pieces of the prefix
-  long long item_p = 0;
-  int rp = 0;
-  if (p.tiles_p > 0) {
-    item_p = static_cast<long long>(b / p.n_b) * p.Hkv + h;
-    rp = ((b % p.n_b) * p.G + g) * p.Tq + t;
-    const long long sp = item_p * p.tiles_p;
-    first_p = static_cast<int>(sp / p.quota_p);
-    pre = static_cast<int>((sp + p.tiles_p - 1) / p.quota_p) - first_p + 1;
-  }
-  const int own = last - first + 1;
-  float mx = -INFINITY, sum = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i = warp; i < own + pre; i += kJoinWarps) {
-    const float *po, *pl;
-    if (i < own) {
-      const long long row = part_slot(p.all_partial, item, first + i, i == 0) * p.R + r;
-      po = p.part_o + row * kHeadDim;
-      pl = p.part_l + row;
-    } else {
-      const long long row = (item_p + first_p + i - own) * 128 + rp;
-      po = p.pre_o + row * kHeadDim;
-      pl = p.pre_l + row;
+  const int first = s / ln.quota, own = last_piece(ln, s, n) - first + 1;
+  const long long item = static_cast<long long>(b) * heads + hr;
+  const float *po[2] = {p.part_o, p.pre_o}, *pl[2] = {p.part_l, p.pre_l};
+  const long long at[2] = {(item + first) * p.R + r, (item_p + first_p) * 128 + rp};
+  const int step[2] = {p.R, 128}, count[2] = {own, pre};
+  float mx = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    for (int c = lane; c < count[k]; c += 32)
+      mx = fmaxf(mx, pl[k][at[k] + static_cast<long long>(c) * step[k]]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  PartSum acc{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f};
+  if (mx > -INFINITY) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll 4
+      for (int c = W == 1 ? 0 : warp; c < count[k]; c += W) {
+        const long long x = at[k] + static_cast<long long>(c) * step[k];
+        acc.add(part_row(po[k], x, lane), ptx::ex2(pl[k][x] - mx));
+      }
     }
-    const float lg = *pl;
-    const float4 y = reinterpret_cast<const float4*>(po)[lane];
-    if (lg == -INFINITY) continue;
-    const float mn = fmaxf(mx, lg);
-    const float fa = ptx::ex2(mx - mn), fb = ptx::ex2(lg - mn);
-    acc.x = acc.x * fa + y.x * fb;
-    acc.y = acc.y * fa + y.y * fb;
-    acc.z = acc.z * fa + y.z * fb;
-    acc.w = acc.w * fa + y.w * fb;
-    sum = sum * fa + fb;
-    mx = mn;
   }
-  so[warp][lane] = acc;
-  if (lane == 0) {
-    sl[warp] = sum;
-    sm[warp] = mx;
-  }
-  __syncthreads();
-  if (warp != 0) return;
-  float top = -INFINITY;
+  if (W > 1) {
+    so[warp][lane] = acc.acc;
+    if (lane == 0) sl[warp] = acc.sum;
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sm[w]);
-  float total = 0.0f;
-  float4 out = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    if (sm[w] == -INFINITY) continue;
-    const float f = ptx::ex2(sm[w] - top);
-    const float4 y = so[w][lane];
-    total += sl[w] * f;
-    out.x += y.x * f;
-    out.y += y.y * f;
-    out.z += y.z * f;
-    out.w += y.w * f;
+    for (int w = 1; w < W; ++w) {
+      const float4 y = so[w][lane];
+      acc.acc.x += y.x;
+      acc.acc.y += y.y;
+      acc.acc.z += y.z;
+      acc.acc.w += y.w;
+      acc.sum += sl[w];
+    }
   }
-  const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-  const long long row = blockIdx.x;
-  reinterpret_cast<uint2*>(p.o)[row * (kHeadDim / 4) + lane] =
-      make_uint2(pack_out(out.x * inv, out.y * inv, p.out_bf16), pack_out(out.z * inv, out.w * inv, p.out_bf16));
-  if (p.lse != nullptr && lane == 0)
-    p.lse[row] = total > 0.0f ? (top + log2f(total)) * 0.69314718055994531f : -INFINITY;
+  const float inv = acc.sum > 0.0f ? 1.0f / acc.sum : 0.0f;
+  store_row(p.o, p.lse, p.out_bf16, row,
+            make_float4(acc.acc.x * inv, acc.acc.y * inv, acc.acc.z * inv, acc.acc.w * inv),
+            acc.sum > 0.0f ? mx + log2f(acc.sum) : -INFINITY, lane);
+}
+
+// Joins the items that the many-row kernel's line was cut in: at most one begins in each CTA and
+// goes on in the next ones (TileCut).  Block (c, y): rows 16 y .. of that item, a warp each four.
+struct CutJoin {
+  const TileCut* cuts;
+  RowTiles rt;
+  int Hkv, Tq;
+  void* o;
+  float* lse;
+  int out_bf16;
+  const float* part_o;
+  const float* part_l;
+};
+__global__ void __launch_bounds__(kJoinWarps * 32) join_cuts_kernel(const __grid_constant__ CutJoin p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = blockIdx.x;
+  pdl_wait();
+  const TileCut cut = p.cuts[first];
+  if (cut.v < 0) return;
+  const int b = cut.v / p.rt.per_seq, t0 = (cut.v - b * p.rt.per_seq) * p.rt.n_t;
+  for (int k = 0; k < 4; ++k) {
+    const int r = blockIdx.y * 16 + warp * 4 + k;
+    const int g = r / p.rt.n_t, t = t0 + r - g * p.rt.n_t;
+    if (g >= p.rt.G || t >= p.Tq) continue;
+    float mx = -INFINITY;
+    for (int c = lane; c < cut.pieces; c += 32)
+      mx = fmaxf(mx, p.part_l[part_slot(0, 0, first + c, c == 0) * 128 + r]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    PartSum acc{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f};
+    if (mx > -INFINITY) {
+#pragma unroll 4
+      for (int c = 0; c < cut.pieces; ++c) {
+        const long long x = part_slot(0, 0, first + c, c == 0) * 128 + r;
+        acc.add(part_row(p.part_o, x, lane), ptx::ex2(p.part_l[x] - mx));
+      }
+    }
+    const float inv = acc.sum > 0.0f ? 1.0f / acc.sum : 0.0f;
+    const long long row = ((static_cast<long long>(b) * p.Hkv + cut.h) * p.rt.G + g) * p.Tq + t;
+    store_row(p.o, p.lse, p.out_bf16, row,
+              make_float4(acc.acc.x * inv, acc.acc.y * inv, acc.acc.z * inv, acc.acc.w * inv),
+              acc.sum > 0.0f ? mx + log2f(acc.sum) : -INFINITY, lane);
+  }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -548,6 +801,7 @@ int device_sms(int* sms) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return BSATTN_E_CUDA;
+    n = std::min(n, kMaxSms);
     const void* kernels[] = {
         reinterpret_cast<const void*>(decode_kernel<false, 1>),
         reinterpret_cast<const void*>(decode_kernel<true, 1>),
@@ -617,10 +871,9 @@ struct Shape {
   RowTiles rt;      // of the many-row kernel's launch
   int tiles_p, pieces_p;
   long long slots, slots_p;
-  size_t cum, part_o, part_l, cum_p, pre_o, pre_l, bytes;  // offsets into the scratch
+  size_t cum, cuts, part_o, part_l, pre_o, pre_l, bytes;  // offsets into the scratch
 };
 
-constexpr int kFewRows = 16;     // rows of one tile of the few-row kernel
 constexpr int kStackedRows = 64; // more rows of one sequence fill a tile without its neighbours
 
 static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size, int prefix_len,
@@ -635,7 +888,8 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
   s->k0 = s->prefix ? prefix_len : 0;
   s->all_partial = s->prefix;
   // Most tiles one item can have.
-  const long long tiles = (static_cast<long long>(max_pages) * page_size + kTileKeys - 1) / kTileKeys + 1;
+  const int step = s->few ? kStep : kTileKeys;
+  const long long tiles = (static_cast<long long>(max_pages) * page_size + step - 1) / step + 1;
   long long items;
   if (s->few) {
     s->R = rows <= 8 ? 8 : kFewRows;
@@ -654,8 +908,8 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
     if (items * tiles > (1ll << 30)) return BSATTN_E_SHAPE;
     s->rt.count = s->count = static_cast<int>(count);
   }
-  if (items * tiles > (1ll << 30)) return BSATTN_E_SHAPE;
-  s->pieces = static_cast<int>(std::min<long long>(sms, items * tiles));
+  if (items * (tiles * kTileUnits + kAlign) > (1ll << 30)) return BSATTN_E_SHAPE;
+  s->pieces = static_cast<int>(std::min<long long>(s->few ? sms * kCtasPerSm : sms, items * tiles));
   s->slots = s->all_partial ? items + s->pieces : 2ll * s->pieces;
   s->tiles_p = s->pieces_p = 0;
   s->slots_p = 0;
@@ -678,10 +932,10 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
     at += (static_cast<size_t>(n) * sizeof(float) + 255) / 256 * 256;
     return here;
   };
-  s->cum = take(s->count + 1);
+  s->cum = take(s->prefix ? s->count + 3 : 0);
+  s->cuts = take(s->few ? 0 : s->pieces * static_cast<long long>(sizeof(TileCut) / sizeof(float)));
   s->part_o = take(s->slots * s->R * kHeadDim);
   s->part_l = take(s->slots * s->R);
-  s->cum_p = take(s->prefix ? s->rt.count + 1 : 0);
   s->pre_o = take(s->slots_p * 128 * kHeadDim);
   s->pre_l = take(s->slots_p * 128);
   s->bytes = at;
@@ -690,10 +944,10 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
 
 // A launch that may start while its predecessor still runs.
 template <class P>
-static bool launch_overlapped(void (*kernel)(P), unsigned grid, int threads, size_t smem,
+static bool launch_overlapped(void (*kernel)(P), dim3 grid, int threads, size_t smem,
                               cudaStream_t stream, const P& p) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -709,8 +963,8 @@ static bool launch_overlapped(void (*kernel)(P), unsigned grid, int threads, siz
 
 static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix_len, int Hq,
                         float scale, int dtype_flags, int page_size, void* o, float* lse,
-                        void* scratch, size_t scratch_bytes, cudaStream_t stream) {
-  if (!q || !o) return BSATTN_E_NULL;
+                        void* scratch, size_t scratch_bytes, int* counters, cudaStream_t stream) {
+  if (!q || !o || !counters) return BSATTN_E_NULL;
   if ((dtype_flags & ~(BSATTN_OUT_BF16 | BSATTN_IN_BF16)) != 0) return BSATTN_E_DTYPE;
   if ((reinterpret_cast<uintptr_t>(q) & 15u) != 0 || (reinterpret_cast<uintptr_t>(o) & 15u) != 0 ||
       (reinterpret_cast<uintptr_t>(scratch) & 15u) != 0)
@@ -745,7 +999,7 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     t.out_bf16 = out_bf16;
     t.pieces = s.prefix ? s.pieces_p : s.pieces;
     t.slots = s.prefix ? s.slots_p : s.slots;
-    t.cum = reinterpret_cast<int*>(base + (s.prefix ? s.cum_p : s.cum));
+    t.cuts = reinterpret_cast<TileCut*>(base + s.cuts);
     t.part_o = reinterpret_cast<float*>(base + (s.prefix ? s.pre_o : s.part_o));
     t.part_l = reinterpret_cast<float*>(base + (s.prefix ? s.pre_l : s.part_l));
     if ((rc = tile_launch(t, page_size, stream)) != BSATTN_OK) return rc;
@@ -765,6 +1019,7 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     p.cum = reinterpret_cast<int*>(base + s.cum);
     p.part_o = reinterpret_cast<float*>(base + s.part_o);
     p.part_l = reinterpret_cast<float*>(base + s.part_l);
+    p.counters = counters;
     const unsigned grid = static_cast<unsigned>(s.pieces);
     void (*kernel)(AttnParams) = s.R == 8 ? (bf16 ? decode_kernel<true, 1> : decode_kernel<false, 1>)
                                           : (bf16 ? decode_kernel<true, 2> : decode_kernel<false, 2>);
@@ -776,34 +1031,51 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
       if (cudaGetLastError() != cudaSuccess) return BSATTN_E_CUDA;
     }
   }
-  JoinParams j;
-  j.Hkv = cache.Hkv;
-  j.G = Hq / cache.Hkv;
-  j.Tq = cache.Tq;
-  j.o = o;
-  j.lse = lse;
-  j.out_bf16 = out_bf16;
-  j.cum = reinterpret_cast<const int*>(base + s.cum);
-  j.part_o = reinterpret_cast<const float*>(base + s.part_o);
-  j.part_l = reinterpret_cast<const float*>(base + s.part_l);
-  j.count = s.count;
-  j.pieces = s.pieces;
-  j.R = s.R;
-  j.row_tiles = s.row_tiles;
-  j.all_partial = s.all_partial;
-  j.n_t = s.few ? 0 : s.rt.n_t;
-  j.per_seq = s.few ? 1 : s.rt.per_seq;
-  j.pre_o = reinterpret_cast<const float*>(base + s.pre_o);
-  j.pre_l = reinterpret_cast<const float*>(base + s.pre_l);
-  j.n_b = s.prefix ? s.rt.n_b : 1;
-  j.tiles_p = s.tiles_p;
-  j.quota_p = 1;
   if (s.prefix) {
-    const long long line = static_cast<long long>(s.rt.count) * cache.Hkv * s.tiles_p;
-    j.quota_p = static_cast<int>((line + s.pieces_p - 1) / s.pieces_p);
+    RowJoin j;
+    j.Hkv = cache.Hkv;
+    j.rows = s.rows;
+    j.total = static_cast<long long>(cache.B) * Hq * cache.Tq;
+    j.o = o;
+    j.lse = lse;
+    j.out_bf16 = out_bf16;
+    j.cum = reinterpret_cast<const int*>(base + s.cum);
+    j.part_o = reinterpret_cast<const float*>(base + s.part_o);
+    j.part_l = reinterpret_cast<const float*>(base + s.part_l);
+    j.B = cache.B;
+    j.R = s.R;
+    j.row_tiles = s.row_tiles;
+    j.pre_o = reinterpret_cast<const float*>(base + s.pre_o);
+    j.pre_l = reinterpret_cast<const float*>(base + s.pre_l);
+    j.n_b = s.rt.n_b;
+    j.tiles_p = s.tiles_p;
+    const long long items_p = static_cast<long long>(s.rt.count) * cache.Hkv;
+    j.quota_p = static_cast<int>((items_p * s.tiles_p + s.pieces_p - 1) / s.pieces_p);
+    // A row of many pieces is shared by four warps.
+    const bool ok =
+        s.pieces_p / items_p >= 8
+            ? launch_overlapped(join_rows_kernel<kJoinWarps>, static_cast<unsigned>(j.total),
+                                kJoinWarps * 32, 0, stream, j)
+            : launch_overlapped(join_rows_kernel<1>,
+                                static_cast<unsigned>((j.total + kJoinWarps - 1) / kJoinWarps),
+                                kJoinWarps * 32, 0, stream, j);
+    if (!ok) return BSATTN_E_CUDA;
+  } else if (!s.few) {
+    CutJoin j;
+    j.cuts = reinterpret_cast<const TileCut*>(base + s.cuts);
+    j.rt = s.rt;
+    j.Hkv = cache.Hkv;
+    j.Tq = cache.Tq;
+    j.o = o;
+    j.lse = lse;
+    j.out_bf16 = out_bf16;
+    j.part_o = reinterpret_cast<const float*>(base + s.part_o);
+    j.part_l = reinterpret_cast<const float*>(base + s.part_l);
+    const unsigned groups = static_cast<unsigned>((s.rt.n_t * s.rt.G + 15) / 16);
+    if (!launch_overlapped(join_cuts_kernel, dim3(static_cast<unsigned>(s.pieces), groups),
+                           kJoinWarps * 32, 0, stream, j))
+      return BSATTN_E_CUDA;
   }
-  const unsigned rows = static_cast<unsigned>(static_cast<long long>(cache.B) * Hq * cache.Tq);
-  if (!launch_overlapped(join_kernel, rows, kJoinWarps * 32, 0, stream, j)) return BSATTN_E_CUDA;
   return BSATTN_OK;
 }
 
@@ -831,9 +1103,11 @@ int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages, in
   return BSATTN_OK;
 }
 
+int bsattn_paged_counters(void) { return kMaxSms * kCtasPerSm * kFewRows; }
+
 int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, float* lse, int window,
                      int global_blocks, int prefix_len, float scale, void* scratch,
-                     size_t scratch_bytes) {
+                     size_t scratch_bytes, int32_t* counters) {
   Cache c;
   const int rc = fill_cache(&c, call);
   if (rc != BSATTN_OK) return rc;
@@ -847,7 +1121,7 @@ int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, floa
     return BSATTN_E_SHAPE;
   const Rule rule{0, window, global_blocks};
   return launch_paged(q, c, rule, prefix_len, call->Hq, scale, call->dtype_flags, call->page_size, o,
-                      lse, scratch, scratch_bytes, static_cast<cudaStream_t>(call->stream));
+                      lse, scratch, scratch_bytes, counters, static_cast<cudaStream_t>(call->stream));
 }
 
 }  // extern "C"

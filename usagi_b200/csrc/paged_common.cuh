@@ -18,7 +18,7 @@ int launch_test_wait();                  // bsattn_test_unsignalled_wait
 namespace paged {
 
 constexpr int kHeadDim = 128;
-constexpr int kTileKeys = 128;  // keys of one tile: the block size of the window rule
+constexpr int kTileKeys = 128;  // the block size of the window rule, keys of a tensor-core tile
 
 // The cache and the batch as the kernels see them.  Strides are in bytes; the last dimension of
 // the pages is contiguous.
@@ -61,48 +61,22 @@ __device__ __forceinline__ int page_checked(const Cache& c, int page) {
   return -1;
 }
 
-// The key tiles of one sequence.  Row t is the token at position first + t and sees keys j <= its
-// position; with a window it sees blocks j / 128 < glob and j / 128 > position / 128 - window.
-// Tiles are the blocks any live row sees, in ascending order: n_glob leading ones, then those from
-// lo_block on.  Without a window the tiles start at key k0 (the end of a shared prefix, or 0).  A
-// sequence with no key still gets one tile, so that every row is written by the same path.
-struct Tiles {
-  int len, rows, first;
-  int n, n_glob, lo_block;
-};
+// Which keys a call reads: those from k0 on (behind a shared prefix), or by the window rule
+// (window > 0, k0 == 0): for a row in block i = position / 128 the blocks < glob and > i - window.
 struct Rule {
-  int k0, window, glob;  // window == 0: every key
+  int k0, window, glob;
 };
-__device__ __forceinline__ Tiles tiles_of(const Cache& c, const Rule& r, int b) {
-  const SeqLen s = seq_len(c, b);
-  Tiles t;
-  t.len = s.len;
-  t.rows = s.rows;
-  t.first = s.len - s.rows;
-  t.n_glob = 0;
-  t.lo_block = 0;
-  int n = 0;
-  if (s.rows > 0 && s.len > r.k0) {
-    if (r.window == 0) {
-      n = (s.len - r.k0 + kTileKeys - 1) / kTileKeys;
-    } else {
-      t.lo_block = max(0, max(t.first, 0) / kTileKeys - r.window + 1);
-      t.n_glob = min(r.glob, t.lo_block);
-      n = t.n_glob + (s.len - 1) / kTileKeys - t.lo_block + 1;
-    }
-  }
-  t.n = max(n, 1);
-  return t;
-}
-__device__ __forceinline__ int tile_key(const Tiles& t, const Rule& r, int tile) {
-  return r.k0 + (tile < t.n_glob ? tile : t.lo_block + tile - t.n_glob) * kTileKeys;
-}
+
+// The live rows of a sequence: row t is the token at position first + t.
+struct Rows {
+  int rows, first;
+};
 
 // The keys one row sees: j < limit, and j >= lo or j < glob_end.  limit == 0: none.
 struct RowKeys {
   int limit, lo;
 };
-__device__ __forceinline__ RowKeys row_keys(const Tiles& t, const Rule& r, int row_t) {
+__device__ __forceinline__ RowKeys row_keys(const Rows& t, const Rule& r, int row_t) {
   RowKeys k;
   const int pos = t.first + row_t;
   k.limit = (row_t < t.rows && pos >= 0) ? pos + 1 : 0;

@@ -12,11 +12,12 @@
 //
 // The work is cut like the few-row kernel's: the key tiles of all (tile of rows, K/V head) items
 // form one line in equal pieces, one per CTA.  A CTA is a pipeline of sixteen warps:
-//   warp 0      producer: Q per item; K and V tiles by TMA, one box per page and 64-column half, the
-//               lanes of the warp issuing the boxes of a tile side by side.  The page table is read
-//               one tile ahead.  Rows of V behind the sequence's end (recycled slots may hold NaN,
-//               and 0 * NaN is NaN) are overwritten with zeros in shared memory once the copy has
-//               landed, before the tile is handed on; rows of K need not be, their scores are masked;
+//   warp 0, 3   producers of Q and K, and of V, by TMA: one box per page and 64-column half, the
+//               lanes of a warp issuing the boxes of a tile.  The page table is read one tile ahead.
+//               With small pages the issue of the boxes is what bounds a producer, hence two.  Rows
+//               of V behind the sequence's end (recycled slots may hold NaN, and 0 * NaN is NaN) are
+//               overwritten with zeros in shared memory once the copy has landed, before the tile is
+//               handed on; rows of K need not be, their scores are masked;
 //   warp 1, 2   tcgen05 issuers of P V and of Q K^T;
 //   warps 4-11  softmax, two warpgroups, keys 0..63 and 64..127 of every tile: thread t owns row t.
 //               They exchange row maxima through shared memory; the running maximum moves only when
@@ -38,7 +39,7 @@ namespace paged {
 namespace tile {
 
 constexpr int kRows = 128;
-constexpr int kStages = 4;
+constexpr int kStages = 2;  // of K and of V each
 constexpr int kTileBytes = kTileKeys * kHeadDim * 2;  // 32 KB
 constexpr int kHalfBytes = kTileBytes / 2;            // 128 rows x 64 columns, 128-byte swizzle
 constexpr int kThreads = 512;
@@ -67,7 +68,7 @@ struct Params {
   int Hq;
   float scale_log2;
   int out_bf16;
-  int* cum;
+  TileCut* cuts;
   float* part_l;
   unsigned long long timeout_ns;
   int test_wait;  // test hook: the Q K^T issuer first waits on a barrier that nothing signals
@@ -85,17 +86,17 @@ struct Seg {
 
 struct alignas(1024) Smem {
   uint8_t q[2][kTileBytes];
-  uint8_t kv[kStages][kTileBytes];
+  uint8_t kv[2][kStages][kTileBytes];  // K, V
   uint8_t ostage[kHalfBytes];
   float xmax[2][2][kRows];
   float stats[2][3][kRows];
   uint64_t q_full[2], q_empty[2];
-  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t kv_full[2][kStages], kv_empty[2][kStages];
   uint64_t s_full[2], p_rdy[2][2], pv_done[2], xchg[2][4];
   uint64_t o_full[2], o_free[2], stats_rdy[2];
   Seg segs[kRing];
   uint64_t seg_full[kRing], seg_empty[kRing];
-  uint64_t tail;   // copies of a tile whose rest is filled with zeros
+  uint64_t tail[2];  // copies of a tile whose rest is filled with zeros
   uint64_t drain, unsignalled;
   int warp_sum[kThreads / 32];
   int found[3];
@@ -155,36 +156,38 @@ __device__ __forceinline__ void wait_drain(uint32_t bar, uint32_t parity, const 
 // The key tiles of virtual sequence v: those its last live row sees, at least one.
 struct VTiles {
   int b0, t0, n;
-  Tiles t;
+  int len, n_glob, lo_block;
+  Rows r;
 };
 __device__ __forceinline__ VTiles vtiles(const Params& p, int v) {
   VTiles x;
   if (p.prefix_len > 0) {
     x.b0 = v * p.rt.n_b;
     x.t0 = 0;
-    x.t.len = p.prefix_len;
-    x.t.rows = x.t.first = x.t.n_glob = x.t.lo_block = 0;
+    x.len = p.prefix_len;
+    x.r = Rows{0, 0};
+    x.n_glob = x.lo_block = 0;
     x.n = (p.prefix_len + kTileKeys - 1) / kTileKeys;
     return x;
   }
   x.b0 = v / p.rt.per_seq;
   x.t0 = (v - x.b0 * p.rt.per_seq) * p.rt.n_t;
   const SeqLen s = seq_len(p.c, x.b0);
-  x.t.len = s.len;
-  x.t.rows = s.rows;
-  x.t.first = s.len - s.rows;
-  x.t.n_glob = 0;
-  x.t.lo_block = 0;
-  const int last = x.t.first + min(x.t0 + p.rt.n_t, s.rows) - 1;  // position of the last live row
+  x.len = s.len;
+  x.r.rows = s.rows;
+  x.r.first = s.len - s.rows;
+  x.n_glob = 0;
+  x.lo_block = 0;
+  const int last = x.r.first + min(x.t0 + p.rt.n_t, s.rows) - 1;  // position of the last live row
   int n = 0;
   if (x.t0 < s.rows && last >= 0) {
     if (p.rule.window > 0) {
-      x.t.lo_block = max(0, max(x.t.first + x.t0, 0) / kTileKeys - p.rule.window + 1);
-      x.t.n_glob = min(p.rule.glob, x.t.lo_block);
+      x.lo_block = max(0, max(x.r.first + x.t0, 0) / kTileKeys - p.rule.window + 1);
+      x.n_glob = min(p.rule.glob, x.lo_block);
     }
-    n = x.t.n_glob + last / kTileKeys - x.t.lo_block + 1;
+    n = x.n_glob + last / kTileKeys - x.lo_block + 1;
   } else {
-    x.t.len = 0;  // no live row: one tile of zeros
+    x.len = 0;  // no live row: one tile of zeros
   }
   x.n = max(n, 1);
   return x;
@@ -238,233 +241,205 @@ __device__ __forceinline__ void walk_next(Walk& x, Smem& sh, const Params& p) {
 }
 
 // ------------------------------------------------------------------------------------------
-// Producer: the whole warp.  Load order K0, K1, V0, K2, V1, ...; Q of a segment before its first K.
+// Producers: a whole warp for K (and Q, and the segments), one for V.
 // ------------------------------------------------------------------------------------------
-__device__ void producer_role(Smem& sh, const CUtensorMap* tq, const CUtensorMap* tk,
-                              const CUtensorMap* tv, const Params& p, int begin, int end) {
-  const int lane = threadIdx.x & 31;
+struct Stream {
+  int is_v, stage;
+  uint32_t phase, issued, last_parity;  // bit per stage: a copy was issued, its phase
+  uint32_t tail_phase, tail_busy;
+};
+
+// Page of this lane's box (lane / 2) of the tile at key0, or -1: past the end, or no such box.
+__device__ __forceinline__ int box_page(const Params& p, const Seg& s, int j) {
+  const int box = (threadIdx.x & 31) >> 1;
+  const int key = seg_key(s, j) + box * p.box_rows;
+  if (box >= p.boxes || key >= s.load_end) return -1;
+  const int b = p.prefix_len > 0 ? 0 : s.b0;
+  return __ldg(p.c.table + b * p.c.table_stride + (key >> p.c.page_shift));
+}
+
+__device__ __forceinline__ bool load_tile(Smem& sh, const Params& p, Stream& x, const CUtensorMap* map,
+                                          const Seg& s, int j, int page) {
+  const int lane = threadIdx.x & 31, box = lane >> 1, half = lane & 1;
   const bool lead = lane == 0;
-  int stage = 0;
-  uint32_t phase = 0, issued = 0, last_parity = 0;
-  uint32_t q_issued = 0, q_last = 0;
-  uint32_t tail_phase = 0, tail_busy = 0;
-  bool ok = true;
-
-  // K walks the line itself.
-  int v = sh.found[0], h = sh.found[1], tl = sh.found[2];
-  VTiles vt = vtiles(p, v);
-  int left = end - begin;
-  Seg ks;
-  int kj = 0, kii = 0;
-  auto open_seg = [&]() {
-    ks.v = v;
-    ks.h = h;
-    ks.tile0 = tl;
-    ks.n = min(vt.n - tl, left);
-    ks.b0 = vt.b0;
-    ks.t0 = vt.t0;
-    ks.first = vt.t.first;
-    ks.rows = vt.t.rows;
-    ks.load_end = vt.t.len;
-    ks.n_glob = vt.t.n_glob;
-    ks.lo_block = vt.t.lo_block;
-    ks.whole = tl == 0 && ks.n == vt.n;
-    kj = 0;
-    left -= ks.n;
-    if (tl + ks.n == vt.n) {
-      tl = 0;
-      if (++h == p.c.Hkv) {
-        h = 0;
-        if (++v < p.rt.count) vt = vtiles(p, v);
-      }
-    } else {
-      tl += ks.n;
+  if (!wait_warp(ptx::smem_u32(&sh.kv_empty[x.is_v][x.stage]), x.phase ^ 1u, sh, p)) return false;
+  const uint32_t full = ptx::smem_u32(&sh.kv_full[x.is_v][x.stage]);
+  const uint32_t tail = ptx::smem_u32(&sh.tail[x.is_v]);
+  const uint32_t dst = ptx::smem_u32(sh.kv[x.is_v][x.stage]);
+  const int key0 = seg_key(s, j);
+  const int have = s.load_end - key0;  // rows that hold a token
+  const bool mine = box < p.boxes && box * p.box_rows < have;
+  if (mine) page = page_checked(p.c, page);
+  const bool get = mine && page >= 0;
+  const uint32_t got = __ballot_sync(0xffffffffu, get);
+  const bool hole = __any_sync(0xffffffffu, mine && !get);
+  const uint32_t bytes = __popc(got) * p.box_rows * 128;
+  // Rows that must be zero: of V behind the end, of both where there is no page.
+  const bool fill = hole || (x.is_v && have < kTileKeys);
+  const uint32_t bar = fill ? tail : full;
+  if (lead && bytes > 0) ptx::mbar_expect_tx(bar, bytes);
+  if (lead && bytes == 0 && !fill) ptx::mbar_arrive(bar);
+  __syncwarp();
+  if (get)
+    tma_load_5d(dst + half * kHalfBytes + box * p.box_rows * 128, map, bar, 0,
+                key0 & (p.page_size - 1) & ~(p.box_rows - 1), s.h, page, half);
+  if (fill) {
+    if (bytes > 0) {
+      x.tail_busy = 1;
+      if (!wait_warp(tail, x.tail_phase, sh, p)) return false;
+      x.tail_phase ^= 1u;
+      x.tail_busy = 0;
     }
-  };
-  // Page of box `i` (lane i / 2) of the tile at key0, or -1: past the end, or no page.
-  const int box = lane >> 1, half = lane & 1;
-  auto pages = [&](const Seg& s, int j) {
-    const int key = seg_key(s, j) + box * p.box_rows;
-    if (box >= p.boxes || key >= s.load_end) return -1;
-    const int b = p.prefix_len > 0 ? 0 : s.b0;
-    return __ldg(p.c.table + b * p.c.table_stride + (key >> p.c.page_shift));
-  };
-
-  auto load_tile = [&](const CUtensorMap* map, const Seg& s, int j, int page, bool is_v) -> bool {
-    if (!wait_warp(ptx::smem_u32(&sh.kv_empty[stage]), phase ^ 1u, sh, p)) return false;
-    const uint32_t full = ptx::smem_u32(&sh.kv_full[stage]);
-    const uint32_t dst = ptx::smem_u32(sh.kv[stage]);
-    const int key0 = seg_key(s, j);
-    const int have = s.load_end - key0;  // rows that hold a token
-    const bool mine = box < p.boxes && box * p.box_rows < have;
-    if (mine) page = page_checked(p.c, page);
-    const bool get = mine && page >= 0;
-    const uint32_t got = __ballot_sync(0xffffffffu, get);
-    const bool hole = __any_sync(0xffffffffu, mine && !get);
-    const uint32_t bytes = __popc(got) * p.box_rows * 128;
-    // Rows that must be zero: of V behind the end, of both where there is no page.
-    const bool fill = hole || (is_v && have < kTileKeys);
-    const uint32_t bar = fill ? ptx::smem_u32(&sh.tail) : full;
-    if (lead && bytes > 0) ptx::mbar_expect_tx(bar, bytes);
-    if (lead && bytes == 0 && !fill) ptx::mbar_arrive(bar);
+    // Lane l writes piece l % 8 of half (l / 8) % 2, rows l / 16, + 2, ...
+    for (int row = lane >> 4; row < kTileKeys; row += 2) {
+      const bool there = row < have && ((got >> ((row / p.box_rows) * 2)) & 1u);
+      if (!there)
+        ptx::sts128(dst + ((lane >> 3) & 1) * kHalfBytes + row * 128 + (lane & 7) * 16, 0, 0, 0, 0);
+    }
+    ptx::fence_async_smem();
     __syncwarp();
-    if (get)
-      tma_load_5d(dst + half * kHalfBytes + box * p.box_rows * 128, map, bar, 0,
-                  key0 & (p.page_size - 1) & ~(p.box_rows - 1), s.h, page, half);
-    issued |= 1u << stage;
-    last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
-    if (fill) {
-      if (bytes > 0) {
-        tail_busy = 1;
-        if (!wait_warp(ptx::smem_u32(&sh.tail), tail_phase, sh, p)) {
-          issued &= ~(1u << stage);  // nothing will complete on its barrier
-          return false;
-        }
-        tail_phase ^= 1u;
-        tail_busy = 0;
-      }
-      // Lane l writes piece l % 8 of half (l / 8) % 2, rows l / 16, + 2, ...
-      for (int row = lane >> 4; row < kTileKeys; row += 2) {
-        const bool there = row < have && ((got >> ((row / p.box_rows) * 2)) & 1u);
-        if (!there)
-          ptx::sts128(dst + ((lane >> 3) & 1) * kHalfBytes + row * 128 + (lane & 7) * 16, 0, 0, 0, 0);
-      }
-      ptx::fence_async_smem();
-      __syncwarp();
-      if (lead) ptx::mbar_arrive(full);
-    }
-    if (++stage == kStages) stage = 0, phase ^= 1u;
-    return true;
-  };
-
-  auto load_q = [&]() -> bool {
-    const int b = kii & 1;
-    const uint32_t ph = (static_cast<uint32_t>(kii) >> 1) & 1u;
-    if (!wait_warp(ptx::smem_u32(&sh.q_empty[b]), ph ^ 1u, sh, p)) return false;
-    if (lead) {
-      const uint32_t full = ptx::smem_u32(&sh.q_full[b]);
-      const int rows = p.rt.n_t * p.rt.G * p.rt.n_b;
-      ptx::mbar_expect_tx(full, 2 * rows * 128);
-      for (int z = 0; z < 2; ++z)
-        tma_load_5d(ptx::smem_u32(sh.q[b]) + z * kHalfBytes, tq, full, 0, ks.t0, ks.h * p.rt.G,
-                    ks.b0, z);
-    }
-    q_issued |= 1u << b;
-    q_last = (q_last & ~(1u << b)) | (ph << b);
-    return true;
-  };
-
-  // vw trails K by two tiles and uses the pages K's walk has read: pv0 of its tile, pv1 of the next.
-  Walk vw;
-  int pk = -1, pv0 = -1, pv1 = -1;
-  bool k_valid = true;
-  auto load_k = [&]() -> bool {
-    if (kj == 0 && !load_q()) return false;
-    const int page = pk;
-    const Seg cur = ks;
-    const int j = kj;
-    // Step on and ask for the next tile's pages before this tile's copies are issued.
-    bool publish = false;
-    if (++kj == ks.n) {
-      ++kii;
-      if (left > 0) {
-        open_seg();
-      } else {
-        k_valid = false;
-        ks.n = 0;
-      }
-      publish = true;
-    }
-    if (k_valid) pk = pages(ks, kj);
-    if (!load_tile(tk, cur, j, page, false)) return false;
-    if (publish && !ring_write(sh, p, kii, ks, lead)) return false;
-    pv1 = page;
-    return true;
-  };
-
-  open_seg();
-  ok = ring_write(sh, p, 0, ks, lead);
-  pk = pages(ks, 0);
-  if (ok) ok = load_k();
-  pv0 = pv1;
-  if (ok && k_valid) ok = load_k();
-  // The V stream's ring reads count once: lane 0 arrives for the warp.
-  vw.ii = vw.j = vw.t = 0;
-  vw.valid = false;
-  auto v_read = [&]() -> bool {
-    const int slot = vw.ii & (kRing - 1);
-    if (!wait_warp(ptx::smem_u32(&sh.seg_full[slot]), static_cast<uint32_t>(vw.ii / kRing) & 1u, sh, p))
-      return false;
-    vw.s = sh.segs[slot];
-    __syncwarp();
-    if (lead) ptx::mbar_arrive(ptx::smem_u32(&sh.seg_empty[slot]));
-    vw.valid = vw.s.n > 0;
-    return true;
-  };
-  if (ok) ok = v_read();
-  while (ok && vw.valid) {
-    ok = load_tile(tv, vw.s, vw.j, pv0, true);
-    if (!ok) break;
-    pv0 = pv1;
-    if (k_valid) ok = load_k();
-    if (!ok) break;
-    if (++vw.j == vw.s.n) {
-      vw.j = 0;
-      ++vw.ii;
-      ok = v_read();
-    }
+    if (lead) ptx::mbar_arrive(full);
   }
-  // No copy may still be landing in shared memory when the CTA exits.
-  if (lead) {
+  x.issued |= 1u << x.stage;
+  x.last_parity = (x.last_parity & ~(1u << x.stage)) | (x.phase << x.stage);
+  if (++x.stage == kStages) x.stage = 0, x.phase ^= 1u;
+  return true;
+}
+
+// No copy may still be landing in shared memory when the CTA exits.
+__device__ __forceinline__ void drain_stream(Smem& sh, const Params& p, const Stream& x) {
+  if ((threadIdx.x & 31) == 0) {
     for (int i = 0; i < kStages; ++i)
-      if ((issued >> i) & 1u)
-        wait_drain(ptx::smem_u32(&sh.kv_full[i]), (last_parity >> i) & 1u, p);
-    for (int b = 0; b < 2; ++b)
-      if ((q_issued >> b) & 1u)
-        wait_drain(ptx::smem_u32(&sh.q_full[b]), (q_last >> b) & 1u, p);
-    if (tail_busy) wait_drain(ptx::smem_u32(&sh.tail), tail_phase, p);
+      if ((x.issued >> i) & 1u)
+        wait_drain(ptx::smem_u32(&sh.kv_full[x.is_v][i]), (x.last_parity >> i) & 1u, p);
+    if (x.tail_busy) wait_drain(ptx::smem_u32(&sh.tail[x.is_v]), x.tail_phase, p);
   }
   __syncwarp();
 }
 
-// ------------------------------------------------------------------------------------------
-// MMA issuers (lane 0 of their warps).  Ring positions follow the load order: K(t) at t for t < 2
-// and 2t - 1 after; V(t) at 2t + 2, the CTA's last V at 2t + 1.
-// ------------------------------------------------------------------------------------------
-__device__ __forceinline__ void ring_slot(int pos, int& stage, uint32_t& phase) {
-  stage = pos % kStages;
-  phase = static_cast<uint32_t>(pos / kStages) & 1u;
+__device__ void producer_k_role(Smem& sh, const CUtensorMap* tq, const CUtensorMap* tk, const Params& p,
+                                int begin, int end, int quota) {
+  const bool lead = (threadIdx.x & 31) == 0;
+  uint32_t q_issued = 0, q_last = 0;
+  Stream x{0, 0, 0, 0, 0, 0, 0};
+  int v = sh.found[0], h = sh.found[1], tl = sh.found[2];
+  VTiles vt = vtiles(p, v);
+  int left = end - begin;
+  Seg s, next;
+  // The next segment of the line (n == 0: none).
+  auto step = [&](Seg& o) {
+    o.n = 0;
+    if (left == 0) return;
+    o.v = v;
+    o.h = h;
+    o.tile0 = tl;
+    o.n = min(vt.n - tl, left);
+    o.b0 = vt.b0;
+    o.t0 = vt.t0;
+    o.first = vt.r.first;
+    o.rows = vt.r.rows;
+    o.load_end = vt.len;
+    o.n_glob = vt.n_glob;
+    o.lo_block = vt.lo_block;
+    o.whole = tl == 0 && o.n == vt.n;
+    if (lead && p.prefix_len == 0 && tl == 0 && o.n < vt.n)
+      p.cuts[blockIdx.x] = TileCut{v, h, 1 + (vt.n - o.n + quota - 1) / quota, 0};
+    left -= o.n;
+    tl += o.n;
+    if (tl < vt.n) return;
+    tl = 0;
+    if (++h < p.c.Hkv) return;
+    h = 0;
+    if (++v < p.rt.count) vt = vtiles(p, v);
+  };
+  step(s);
+  bool ok = ring_write(sh, p, 0, s, lead);
+  int page = box_page(p, s, 0);
+  for (int k = 0; ok && s.n > 0; ++k) {
+    const int b = k & 1;
+    const uint32_t ph = (static_cast<uint32_t>(k) >> 1) & 1u;
+    ok = wait_warp(ptx::smem_u32(&sh.q_empty[b]), ph ^ 1u, sh, p);
+    if (!ok) break;
+    if (lead) {
+      const uint32_t full = ptx::smem_u32(&sh.q_full[b]);
+      ptx::mbar_expect_tx(full, 2 * p.rt.n_t * p.rt.G * p.rt.n_b * 128);
+      for (int z = 0; z < 2; ++z)
+        tma_load_5d(ptx::smem_u32(sh.q[b]) + z * kHalfBytes, tq, full, 0, s.t0, s.h * p.rt.G, s.b0, z);
+    }
+    q_issued |= 1u << b;
+    q_last = (q_last & ~(1u << b)) | (ph << b);
+    for (int j = 0; ok && j < s.n; ++j) {
+      const int now = page;
+      const bool last = j + 1 == s.n;
+      if (last) {
+        step(next);
+        if (next.n > 0) page = box_page(p, next, 0);
+      } else {
+        page = box_page(p, s, j + 1);
+      }
+      ok = load_tile(sh, p, x, tk, s, j, now);
+      if (ok && last) ok = ring_write(sh, p, k + 1, next, lead);
+    }
+    s = next;
+  }
+  drain_stream(sh, p, x);
+  if (lead)
+    for (int b = 0; b < 2; ++b)
+      if ((q_issued >> b) & 1u) wait_drain(ptx::smem_u32(&sh.q_full[b]), (q_last >> b) & 1u, p);
+  __syncwarp();
 }
 
+__device__ void producer_v_role(Smem& sh, const CUtensorMap* tv, const Params& p) {
+  const bool lead = (threadIdx.x & 31) == 0;
+  Stream x{1, 0, 0, 0, 0, 0, 0};
+  bool ok = true;
+  for (int k = 0; ok; ++k) {
+    const int slot = k & (kRing - 1);
+    if (!wait_warp(ptx::smem_u32(&sh.seg_full[slot]), static_cast<uint32_t>(k / kRing) & 1u, sh, p)) break;
+    const Seg s = sh.segs[slot];
+    __syncwarp();
+    if (lead) ptx::mbar_arrive(ptx::smem_u32(&sh.seg_empty[slot]));
+    if (s.n == 0) break;
+    int page = box_page(p, s, 0);
+    for (int j = 0; ok && j < s.n; ++j) {
+      const int now = page;
+      if (j + 1 < s.n) page = box_page(p, s, j + 1);
+      ok = load_tile(sh, p, x, tv, s, j, now);
+    }
+  }
+  drain_stream(sh, p, x);
+}
+
+// ------------------------------------------------------------------------------------------
+// MMA issuers (lane 0 of their warps).  Tile t uses stage t % 2 of K and of V, and S buffer t % 2.
+// ------------------------------------------------------------------------------------------
 template <bool BF16>
 __device__ void mma_s_role(Smem& sh, const Params& p, uint32_t tmem) {
   constexpr uint32_t idesc = ptx::idesc_f16_f32(128, 128, false, BF16);
   const uint64_t q_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.q[0]), 16, 1024);
-  const uint64_t k_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.kv[0]), 16, 1024);
+  const uint64_t k_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.kv[0][0]), 16, 1024);
   if (p.test_wait && !wait_one(ptx::smem_u32(&sh.unsignalled), 0, sh, p)) return;
   Walk x;
   walk_begin(x, sh, p);
   while (x.valid) {
     const int qb = x.ii & 1, sb = x.t & 1;
-    int stage;
-    uint32_t phase;
-    ring_slot(x.t < 2 ? x.t : 2 * x.t - 1, stage, phase);
+    const uint32_t tph = (static_cast<uint32_t>(x.t) >> 1) & 1u;
     if (x.j == 0 &&
         !wait_one(ptx::smem_u32(&sh.q_full[qb]), (static_cast<uint32_t>(x.ii) >> 1) & 1u, sh, p))
       return;
-    if (!wait_one(ptx::smem_u32(&sh.kv_full[stage]), phase, sh, p)) return;
+    if (!wait_one(ptx::smem_u32(&sh.kv_full[0][sb]), tph, sh, p)) return;
     if (x.t >= 2 &&  // P V(t-2) has read the P stored in S[sb]
-        !wait_one(ptx::smem_u32(&sh.pv_done[sb]), (static_cast<uint32_t>(x.t - 2) >> 1) & 1u, sh, p))
+        !wait_one(ptx::smem_u32(&sh.pv_done[sb]), tph ^ 1u, sh, p))
       return;
     ptx::tc_fence_after();
     const uint64_t qd = q_desc0 + static_cast<uint32_t>((qb * kTileBytes) >> 4);
-    const uint64_t kd = k_desc0 + static_cast<uint32_t>((stage * kTileBytes) >> 4);
+    const uint64_t kd = k_desc0 + static_cast<uint32_t>((sb * kTileBytes) >> 4);
 #pragma unroll
     for (int kk = 0; kk < kHeadDim / 16; ++kk) {
       const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
       ptx::mma_ss(tmem + sb * 128, qd + off, kd + off, idesc, kk > 0 ? 1u : 0u);
     }
-    ptx::tc_commit(ptx::smem_u32(&sh.kv_empty[stage]));
+    ptx::tc_commit(ptx::smem_u32(&sh.kv_empty[0][sb]));
     ptx::tc_commit(ptx::smem_u32(&sh.s_full[sb]));
     if (x.j == x.s.n - 1) ptx::tc_commit(ptx::smem_u32(&sh.q_empty[qb]));
     walk_next(x, sh, p);
@@ -474,34 +449,28 @@ __device__ void mma_s_role(Smem& sh, const Params& p, uint32_t tmem) {
 template <bool BF16>
 __device__ void mma_pv_role(Smem& sh, const Params& p, uint32_t tmem) {
   constexpr uint32_t idesc = ptx::idesc_f16_f32(128, 128, true, BF16);
-  const uint64_t v_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.kv[0]), kHalfBytes, 1024);
-  Walk x, nx;
+  const uint64_t v_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.kv[1][0]), kHalfBytes, 1024);
+  Walk x;
   walk_begin(x, sh, p);
-  nx = x;
-  if (nx.valid) walk_next(nx, sh, p);
   while (x.valid) {
     const int ob = x.ii & 1, sb = x.t & 1;
     const uint32_t tph = (static_cast<uint32_t>(x.t) >> 1) & 1u;
-    int stage;
-    uint32_t phase;
-    ring_slot(nx.valid ? 2 * x.t + 2 : 2 * x.t + 1, stage, phase);
-    if (!wait_one(ptx::smem_u32(&sh.kv_full[stage]), phase, sh, p)) return;
+    if (!wait_one(ptx::smem_u32(&sh.kv_full[1][sb]), tph, sh, p)) return;
     if (x.j == 0 && x.ii >= 2 &&  // O[ob] read out by the epilogue of segment ii - 2
         !wait_one(ptx::smem_u32(&sh.o_free[ob]), ((static_cast<uint32_t>(x.ii) >> 1) + 1u) & 1u, sh, p))
       return;
     if (!wait_one(ptx::smem_u32(&sh.p_rdy[sb][0]), tph, sh, p)) return;
     if (!wait_one(ptx::smem_u32(&sh.p_rdy[sb][1]), tph, sh, p)) return;
     ptx::tc_fence_after();
-    const uint64_t vd = v_desc0 + static_cast<uint32_t>((stage * kTileBytes) >> 4);
+    const uint64_t vd = v_desc0 + static_cast<uint32_t>((sb * kTileBytes) >> 4);
 #pragma unroll
     for (int kk = 0; kk < kTileKeys / 16; ++kk)
       ptx::mma_ts(tmem + kOCol + ob * 128, tmem + sb * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
                   vd + static_cast<uint32_t>((kk * 2048) >> 4), idesc, (x.j > 0 || kk > 0) ? 1u : 0u);
-    ptx::tc_commit(ptx::smem_u32(&sh.kv_empty[stage]));
+    ptx::tc_commit(ptx::smem_u32(&sh.kv_empty[1][sb]));
     ptx::tc_commit(ptx::smem_u32(&sh.pv_done[sb]));
     if (x.j == x.s.n - 1) ptx::tc_commit(ptx::smem_u32(&sh.o_full[ob]));
-    x = nx;
-    if (nx.valid) walk_next(nx, sh, p);
+    walk_next(x, sh, p);
   }
 }
 
@@ -522,16 +491,12 @@ __device__ __forceinline__ Row row_of(const Params& p, const Seg& s, int t) {
     r.b = -1;
     return r;
   }
-  Tiles tl;
+  Rows rows{s.rows, s.first};
   if (p.prefix_len > 0) {
     const SeqLen q = seq_len(p.c, r.b);
-    tl.rows = q.rows;
-    tl.first = q.len - q.rows;
-  } else {
-    tl.rows = s.rows;
-    tl.first = s.first;
+    rows = Rows{q.rows, q.len - q.rows};
   }
-  r.k = row_keys(tl, p.rule, r.t);
+  r.k = row_keys(rows, p.rule, r.t);
   if (p.prefix_len > 0) r.k.limit = min(r.k.limit, p.prefix_len);
   return r;
 }
@@ -788,15 +753,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       init(sh.stats_rdy[b], 256);
       for (int q = 0; q < 4; ++q) init(sh.xchg[b][q], 64);
     }
-    for (int i = 0; i < kStages; ++i) {
-      init(sh.kv_full[i], 1);
-      init(sh.kv_empty[i], 1);
+    for (int i = 0; i < 2 * kStages; ++i) {
+      init(sh.kv_full[i / kStages][i % kStages], 1);
+      init(sh.kv_empty[i / kStages][i % kStages], 1);
     }
     for (int i = 0; i < kRing; ++i) {
       init(sh.seg_full[i], 1);
       init(sh.seg_empty[i], kRingReaders);
     }
-    init(sh.tail, 1);
+    init(sh.tail[0], 1);
+    init(sh.tail[1], 1);
     init(sh.drain, 2);
     init(sh.unsignalled, 1);
     sh.abort_flag = 0;
@@ -828,7 +794,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int end = min(begin + quota, line);
   for (int v = v0; v < v1; ++v) {
     const int n = vtiles(p, v).n;
-    if (blockIdx.x == 0) p.cum[v] = before;
     const int rel = begin - before * p.c.Hkv;
     if (rel >= 0 && rel < n * p.c.Hkv) {
       sh.found[0] = v;
@@ -837,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     before += n;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.cum[p.rt.count] = total;
+  if (threadIdx.x == 0 && p.prefix_len == 0) p.cuts[blockIdx.x] = TileCut{-1, 0, 0, 0};
   if (warp == 0 && lane == 0) {
     ptx::tma_prefetch_desc(&tq);
     ptx::tma_prefetch_desc(&tk);
@@ -861,7 +826,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp < kSoftmaxWarp0) {
     ptx::setmaxnreg_dec<kControlRegs>();
     if (warp == 0) {
-      producer_role(sh, &tq, &tk, &tv, p, begin, end);
+      producer_k_role(sh, &tq, &tk, p, begin, end, quota);
+    } else if (warp == 3) {
+      producer_v_role(sh, &tv, p);
     } else if (warp == 1) {
       if (lane == 0) mma_pv_role<BF16>(sh, p, tmem);
     } else if (warp == 2) {
@@ -987,7 +954,7 @@ int tile_launch(const TileCall& call, int page_size, cudaStream_t stream) {
   p.Hq = call.Hq;
   p.scale_log2 = call.scale_log2;
   p.out_bf16 = call.out_bf16;
-  p.cum = call.cum;
+  p.cuts = call.cuts;
   p.part_l = call.part_l;
   p.timeout_ns = launch_timeout_ns();
   p.test_wait = launch_test_wait();

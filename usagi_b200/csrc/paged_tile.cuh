@@ -14,6 +14,12 @@ struct RowTiles {
   int count;    // virtual sequences of the call
 };
 
+// What CTA c leaves for the join: the item that begins in it and goes on in the next ones, and in
+// how many CTAs it lies (v < 0: none).  Its pieces are slots 2 c + 1, then 2 (c + 1), 2 (c + 2), ...
+struct TileCut {
+  int v, h, pieces, unused;
+};
+
 struct TileCall {
   Cache c;
   Rule rule;       // k0 is 0
@@ -27,7 +33,7 @@ struct TileCall {
   int in_bf16, out_bf16;
   int pieces;      // CTAs
   long long slots; // partial outputs of 128 rows
-  int* cum;        // [rt.count + 1]: prefix sums of tiles
+  TileCut* cuts;   // [pieces], without a prefix
   float* part_o;   // [slots, 128, 128]
   float* part_l;   // [slots, 128], log2
 };

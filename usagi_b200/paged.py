@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import threading
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -287,6 +288,26 @@ def _attn(q, k_pages, v_pages, block_table, seq_lens, q_lens, window, global_blo
     return out, lse
 
 
+_counter_lock = threading.Lock()
+_counter_sets: dict = {}
+
+
+def _counters(dev, stream) -> torch.Tensor:
+    """The counters of a call: one set per CUDA stream, whose calls follow one another; a captured
+    call gets its own, zeroed by the graph, since graphs of one stream may be replayed at once."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(_lib.load().bsattn_paged_counters(), dtype=torch.int32, device=dev)
+    key = (dev.index, stream)
+    t = _counter_sets.get(key)
+    if t is None:
+        with _counter_lock:
+            t = _counter_sets.get(key)
+            if t is None:
+                t = torch.zeros(_lib.load().bsattn_paged_counters(), dtype=torch.int32, device=dev)
+                _counter_sets[key] = t
+    return t
+
+
 def _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags, rule):
     index = dev.index
     stream = torch._C._cuda_getCurrentRawStream(index)
@@ -297,6 +318,6 @@ def _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags,
     call = _PACK(*head, Hq, Hkv, Tq, flags, ws.data_ptr(), 4 * ws.numel(), stream)
     rc = _lib.load().bsattn_paged_fwd(call, q.data_ptr(), out.data_ptr(),
                                       None if lse is None else lse.data_ptr(), *rule,
-                                      scratch.data_ptr(), need)
+                                      scratch.data_ptr(), need, _counters(dev, stream).data_ptr())
     if rc != 0:
         raise BsattnError(rc, "bsattn_paged_fwd")
