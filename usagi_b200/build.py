@@ -25,8 +25,8 @@ LIB_PATH = PKG_DIR / LIB_NAME
 STAMP_PATH = PKG_DIR / (LIB_NAME + ".sha256")
 
 SOURCES = ["bsattn_fwd.cu", "csr_build.cu", "peer.cu", "paged_append.cu", "paged_attn.cu",
-           "paged_tile.cu"]
-HEADERS = ["sm100_ptx.cuh", "paged_common.cuh", "paged_tile.cuh"]
+           "paged_few.cu", "paged_tile.cu"]
+HEADERS = ["sm100_ptx.cuh", "paged_common.cuh", "paged_few.cuh", "paged_tile.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,665 +1,20 @@
-// paged_attn.cu -- attention of new tokens over a paged K/V cache.
+// paged_attn.cu -- attention over a paged K/V cache: the calls, which kernels they take, and the joins
+// of partial results.
 //
-// Rows: q [B, Hq, Tq, 128]; the G = Hq / Hkv query heads that share a K/V head form, with their Tq
-// tokens, the G * Tq rows (g-major) that one pass over that head's keys serves.  For row (g, t) at
-// position p = seq_lens[b] - q_lens[b] + t:
-//     o = sum_j softmax_j(scale q . k_j) v_j over the keys j <= p (and the window rule),
-//     lse = ln sum_j exp(scale q . k_j);  no key: o = 0, lse = -inf.
-//
-// Few rows (the decode form).  Every key costs 512 bytes of HBM and G * Tq * 512 operations, so
-// the bound is memory; what matters is that all SMs read all the time and that nothing waits for
-// anything else.
-//   * Work: an item is (sequence, K/V head, tile of rows), a tile is 64 keys.  All items form one
-//     line, measured in units of 16 keys (plus a few per item for what its end costs); it is cut
-//     into equal pieces, and a CTA takes the tiles that begin in its piece.  So a long sequence is
-//     split over many CTAs, a short one shares a CTA with others, and half-empty tiles do not
-//     unbalance them.  The lengths are on the device: each CTA adds them up itself, in a few
-//     microseconds at most, and no host copy is needed.
-//   * A CTA is four warps on their own, and two CTAs share an SM, so that one's item ends are hidden
-//     behind the other's work: warp w owns keys 16w .. 16w+15 of every tile, loads them with cp.async
-//     into a private ring (16-byte pieces swizzled so that ldmatrix reads without
-//     bank conflicts) and keeps its own running maximum, sum and output.  No barrier is met until
-//     a piece of an item ends; the ring runs across item borders.
-//   * Keys are the M dimension of the warp MMAs (m16n8k16): S^T = K Q^T and O^T = V^T P^T, so eight
-//     rows fill an MMA's N and none of it is spent on padding; P^T moves from the accumulator to
-//     the operand layout with movmatrix, in registers.
-//   * The running maximum moves only when a score passes it by more than 2^8 (then P stays within
-//     2^8, far inside fp16 and bf16); the usual step costs one vote instead of a reduction.
-//   * At the end of a piece the warps' outputs are merged through shared memory in warp
-//     order.  A piece that is a whole item writes o and lse; others leave (o, log2 sum) in 32 bits,
-//     and the warp that finds its row's pieces complete adds them, in the order of the line: results
-//     do not depend on timing.
-// Keys past a sequence's end are loaded as zeros, never read: a recycled page may hold anything.
-// P is rounded to the type of V, as the tensor cores take it; its sum is of the unrounded values.
+// Rows of q that share a K/V head (G = Hq / Hkv query heads, Tq tokens) go together:
+//   * up to 16 rows: the few-row kernel (paged_few.cu), which is bound by memory;
+//   * more: the many-row kernel (paged_tile.cu), tiles of 128 rows on the tensor cores;
+//   * behind a shared prefix: the prefix's keys by the many-row kernel, over the stacked rows of the
+//     whole batch, the sequences' own keys by the few-row kernel at the same time, and a join of both.
 #include <algorithm>
 #include <mutex>
 
-#include "paged_common.cuh"
+#include "paged_few.cuh"
 #include "paged_tile.cuh"
 #include "sm100_ptx.cuh"
 
 namespace bsattn {
 namespace paged {
-
-constexpr int kWarps = 4;
-constexpr int kCtasPerSm = 2;
-constexpr int kThreadsD = kWarps * 32;
-constexpr int kStages = 3;
-constexpr int kSlice = 16;                        // keys of a tile per warp
-constexpr int kSliceBytes = kSlice * kHeadDim * 2;  // 4 KB of K or of V
-constexpr int kOPitch = kHeadDim + 4;             // floats between rows of the merge buffer
-constexpr float kRescaleLog2 = 8.0f;
-constexpr int kMaxSms = 160;     // SMs a call uses at most (a B200 has 148)
-constexpr int kFewRows = 16;     // rows of one tile of the few-row kernel
-constexpr int kStep = kWarps * kSlice;  // keys of a tile
-static_assert(kTileKeys % kStep == 0, "the window rule counts whole tiles");
-
-struct AttnParams {
-  Cache c;
-  Rule rule;
-  const void* q;
-  void* o;
-  float* lse;
-  int rows, row_tiles;  // rows = G * Tq; row_tiles = ceil(rows / R)
-  float scale_log2;
-  int out_bf16;
-  int all_partial;  // behind a shared prefix: no piece is a whole result
-  // Scratch: for the row join the sequences' places on the line [B + 1], its quota and alignment;
-  // partial outputs and their log2 sums.
-  int* cum;
-  float* part_o;
-  float* part_l;
-  int* counters;  // [pieces, kFewRows], zero between calls: written pieces of a split item, by warp
-};
-
-template <int NB>
-struct DecodeSmem {
-  uint8_t ring[kWarps][kStages][2][kSliceBytes];
-  float o[kWarps][8][kOPitch];
-  float m[kWarps][8], l[kWarps][8];
-  uint64_t o_free;  // all warps have read `o`
-  unsigned long long warp_sum[kWarps];
-  int found[4];
-};
-
-// Where a piece of item `item` that CTA `cta` holds leaves its partial output.  A CTA holds at most
-// one piece that begins its item and one other; when whole items are partial too, item + cta
-// numbers all pieces, since along the line one of the two always grows.
-__device__ __forceinline__ long long part_slot(int all_partial, long long item, int cta, bool head) {
-  return all_partial ? item + cta : 2ll * cta + (head ? 1 : 0);
-}
-
-// The key tiles of one sequence, those any live row sees, in ascending order: n_glob leading ones,
-// then those from key `lo` on.  A sequence without a key still gets one tile, so that every row is
-// written by the same path.
-struct Tiles {
-  int len;
-  Rows r;
-  int n, n_glob, lo;
-  int last;  // keys of the last tile
-};
-__device__ __forceinline__ int tile_key(const Tiles& t, int tile) {
-  return tile < t.n_glob ? tile * kStep : t.lo + (tile - t.n_glob) * kStep;
-}
-__device__ __forceinline__ Tiles tiles_of(const Cache& c, const Rule& r, int b) {
-  const SeqLen s = seq_len(c, b);
-  Tiles t;
-  t.len = s.len;
-  t.r = Rows{s.rows, s.len - s.rows};
-  t.lo = r.k0;
-  t.n_glob = 0;
-  t.n = 1;
-  t.last = 0;
-  if (s.rows > 0 && s.len > r.k0) {
-    if (r.window > 0) {
-      const int block = max(0, max(t.r.first, 0) / kTileKeys - r.window + 1);
-      t.lo = block * kTileKeys;
-      t.n_glob = min(r.glob, block) * (kTileKeys / kStep);
-    }
-    const int n = (s.len - t.lo + kStep - 1) / kStep;
-    t.last = s.len - t.lo - (n - 1) * kStep;
-    t.n = t.n_glob + n;
-  }
-  return t;
-}
-
-// The line.  Tile k of an item begins kTileUnits k units behind it.  Small calls are cut item by item
-// (align > 0: items are rounded up to pieces of `align` units, so no CTA has two), larger ones in
-// equal pieces wherever that falls.
-constexpr int kTileUnits = kStep / kSlice;
-constexpr int kItemUnits = 2;
-constexpr int kAlign = 16;
-__device__ __forceinline__ int units_of(const Tiles& t, int align) {
-  const int starts = kTileUnits * (t.n - 1);
-  return align > 0 ? (starts / align + 1) * align
-                   : starts + max((t.last + kSlice - 1) / kSlice, 1) + kItemUnits;
-}
-// Pieces of an item of that many units that begins at unit `at`: every CTA from the first one to
-// that of the last tile holds a tile, since a piece is no shorter than one.
-struct Line {
-  int quota, align;
-};
-__device__ __forceinline__ int last_piece(const Line& x, int at, int units) {
-  if (x.align > 0) return (at + units) / x.quota - 1;
-  return (at + (units - kItemUnits - 1) / kTileUnits * kTileUnits) / x.quota;
-}
-
-// A split item of this CTA: the CTAs it lies in, its first row of q and its rows.
-struct Split {
-  int first, last, rows;
-  long long q_row;
-};
-
-// A tile on the line.
-struct Cursor {
-  int b, h, tile;  // h counts (K/V head, row tile)
-  int item, u;     // first unit of the item, and of the tile
-  Tiles t;
-};
-
-__device__ __forceinline__ void store_row(void* o, float* lse, int out_bf16, long long row, float4 v,
-                                          float lg, int lane) {
-  reinterpret_cast<uint2*>(o)[row * (kHeadDim / 4) + lane] =
-      make_uint2(pack_out(v.x, v.y, out_bf16), pack_out(v.z, v.w, out_bf16));
-  if (lse != nullptr && lane == 0) lse[row] = lg * 0.69314718055994531f;
-}
-
-// A weighted sum of partial rows, which are read past L1: other SMs may have written them while
-// this kernel ran.
-struct PartSum {
-  float4 acc;
-  float sum;
-  __device__ __forceinline__ void add(float4 y, float w) {
-    acc.x += y.x * w;
-    acc.y += y.y * w;
-    acc.z += y.z * w;
-    acc.w += y.w * w;
-    sum += w;
-  }
-};
-__device__ __forceinline__ float4 part_row(const float* po, long long row, int lane) {
-  return __ldcg(reinterpret_cast<const float4*>(po) + row * (kHeadDim / 4) + lane);
-}
-
-// One warp, kRowsPerWarp rows: o = sum_c o_c 2^(l_c - l), l = log2 sum 2^l_c over the pieces of CTAs
-// first .. last, in that order, eight pieces of each row asked for at a time.
-constexpr int kRowsPerWarp = 8 / kWarps;
-__device__ __noinline__ void join_own(const AttnParams& p, long long row, int r, int live, int R,
-                                      int first, int last, int lane) {
-  constexpr int kAtOnce = 8;
-  const int n = last - first + 1;
-  float mx[kRowsPerWarp];
-  PartSum s[kRowsPerWarp];
-#pragma unroll
-  for (int k = 0; k < kRowsPerWarp; ++k) {
-    mx[k] = -INFINITY;
-    s[k] = PartSum{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f};
-  }
-  for (int c0 = 0; c0 < n; c0 += kAtOnce) {
-    float4 y[kRowsPerWarp][kAtOnce];
-    float lg[kRowsPerWarp][kAtOnce];
-#pragma unroll
-    for (int c = 0; c < kAtOnce; ++c)
-#pragma unroll
-      for (int k = 0; k < kRowsPerWarp; ++k) {
-        lg[k][c] = -INFINITY;
-        y[k][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (c0 + c < n && k < live) {
-          const long long at = part_slot(0, 0, first + c0 + c, c0 + c == 0) * R + r + k;
-          lg[k][c] = __ldcg(p.part_l + at);
-          y[k][c] = part_row(p.part_o, at, lane);
-        }
-      }
-#pragma unroll
-    for (int k = 0; k < kRowsPerWarp; ++k) {
-      float top = mx[k];
-#pragma unroll
-      for (int c = 0; c < kAtOnce; ++c) top = fmaxf(top, lg[k][c]);
-      if (top == -INFINITY) continue;
-      const float f = ptx::ex2(mx[k] - top);
-      mx[k] = top;
-      s[k].acc = make_float4(s[k].acc.x * f, s[k].acc.y * f, s[k].acc.z * f, s[k].acc.w * f);
-      s[k].sum *= f;
-#pragma unroll
-      for (int c = 0; c < kAtOnce; ++c) s[k].add(y[k][c], ptx::ex2(lg[k][c] - top));
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < kRowsPerWarp; ++k) {
-    if (k >= live) continue;
-    const float inv = s[k].sum > 0.0f ? 1.0f / s[k].sum : 0.0f;
-    const float4 a = s[k].acc;
-    store_row(p.o, p.lse, p.out_bf16, row + k, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv),
-              s[k].sum > 0.0f ? mx[k] + log2f(s[k].sum) : -INFINITY, lane);
-  }
-}
-
-// The other warps of this CTA are past a __syncthreads and on their way to this arrival: the wait
-// ends within the few hundred cycles that they take to read the buffer.
-__device__ __forceinline__ void wait_merge(uint32_t bar, uint32_t parity) {
-  for (int it = 0; it < (1 << 20) && !ptx::mbar_try_wait(bar, parity); ++it) {
-  }
-}
-
-template <bool BF16, int NB>
-__global__ void __launch_bounds__(kThreadsD, kCtasPerSm) decode_kernel(const __grid_constant__ AttnParams p) {
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  DecodeSmem<NB>& sh = *reinterpret_cast<DecodeSmem<NB>*>(smem_raw);
-  constexpr int R = 8 * NB;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t4 = lane & 3;
-  const int per_seq = p.c.Hkv * p.row_tiles;
-  const uint32_t o_free = ptx::smem_u32(&sh.o_free);
-  pdl_trigger();
-  if (threadIdx.x == 0) {
-    ptx::mbar_init(o_free, kWarps);
-    ptx::fence_mbar_init();
-    sh.found[0] = -1;
-  }
-
-  // Where this CTA's piece of the line starts.
-  const int chunk = (p.c.B + kThreadsD - 1) / kThreadsD;
-  const int b0 = min(static_cast<int>(threadIdx.x) * chunk, p.c.B);
-  const int b1 = min(b0 + chunk, p.c.B);
-  unsigned long long mine = 0;  // units, and in the upper half aligned ones
-  for (int b = b0; b < b1; ++b) {
-    const Tiles t = tiles_of(p.c, p.rule, b);
-    mine += static_cast<unsigned>(units_of(t, 0)) +
-            (static_cast<unsigned long long>(units_of(t, kAlign)) << 32);
-  }
-  unsigned long long incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += up;
-  }
-  if (lane == 31) sh.warp_sum[warp] = incl;
-  __syncthreads();
-  unsigned long long total2 = 0, before2 = incl - mine;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before2 += sh.warp_sum[w];
-    total2 += sh.warp_sum[w];
-  }
-  const int pieces = static_cast<int>(gridDim.x);
-  Line ln;
-  ln.align = static_cast<long long>(total2 >> 32) * per_seq <= static_cast<long long>(pieces) * kAlign
-                 ? kAlign : 0;
-  const int total = static_cast<int>(ln.align ? total2 >> 32 : total2 & 0xffffffffu);
-  int before = static_cast<int>(ln.align ? before2 >> 32 : before2 & 0xffffffffu);
-  const int line = total * per_seq;
-  ln.quota = ln.align ? kAlign : max((line + pieces - 1) / pieces, kTileUnits);
-  const int begin = static_cast<int>(
-      min(static_cast<long long>(blockIdx.x) * ln.quota, static_cast<long long>(line)));
-  const int end = min(begin + ln.quota, line);
-  for (int b = b0; b < b1; ++b) {
-    const Tiles t = tiles_of(p.c, p.rule, b);
-    const int n = units_of(t, ln.align);
-    if (blockIdx.x == 0 && p.all_partial) p.cum[b] = before;
-    const int rel = begin - before * per_seq;
-    if (rel >= 0 && rel < n * per_seq) {
-      // The first tile that begins at or behind `begin`, maybe of the next item.
-      int h = rel / n, tile = (rel - h * n + kTileUnits - 1) / kTileUnits;
-      if (tile >= t.n) ++h, tile = 0;
-      const bool roll = h == per_seq;
-      sh.found[1] = roll ? 0 : h;
-      sh.found[2] = tile;
-      sh.found[3] = before * per_seq + h * n;
-      sh.found[0] = b + roll;
-    }
-    before += n;
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0 && p.all_partial) {
-    p.cum[p.c.B] = total;
-    p.cum[p.c.B + 1] = ln.quota;
-    p.cum[p.c.B + 2] = ln.align;
-  }
-  __syncthreads();
-  const int b_first = sh.found[0];
-  if (begin >= end || b_first < 0 || b_first >= p.c.B ||
-      sh.found[3] + sh.found[2] * kTileUnits >= end) {
-    pdl_wait();
-    return;
-  }
-
-  auto advance = [&](Cursor& x) {
-    if (++x.tile < x.t.n) {
-      x.u += kTileUnits;
-      return;
-    }
-    x.tile = 0;
-    x.item += units_of(x.t, ln.align);
-    x.u = x.item;
-    if (++x.h < per_seq) return;
-    x.h = 0;
-    if (++x.b < p.c.B) x.t = tiles_of(p.c, p.rule, x.b);
-  };
-  // First key of this warp's slice.
-  auto slice_key = [&](const Cursor& x) { return tile_key(x.t, x.tile) + warp * kSlice; };
-  auto page_at = [&](const Cursor& x) {
-    const int key = slice_key(x);
-    return key < x.t.len ? __ldg(p.c.table + x.b * p.c.table_stride + (key >> p.c.page_shift)) : 0;
-  };
-
-  // Loads.  Lane l moves piece l % 16 of rows l / 16, l / 16 + 2, ...; the page of the next slice
-  // is asked for one step ahead.
-  Cursor ld;
-  ld.b = b_first;
-  ld.h = sh.found[1];
-  ld.tile = sh.found[2];
-  ld.item = sh.found[3];
-  ld.u = ld.item + ld.tile * kTileUnits;
-  ld.t = tiles_of(p.c, p.rule, ld.b);
-  Cursor cx = ld;
-  int ld_page = page_at(ld);
-  const uint32_t ring = ptx::smem_u32(sh.ring[warp]);
-  const int lr = lane >> 4, lc = lane & 15;
-  int ld_i = 0;
-  auto load_next = [&]() {
-    if (ld.u < end) {
-      const int key = slice_key(ld);
-      if (key < ld.t.len) {
-        const int page = page_checked(p.c, ld_page);
-        const long long pg = max(page, 0);
-        const long long head = ld.h / p.row_tiles;
-        const long long slot = key & ((1 << p.c.page_shift) - 1);
-        const char* ks = p.c.k + pg * p.c.k_page + head * p.c.k_head + (slot + lr) * p.c.k_tok + lc * 16;
-        const char* vs = p.c.v + pg * p.c.v_page + head * p.c.v_head + (slot + lr) * p.c.v_tok + lc * 16;
-        const uint32_t dst = ring + (ld_i % kStages) * (2 * kSliceBytes);
-        const int have = page < 0 ? 0 : ld.t.len - key;
-#pragma unroll
-        for (int i = 0; i < kSlice / 2; ++i) {
-          const int row = 2 * i + lr;
-          const uint32_t d = dst + row * (kHeadDim * 2) + ((lc ^ (row & 7)) << 4);
-          const uint32_t bytes = row < have ? 16u : 0u;
-          cp_async16(d, ks + 2 * i * p.c.k_tok, bytes);
-          cp_async16(d + kSliceBytes, vs + 2 * i * p.c.v_tok, bytes);
-        }
-      }
-      ++ld_i;
-      advance(ld);
-      if (ld.u < end) ld_page = page_at(ld);
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) load_next();
-
-  // Per-lane state: columns (rows of q) 8 nb + 2 t4 and + 1.
-  uint32_t qf[NB][8][2];
-  float o[NB][8][4];
-  float m[NB][2], l[NB][2];
-  RowKeys rk[NB][2];
-  int min_limit = 0, max_lo = 0;
-  bool fresh = true;
-  int seg_tile0 = 0;
-  uint32_t merges = 0;  // uses of the merge buffer so far
-  Split rest{0, 0, 0, 0}, head{0, 0, 0, 0};
-
-  // First row of q of item (b, h).
-  auto q_row_of = [&](int b, int h) {
-    const int head = h / p.row_tiles;
-    return (static_cast<long long>(b) * p.c.Hkv + head) * p.rows + (h - head * p.row_tiles) * R;
-  };
-  auto load_q = [&](int b, int h, uint32_t(&f)[NB][8][2]) {
-    const int left = p.rows - (h % p.row_tiles) * R;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) +
-                            (q_row_of(b, h) + nb * 8 + g) * (kHeadDim / 2) + t4;
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        f[nb][kk][0] = nb * 8 + g < left ? __ldg(src + kk * 8) : 0u;
-        f[nb][kk][1] = nb * 8 + g < left ? __ldg(src + kk * 8 + 4) : 0u;
-      }
-    }
-  };
-  // With registers to spare (NB == 1) the next item's rows are fetched while this one is computed.
-  constexpr bool kAhead = NB == 1;
-  uint32_t qn[kAhead ? NB : 1][8][2];
-  if constexpr (kAhead) load_q(cx.b, cx.h, qn);
-
-  for (int i = 0; cx.u < end; ++i) {
-    const int row0 = (cx.h % p.row_tiles) * R;
-    if (fresh) {
-      fresh = false;
-      seg_tile0 = cx.tile;
-      min_limit = 0x7fffffff;
-      max_lo = 0;
-      if constexpr (kAhead) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          qf[0][kk][0] = qn[0][kk][0];
-          qf[0][kk][1] = qn[0][kk][1];
-        }
-        const bool roll = cx.h + 1 == per_seq;
-        if (cx.item + units_of(cx.t, ln.align) < end) load_q(cx.b + roll, roll ? 0 : cx.h + 1, qn);
-      } else {
-        load_q(cx.b, cx.h, qf);
-      }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int rr = row0 + nb * 8 + 2 * t4 + e;
-          rk[nb][e] = row_keys(cx.t.r, p.rule, p.c.Tq == 1 ? 0 : rr % p.c.Tq);
-          if (rr >= p.rows) rk[nb][e] = RowKeys{0x7fffffff, 0};
-          min_limit = min(min_limit, rk[nb][e].limit);
-          max_lo = max(max_lo, rk[nb][e].lo);
-          m[nb][e] = -INFINITY;
-          l[nb][e] = 0.0f;
-        }
-#pragma unroll
-        for (int a = 0; a < 8; ++a)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nb][a][e] = 0.0f;
-      }
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        min_limit = min(min_limit, __shfl_xor_sync(0xffffffffu, min_limit, d));
-        max_lo = max(max_lo, __shfl_xor_sync(0xffffffffu, max_lo, d));
-      }
-    }
-
-    cp_async_wait<kStages - 2>();
-    __syncwarp();
-    load_next();
-
-    const int key0 = slice_key(cx);
-    if (key0 < cx.t.len) {
-      const uint32_t kb = ring + (i % kStages) * (2 * kSliceBytes);
-      // S^T: lanes 0-15 address keys 0-15 of the lower 8 columns, lanes 16-31 of the upper.
-      float s[NB][2][4];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[nb][e >> 2][e & 3] = 0.0f;
-      {
-        const int row = lane & 15, up = lane >> 4;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          uint32_t a[4];
-          ldsm4(kb + row * (kHeadDim * 2) + (((2 * kk + up) ^ (row & 7)) << 4), a);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(s[nb][kk & 1], a, qf[nb][kk]);
-        }
-      }
-      // Scores of lane (g, t4): keys key0 + g (e = 0, 1) and + 8 (e = 2, 3); columns 2 t4 + (e & 1).
-      float x[NB][4];
-      bool over = false;
-      const bool masked = key0 + kSlice > min_limit ||
-                          (key0 < max_lo && key0 >= p.rule.glob * kTileKeys);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[nb][e] = (s[nb][0][e] + s[nb][1][e]) * p.scale_log2;
-          if (masked) {
-            const int key = key0 + g + (e >> 1) * 8;
-            const RowKeys k = rk[nb][e & 1];
-            if (key >= k.limit || (key < k.lo && key >= p.rule.glob * kTileKeys))
-              x[nb][e] = -INFINITY;
-          }
-          over |= x[nb][e] > m[nb][e & 1] + kRescaleLog2;
-        }
-      }
-      if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(x[nb][c], x[nb][c + 2]);
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float mn = fmaxf(m[nb][c], mx);
-            const float f = mn == -INFINITY ? 1.0f : ptx::ex2(m[nb][c] - mn);
-            m[nb][c] = mn;
-            l[nb][c] *= f;
-#pragma unroll
-            for (int a = 0; a < 8; ++a) {
-              o[nb][a][c] *= f;
-              o[nb][a][c + 2] *= f;
-            }
-          }
-      }
-      uint32_t pf[NB][2];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float pr[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float mm = m[nb][e & 1];
-          pr[e] = ptx::ex2(x[nb][e] - (mm == -INFINITY ? 0.0f : mm));
-          l[nb][e & 1] += pr[e];
-        }
-        pf[nb][0] = movm_trans(pack16<BF16>(pr[0], pr[1]));
-        pf[nb][1] = movm_trans(pack16<BF16>(pr[2], pr[3]));
-      }
-      // O^T: 16 columns of d per step; lanes 0-7 / 8-15 address keys 0-7 of the lower / upper
-      // eight columns, lanes 16-31 keys 8-15.
-      {
-        const uint32_t vb = kb + kSliceBytes;
-        const int row = (lane & 7) + ((lane >> 4) << 3), up = (lane >> 3) & 1;
-#pragma unroll
-        for (int a = 0; a < 8; ++a) {
-          uint32_t f[4];
-          ldsm4_trans(vb + row * (kHeadDim * 2) + (((2 * a + up) ^ (row & 7)) << 4), f);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(o[nb][a], f, pf[nb]);
-        }
-      }
-    }
-
-    if (cx.tile + 1 == cx.t.n || cx.u + kTileUnits >= end) {
-      // The piece ends: join the warps, eight rows at a time.  One barrier: the buffer was read long
-      // ago (o_free), and each warp adds up its share of the rows with everyone's maxima in hand.
-      const bool whole = !p.all_partial && seg_tile0 == 0 && cx.tile + 1 == cx.t.n;
-      const long long q_row = q_row_of(cx.b, cx.h);
-      const long long slot = part_slot(p.all_partial, static_cast<long long>(cx.b) * per_seq + cx.h,
-                                       static_cast<int>(blockIdx.x), seg_tile0 == 0);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if (merges > 0) wait_merge(o_free, (merges - 1) & 1u);
-        ++merges;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
-          if (g == 0) {
-            sh.m[warp][2 * t4 + c] = m[nb][c];
-            sh.l[warp][2 * t4 + c] = l[nb][c];
-          }
-        }
-#pragma unroll
-        for (int a = 0; a < 8; ++a)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sh.o[warp][2 * t4 + (e & 1)][a * 16 + g + (e >> 1) * 8] = o[nb][a][e];
-        __syncthreads();
-        const int rb = warp * kRowsPerWarp, r = nb * 8 + rb;
-        const int live = min(max(p.rows - row0 - r, 0), kRowsPerWarp);  // rows of this warp
-        float4 acc[kRowsPerWarp];
-        float mx[kRowsPerWarp], sum[kRowsPerWarp];
-#pragma unroll
-        for (int k = 0; k < kRowsPerWarp; ++k) {
-          mx[k] = -INFINITY;
-          sum[k] = 0.0f;
-          acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (k >= live) continue;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) mx[k] = fmaxf(mx[k], sh.m[w][rb + k]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float mw = sh.m[w][rb + k];
-            const float f = mw == -INFINITY ? 0.0f : ptx::ex2(mw - mx[k]);
-            const float4 y = *reinterpret_cast<const float4*>(&sh.o[w][rb + k][lane * 4]);
-            sum[k] += sh.l[w][rb + k] * f;
-            acc[k].x += y.x * f;
-            acc[k].y += y.y * f;
-            acc[k].z += y.z * f;
-            acc[k].w += y.w * f;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(o_free);
-#pragma unroll
-        for (int k = 0; k < kRowsPerWarp; ++k) {
-          if (k >= live) continue;
-          const float inv = sum[k] > 0.0f ? 1.0f / sum[k] : 0.0f;
-          const float lg = sum[k] > 0.0f ? mx[k] + log2f(sum[k]) : -INFINITY;
-          const float4 v = make_float4(acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv);
-          if (whole) {
-            store_row(p.o, p.lse, p.out_bf16, q_row + r + k, v, lg, lane);
-          } else {
-            reinterpret_cast<float4*>(p.part_o)[(slot * R + r + k) * (kHeadDim / 4) + lane] = v;
-            if (lane == 0) p.part_l[slot * R + r + k] = lg;
-          }
-        }
-      }
-      if (!whole) {
-        Split& sp = seg_tile0 == 0 ? head : rest;
-        sp.first = cx.item / ln.quota;
-        sp.last = last_piece(ln, cx.item, units_of(cx.t, ln.align));
-        sp.q_row = q_row;
-        sp.rows = min(p.rows - row0, R);
-      }
-      fresh = true;
-    }
-    advance(cx);
-  }
-  cp_async_wait<0>();
-  if (!p.all_partial && (head.rows > 0 || rest.rows > 0)) {
-    // The warp that finds its rows' pieces complete adds them up, in the order of the line.  Asked
-    // for once, at the CTA's end: the fence and the counter cost a round trip to L2 each.
-    int done[2][NB];
-    __threadfence();
-    __syncwarp();
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const Split& sp = e ? head : rest;
-        const int r = nb * 8 + warp * kRowsPerWarp;
-        done[e][nb] = -1;
-        if (lane == 0 && r < sp.rows)
-          done[e][nb] = atomicAdd(p.counters + sp.first * kFewRows + nb * kWarps + warp, 1);
-      }
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const Split& sp = e ? head : rest;
-        const int r = nb * 8 + warp * kRowsPerWarp;
-        if (__shfl_sync(0xffffffffu, done[e][nb], 0) != sp.last - sp.first || r >= sp.rows) continue;
-        __threadfence();
-        if (lane == 0) p.counters[sp.first * kFewRows + nb * kWarps + warp] = 0;
-        join_own(p, sp.q_row + r, r, min(sp.rows - r, kRowsPerWarp), R, sp.first, sp.last, lane);
-      }
-  }
-  // Behind a shared prefix this kernel starts while the prefix's still runs, and must not end
-  // before it: the join waits for this kernel only.
-  pdl_wait();
-}
 
 // Joins behind a shared prefix: every row of the call, W warps a row, over the pieces of its own
 // keys in the order of the line, then over those of the prefix.
@@ -698,7 +53,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid
   const int c0 = p.cum[b], n = p.cum[b + 1] - c0;
   const Line ln{p.cum[p.B + 1], p.cum[p.B + 2]};
   const int s = c0 * heads + hr * n;
-  const int first = s / ln.quota, own = last_piece(ln, s, n) - first + 1;
+  const int first = s / ln.quota, own = last_cta(ln, s, n) - first + 1;
   const long long item = static_cast<long long>(b) * heads + hr;
   const float *po[2] = {p.part_o, p.pre_o}, *pl[2] = {p.part_l, p.pre_l};
   const long long at[2] = {(item + first) * p.R + r, (item_p + first_p) * 128 + rp};
@@ -710,7 +65,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid
       mx = fmaxf(mx, pl[k][at[k] + static_cast<long long>(c) * step[k]]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-  PartSum acc{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f};
+  PartSum acc;
+  acc.clear();
   if (mx > -INFINITY) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -736,10 +92,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid
       acc.sum += sl[w];
     }
   }
-  const float inv = acc.sum > 0.0f ? 1.0f / acc.sum : 0.0f;
-  store_row(p.o, p.lse, p.out_bf16, row,
-            make_float4(acc.acc.x * inv, acc.acc.y * inv, acc.acc.z * inv, acc.acc.w * inv),
-            acc.sum > 0.0f ? mx + log2f(acc.sum) : -INFINITY, lane);
+  store_row(p.o, p.lse, p.out_bf16, row, acc.normal(), acc.log2_total(mx), lane);
 }
 
 // Joins the items that the many-row kernel's line was cut in: at most one begins in each CTA and
@@ -770,7 +123,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_cuts_kernel(const __grid
       mx = fmaxf(mx, p.part_l[part_slot(0, 0, first + c, c == 0) * 128 + r]);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    PartSum acc{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f};
+    PartSum acc;
+  acc.clear();
     if (mx > -INFINITY) {
 #pragma unroll 4
       for (int c = 0; c < cut.pieces; ++c) {
@@ -778,11 +132,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_cuts_kernel(const __grid
         acc.add(part_row(p.part_o, x, lane), ptx::ex2(p.part_l[x] - mx));
       }
     }
-    const float inv = acc.sum > 0.0f ? 1.0f / acc.sum : 0.0f;
     const long long row = ((static_cast<long long>(b) * p.Hkv + cut.h) * p.rt.G + g) * p.Tq + t;
-    store_row(p.o, p.lse, p.out_bf16, row,
-              make_float4(acc.acc.x * inv, acc.acc.y * inv, acc.acc.z * inv, acc.acc.w * inv),
-              acc.sum > 0.0f ? mx + log2f(acc.sum) : -INFINITY, lane);
+    store_row(p.o, p.lse, p.out_bf16, row, acc.normal(), acc.log2_total(mx), lane);
   }
 }
 
@@ -802,18 +153,9 @@ int device_sms(int* sms) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return BSATTN_E_CUDA;
     n = std::min(n, kMaxSms);
-    const void* kernels[] = {
-        reinterpret_cast<const void*>(decode_kernel<false, 1>),
-        reinterpret_cast<const void*>(decode_kernel<true, 1>),
-        reinterpret_cast<const void*>(decode_kernel<false, 2>),
-        reinterpret_cast<const void*>(decode_kernel<true, 2>)};
-    for (int i = 0; i < 4; ++i)
-      if (cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(i < 2 ? sizeof(DecodeSmem<1>)
-                                                      : sizeof(DecodeSmem<2>))) != cudaSuccess)
-        return BSATTN_E_CUDA;
-    const int rt = tile_setup();
-    if (rt != BSATTN_OK) return rt;
+    int rc2 = few_setup();
+    if (rc2 == BSATTN_OK) rc2 = tile_setup();
+    if (rc2 != BSATTN_OK) return rc2;
     known[dev] = n;
   }
   *sms = known[dev];
@@ -888,7 +230,7 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
   s->k0 = s->prefix ? prefix_len : 0;
   s->all_partial = s->prefix;
   // Most tiles one item can have.
-  const int step = s->few ? kStep : kTileKeys;
+  const int step = s->few ? kSlice : kTileKeys;
   const long long tiles = (static_cast<long long>(max_pages) * page_size + step - 1) / step + 1;
   long long items;
   if (s->few) {
@@ -908,8 +250,8 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
     if (items * tiles > (1ll << 30)) return BSATTN_E_SHAPE;
     s->rt.count = s->count = static_cast<int>(count);
   }
-  if (items * (tiles * kTileUnits + kAlign) > (1ll << 30)) return BSATTN_E_SHAPE;
-  s->pieces = static_cast<int>(std::min<long long>(s->few ? sms * kCtasPerSm : sms, items * tiles));
+  if (items * (tiles + 64) > (1ll << 30)) return BSATTN_E_SHAPE;
+  s->pieces = static_cast<int>(std::min<long long>(sms, items * tiles));
   s->slots = s->all_partial ? items + s->pieces : 2ll * s->pieces;
   s->tiles_p = s->pieces_p = 0;
   s->slots_p = 0;
@@ -940,25 +282,6 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
   s->pre_l = take(s->slots_p * 128);
   s->bytes = at;
   return BSATTN_OK;
-}
-
-// A launch that may start while its predecessor still runs.
-template <class P>
-static bool launch_overlapped(void (*kernel)(P), dim3 grid, int threads, size_t smem,
-                              cudaStream_t stream, const P& p) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess) return true;
-  cudaGetLastError();
-  return false;
 }
 
 static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix_len, int Hq,
@@ -1005,31 +328,25 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     if ((rc = tile_launch(t, page_size, stream)) != BSATTN_OK) return rc;
   }
   if (s.few) {
-    AttnParams p;
-    p.c = cache;
-    p.rule = rule;
-    p.q = q;
-    p.o = o;
-    p.lse = lse;
-    p.rows = s.rows;
-    p.row_tiles = s.row_tiles;
-    p.scale_log2 = scale_log2;
-    p.out_bf16 = out_bf16;
-    p.all_partial = s.all_partial;
-    p.cum = reinterpret_cast<int*>(base + s.cum);
-    p.part_o = reinterpret_cast<float*>(base + s.part_o);
-    p.part_l = reinterpret_cast<float*>(base + s.part_l);
-    p.counters = counters;
-    const unsigned grid = static_cast<unsigned>(s.pieces);
-    void (*kernel)(AttnParams) = s.R == 8 ? (bf16 ? decode_kernel<true, 1> : decode_kernel<false, 1>)
-                                          : (bf16 ? decode_kernel<true, 2> : decode_kernel<false, 2>);
-    const size_t smem = s.R == 8 ? sizeof(DecodeSmem<1>) : sizeof(DecodeSmem<2>);
-    if (s.prefix) {
-      if (!launch_overlapped(kernel, grid, kThreadsD, smem, stream, p)) return BSATTN_E_CUDA;
-    } else {
-      kernel<<<grid, kThreadsD, smem, stream>>>(p);
-      if (cudaGetLastError() != cudaSuccess) return BSATTN_E_CUDA;
-    }
+    FewCall f;
+    f.c = cache;
+    f.rule = rule;
+    f.q = q;
+    f.o = o;
+    f.lse = lse;
+    f.rows = s.rows;
+    f.R = s.R;
+    f.row_tiles = s.row_tiles;
+    f.scale_log2 = scale_log2;
+    f.in_bf16 = bf16;
+    f.out_bf16 = out_bf16;
+    f.all_partial = s.all_partial;
+    f.ctas = s.pieces;
+    f.cum = reinterpret_cast<int*>(base + s.cum);
+    f.part_o = reinterpret_cast<float*>(base + s.part_o);
+    f.part_l = reinterpret_cast<float*>(base + s.part_l);
+    f.counters = counters;
+    if ((rc = few_launch(f, s.prefix, stream)) != BSATTN_OK) return rc;
   }
   if (s.prefix) {
     RowJoin j;
@@ -1052,14 +369,11 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     const long long items_p = static_cast<long long>(s.rt.count) * cache.Hkv;
     j.quota_p = static_cast<int>((items_p * s.tiles_p + s.pieces_p - 1) / s.pieces_p);
     // A row of many pieces is shared by four warps.
-    const bool ok =
-        s.pieces_p / items_p >= 8
-            ? launch_overlapped(join_rows_kernel<kJoinWarps>, static_cast<unsigned>(j.total),
-                                kJoinWarps * 32, 0, stream, j)
-            : launch_overlapped(join_rows_kernel<1>,
-                                static_cast<unsigned>((j.total + kJoinWarps - 1) / kJoinWarps),
-                                kJoinWarps * 32, 0, stream, j);
-    if (!ok) return BSATTN_E_CUDA;
+    const unsigned all = static_cast<unsigned>(j.total);
+    return s.pieces_p / items_p >= 8
+               ? launch(join_rows_kernel<kJoinWarps>, dim3(all), kJoinWarps * 32, 0, true, stream, j)
+               : launch(join_rows_kernel<1>, dim3((all + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32,
+                        0, true, stream, j);
   } else if (!s.few) {
     CutJoin j;
     j.cuts = reinterpret_cast<const TileCut*>(base + s.cuts);
@@ -1072,9 +386,8 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     j.part_o = reinterpret_cast<const float*>(base + s.part_o);
     j.part_l = reinterpret_cast<const float*>(base + s.part_l);
     const unsigned groups = static_cast<unsigned>((s.rt.n_t * s.rt.G + 15) / 16);
-    if (!launch_overlapped(join_cuts_kernel, dim3(static_cast<unsigned>(s.pieces), groups),
-                           kJoinWarps * 32, 0, stream, j))
-      return BSATTN_E_CUDA;
+    return launch(join_cuts_kernel, dim3(static_cast<unsigned>(s.pieces), groups), kJoinWarps * 32, 0,
+                  true, stream, j);
   }
   return BSATTN_OK;
 }
@@ -1103,7 +416,7 @@ int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages, in
   return BSATTN_OK;
 }
 
-int bsattn_paged_counters(void) { return kMaxSms * kCtasPerSm * kFewRows; }
+int bsattn_paged_counters(void) { return kMaxSms * kFewRows; }
 
 int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, float* lse, int window,
                      int global_blocks, int prefix_len, float scale, void* scratch,

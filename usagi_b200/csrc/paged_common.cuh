@@ -89,6 +89,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -160,6 +163,26 @@ __device__ __forceinline__ void pdl_wait() {
 // ---------------------------------------------------------------- host
 // Number of SMs of the current device (checked to be sm_100).
 int device_sms(int* sms);
+
+// Launches a kernel of one parameter record; overlapped: it may start while its predecessor on the
+// stream still runs, and waits for its results with pdl_wait.
+template <class P>
+inline int launch(void (*kernel)(P), dim3 grid, int threads, size_t smem, bool overlapped,
+                  cudaStream_t stream, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlapped ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess) return BSATTN_OK;
+  cudaGetLastError();
+  return BSATTN_E_CUDA;
+}
 
 // Checks a call and fills the kernels' view of its cache (paged_attn.cu).
 int fill_cache(Cache* c, const bsattn_paged_call* call);

@@ -1,0 +1,691 @@
+// paged_few.cu -- attention of a few rows per key over a paged K/V cache: the decode form.
+//
+// Rows: q [B, Hq, Tq, 128]; the G = Hq / Hkv query heads that share a K/V head form, with their Tq
+// tokens, the G * Tq rows (g-major) that one pass over that head's keys serves.  For row (g, t) at
+// position p = seq_lens[b] - q_lens[b] + t:
+//     o = sum_j softmax_j(scale q . k_j) v_j over the keys j <= p (and the window rule),
+//     lse = ln sum_j exp(scale q . k_j);  no key: o = 0, lse = -inf.
+//
+// Every key costs 512 bytes of HBM and G * Tq * 512 operations, so the bound is memory; what matters
+// is that all SMs read all the time and that nothing waits for anything else.
+//   * Every warp is on its own.  It owns a share of the line of all (sequence, K/V head) items
+//     (paged_few.cuh), in units of 16 keys, loads its slices with cp.async into a private ring (16-byte
+//     pieces swizzled so that ldmatrix reads without bank conflicts) and keeps its own running maximum,
+//     sum and output.  The ring runs across item borders.  A short item lies inside one warp's share
+//     and is written by it, with no barrier at all; only at the CTA's end do its warps meet, once, to
+//     add up the items that lie across their shares.  Cutting by units balances sequences of any mix of
+//     lengths.  The lengths are on the device: each CTA adds them up itself.
+//   * Keys are the M dimension of the warp MMAs (m16n8k16): S^T = K Q^T and O^T = V^T P^T, so eight
+//     rows fill an MMA's N and none of it is spent on padding; P^T moves from the accumulator to the
+//     operand layout with movmatrix, in registers.
+//   * The running maximum moves only when a score passes it by more than 2^8 (then P stays within
+//     2^8, far inside fp16 and bf16); the usual step costs one vote instead of a reduction.
+//   * Parts of an item that lies across CTAs are left as (o, log2 sum) in 32 bits, and the warp that
+//     finds its row's parts complete adds them, in the order of the line: results do not depend on
+//     timing.
+// Keys past a sequence's end are loaded as zeros, never read: a recycled page may hold anything.
+// P is rounded to the type of V, as the tensor cores take it; its sum is of the unrounded values.
+#include <algorithm>
+
+#include "paged_few.cuh"
+#include "sm100_ptx.cuh"
+
+namespace bsattn {
+namespace paged {
+namespace few {
+
+constexpr int kStages = 3;
+constexpr int kSliceBytes = kSlice * kHeadDim * 2;  // 4 KB of K or of V
+constexpr int kStageBytes = 2 * kSliceBytes;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr int kAlign = 32;  // units of a CTA in a small call
+// With 16 rows per tile a warp's outputs take twice the room, so fewer warps fit.
+template <int NB>
+constexpr int kWarpsOf = NB == 1 ? 8 : 6;
+
+struct Params {
+  Cache c;
+  Rule rule;
+  const void* q;
+  void* o;
+  float* lse;
+  int rows, row_tiles;
+  float scale_log2;
+  int out_bf16, all_partial, packed;
+  int* cum;
+  float* part_o;
+  float* part_l;
+  int* counters;
+};
+
+// What a warp leaves of an item that is not its own alone: which item, and the rows' maxima and sums.
+template <int NB>
+struct Part {
+  float m[8 * NB], l[8 * NB];
+  int item;           // b * per_seq + h; < 0: none
+  int first, last;    // the CTAs it lies in
+  int live;           // its rows
+  long long q_row;    // the first of them
+};
+
+// The slices of one sequence, those any live row sees, in ascending order: n_glob leading ones, then
+// those from key `lo` on.  A sequence without a key still gets one slice, so that every row is
+// written by the same path.
+struct Slices {
+  int len;
+  Rows r;
+  int n, n_glob, lo;
+};
+__device__ __forceinline__ Slices slices_of(const Params& p, int b) {
+  const SeqLen s = seq_len(p.c, b);
+  Slices t;
+  t.len = s.len;
+  t.r = Rows{s.rows, s.len - s.rows};
+  t.lo = p.rule.k0;
+  t.n_glob = 0;
+  t.n = 1;
+  if (s.rows > 0 && s.len > p.rule.k0) {
+    if (p.rule.window > 0) {
+      const int block = max(0, max(t.r.first, 0) / kTileKeys - p.rule.window + 1);
+      t.lo = block * kTileKeys;
+      t.n_glob = min(p.rule.glob, block) * (kTileKeys / kSlice);
+    }
+    t.n = t.n_glob + (s.len - t.lo + kSlice - 1) / kSlice;
+  }
+  return t;
+}
+
+// A slice on the line.
+struct Cursor {
+  int b, h, k;  // h counts (K/V head, tile of rows)
+  int at;       // first unit of the item
+  Slices t;
+  __device__ __forceinline__ int key() const {
+    return k < t.n_glob ? k * kSlice : t.lo + (k - t.n_glob) * kSlice;
+  }
+};
+
+template <int NB>
+struct Smem {
+  uint8_t ring[kWarpsOf<NB>][kStages][kStageBytes];
+  float rest_o[kWarpsOf<NB>][8 * NB][kHeadDim];  // of the item that began before the warp's share
+  Part<NB> part[kWarpsOf<NB>][2];                // that one, and the one that goes on behind the share
+  unsigned long long warp_sum[kWarpsOf<NB>];
+  Cursor found;
+};
+
+// Where 16-byte piece c (0 .. 31) of row r of a warp's outputs lies: the four rows that the lanes of
+// an accumulator store write at once fall into different banks.
+__device__ __forceinline__ int piece(int r, int c) { return c ^ (r & 6); }
+
+// One warp, one row: o = sum_c o_c 2^(l_c - l), l = log2 sum 2^l_c over the parts of CTAs first ..
+// last, in that order, eight asked for at a time.
+__device__ __noinline__ void join_row(const Params& p, long long row, int r, int R, int first, int last,
+                                      int lane) {
+  constexpr int kAtOnce = 8;
+  const int n = last - first + 1;
+  float mx = -INFINITY;
+  PartSum s;
+  s.clear();
+  for (int c0 = 0; c0 < n; c0 += kAtOnce) {
+    float4 y[kAtOnce];
+    float lg[kAtOnce];
+#pragma unroll
+    for (int c = 0; c < kAtOnce; ++c) {
+      lg[c] = -INFINITY;
+      y[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (c0 + c < n) {
+        const long long at = part_slot(0, 0, first + c0 + c, c0 + c == 0) * R + r;
+        lg[c] = __ldcg(p.part_l + at);
+        y[c] = part_row(p.part_o, at, lane);
+      }
+    }
+    float top = mx;
+#pragma unroll
+    for (int c = 0; c < kAtOnce; ++c) top = fmaxf(top, lg[c]);
+    if (top == -INFINITY) continue;
+    s.scale(ptx::ex2(mx - top));
+    mx = top;
+#pragma unroll
+    for (int c = 0; c < kAtOnce; ++c) s.add(y[c], ptx::ex2(lg[c] - top));
+  }
+  store_row(p.o, p.lse, p.out_bf16, row, s.normal(), s.log2_total(mx), lane);
+}
+
+template <bool BF16, int NB>
+__global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_constant__ Params p) {
+  constexpr int W = kWarpsOf<NB>, kThreads = W * 32, R = 8 * NB;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem<NB>& sh = *reinterpret_cast<Smem<NB>*>(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int per_seq = p.c.Hkv * p.row_tiles;
+  pdl_trigger();
+
+  // The line: every thread adds up some sequences, in plain units and (upper half) aligned ones.
+  const int chunk = (p.c.B + kThreads - 1) / kThreads;
+  const int b0 = min(static_cast<int>(threadIdx.x) * chunk, p.c.B);
+  const int b1 = min(b0 + chunk, p.c.B);
+  unsigned long long mine = 0;
+  Slices t0;  // of sequence b0; the only one in most calls
+  for (int b = b0; b < b1; ++b) {
+    const Slices t = slices_of(p, b);
+    if (b == b0) t0 = t;
+    const int n = t.n;
+    mine += static_cast<unsigned>(units_of(n, 0)) +
+            (static_cast<unsigned long long>(units_of(n, kAlign)) << 32);
+  }
+  unsigned long long incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += up;
+  }
+  if (lane == 31) sh.warp_sum[warp] = incl;
+  __syncthreads();
+  unsigned long long total2 = 0, before2 = incl - mine;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) before2 += sh.warp_sum[w];
+    total2 += sh.warp_sum[w];
+  }
+  const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+  Line ln;
+  ln.align = static_cast<long long>(total2 >> 32) * per_seq <= static_cast<long long>(ctas) * kAlign
+                 ? kAlign : 0;
+  const int total = static_cast<int>(ln.align ? total2 >> 32 : total2 & 0xffffffffu);
+  int before = static_cast<int>(ln.align ? before2 >> 32 : before2 & 0xffffffffu);
+  const int line = total * per_seq;
+  ln.quota = ln.align ? kAlign : (line + ctas - 1) / ctas;
+  const int cta_begin =
+      static_cast<int>(min(static_cast<long long>(cta) * ln.quota, static_cast<long long>(line)));
+  const int cta_end = min(cta_begin + ln.quota, line);
+  // The item that holds the CTA's first unit.
+  for (int b = b0; b < b1; ++b) {
+    if (b > b0) t0 = slices_of(p, b);
+    const int n = units_of(t0.n, ln.align);
+    if (cta == 0 && p.all_partial) p.cum[b] = before;
+    const int rel = cta_begin - before * per_seq;
+    if (rel >= 0 && rel < n * per_seq) {
+      const int h = rel / n;
+      sh.found = Cursor{b, h, 0, before * per_seq + h * n, t0};
+    }
+    before += n;
+  }
+  if (cta == 0 && threadIdx.x == 0 && p.all_partial) {
+    p.cum[p.c.B] = total;
+    p.cum[p.c.B + 1] = ln.quota;
+    p.cum[p.c.B + 2] = ln.align;
+  }
+  __syncthreads();
+  if (cta_begin >= cta_end) {
+    pdl_wait();
+    return;
+  }
+
+  // This warp's share, and its first slice.
+  const int share = (cta_end - cta_begin + W - 1) / W;
+  const int begin = min(cta_begin + warp * share, cta_end), end = min(begin + share, cta_end);
+  auto next_item = [&](Cursor& x) {
+    x.at += units_of(x.t.n, ln.align);
+    x.k = 0;
+    if (++x.h < per_seq) return;
+    x.h = 0;
+    if (++x.b < p.c.B) x.t = slices_of(p, x.b);
+  };
+  Cursor ld = sh.found;
+  while (ld.at < end && ld.at + ld.t.n <= begin) next_item(ld);
+  ld.k = max(begin - ld.at, 0);
+  auto valid = [&](const Cursor& x) { return x.at + x.k < end; };
+  auto advance = [&](Cursor& x) {
+    if (++x.k == x.t.n) next_item(x);
+  };
+  auto page_at = [&](const Cursor& x) {
+    const int key = x.key();
+    return key < x.t.len ? __ldg(p.c.table + x.b * p.c.table_stride + (key >> p.c.page_shift)) : 0;
+  };
+  Cursor cx = ld;
+
+  // Loads.  Lane l moves piece l % 16 of rows l / 16, l / 16 + 2, ...; the page of the next slice is
+  // asked for one step ahead.
+  int ld_page = valid(ld) ? page_at(ld) : 0;
+  const uint32_t ring = ptx::smem_u32(sh.ring[warp]);
+  const int lr = lane >> 4, lc = lane & 15;
+  const uint32_t ld_dst = lr * (kHeadDim * 2) + ((lc ^ lr) << 4);
+  int ld_stage = 0;
+  auto load_next = [&]() {
+    if (valid(ld)) {
+      const int key = ld.key();
+      if (key < ld.t.len) {
+        const int page = page_checked(p.c, ld_page);
+        const long long pg = max(page, 0);
+        const long long head = ld.h / p.row_tiles;
+        const long long slot = (key & ((1 << p.c.page_shift) - 1)) + lr;
+        const char* ks = p.c.k + pg * p.c.k_page + head * p.c.k_head + slot * p.c.k_tok + lc * 16;
+        const char* vs = p.c.v + pg * p.c.v_page + head * p.c.v_head + slot * p.c.v_tok + lc * 16;
+        const uint32_t dst = ring + ld_stage * kStageBytes + ld_dst;
+        const int have = page < 0 ? 0 : ld.t.len - key - lr;
+        // Row 2 i + lr of the slice; its piece c lies at c ^ (row % 8).  With the tokens of a head side
+        // by side every address is a constant away from the first.
+        if (p.packed && page >= 0 && key + kSlice <= ld.t.len) {
+#pragma unroll
+          for (int i = 0; i < kSlice / 2; ++i) {
+            const uint32_t d = (dst ^ ((2 * i & 7) << 4)) + 2 * i * (kHeadDim * 2);
+            cp_async16(d, ks + i * (kHeadDim * 4));
+            cp_async16(d + kSliceBytes, vs + i * (kHeadDim * 4));
+          }
+        } else {
+          const char *ka[kSlice / 2], *va[kSlice / 2];
+#pragma unroll
+          for (int i = 0; i < kSlice / 2; ++i) {
+            ka[i] = ks + i * 2 * p.c.k_tok;
+            va[i] = vs + i * 2 * p.c.v_tok;
+          }
+#pragma unroll
+          for (int i = 0; i < kSlice / 2; ++i) {
+            const uint32_t d = (dst ^ ((2 * i & 7) << 4)) + 2 * i * (kHeadDim * 2);
+            const uint32_t bytes = 2 * i < have ? 16u : 0u;
+            cp_async16(d, ka[i], bytes);
+            cp_async16(d + kSliceBytes, va[i], bytes);
+          }
+        }
+      }
+      if (++ld_stage == kStages) ld_stage = 0;
+      advance(ld);
+      if (valid(ld)) ld_page = page_at(ld);
+    }
+    cp_async_commit();
+  };
+  // First row of q of an item.
+  auto q_row_of = [&](int b, int h) {
+    const int head = h / p.row_tiles;
+    return (static_cast<long long>(b) * p.c.Hkv + head) * p.rows + (h - head * p.row_tiles) * R;
+  };
+  auto load_q = [&](int b, int h, uint32_t(&f)[NB][8][2]) {
+    const int left = p.rows - (h % p.row_tiles) * R;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) +
+                            (q_row_of(b, h) + nb * 8 + g) * (kHeadDim / 2) + t4;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        f[nb][kk][0] = nb * 8 + g < left ? __ldg(src + kk * 8) : 0u;
+        f[nb][kk][1] = nb * 8 + g < left ? __ldg(src + kk * 8 + 4) : 0u;
+      }
+    }
+  };
+
+  // Per-lane state: columns (rows of q) 8 nb + 2 t4 and + 1.
+  uint32_t qf[NB][8][2];
+  float o[NB][8][4];
+  float m[NB][2], l[NB][2];
+  RowKeys rk[NB][2];
+  int min_limit = 0, max_lo = 0;
+  bool fresh = true;
+  int seg_k0 = 0;
+  int stage = 0;
+  // With registers to spare (NB == 1) the next item's rows are fetched while this one is computed.
+  constexpr bool kAhead = NB == 1;
+  uint32_t qn[kAhead ? NB : 1][8][2];
+  if constexpr (kAhead)
+    if (valid(cx)) load_q(cx.b, cx.h, qn);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load_next();
+  if (lane == 0) sh.part[warp][0].item = sh.part[warp][1].item = -1;
+  __syncwarp();
+
+  for (; valid(cx); stage = stage + 1 == kStages ? 0 : stage + 1) {
+    if (fresh) {
+      fresh = false;
+      seg_k0 = cx.k;
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          qf[0][kk][0] = qn[0][kk][0];
+          qf[0][kk][1] = qn[0][kk][1];
+        }
+        const bool roll = cx.h + 1 == per_seq;
+        if (cx.at + units_of(cx.t.n, ln.align) < end) load_q(cx.b + roll, roll ? 0 : cx.h + 1, qn);
+      } else {
+        load_q(cx.b, cx.h, qf);
+      }
+      if (p.c.Tq == 1) {
+        const RowKeys k = row_keys(cx.t.r, p.rule, 0);
+        min_limit = k.limit;
+        max_lo = k.lo;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) rk[nb][0] = rk[nb][1] = k;
+      } else {
+        min_limit = 0x7fffffff;
+        max_lo = 0;
+        const int row0 = (cx.h % p.row_tiles) * R;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int rr = row0 + nb * 8 + 2 * t4 + e;
+            rk[nb][e] = row_keys(cx.t.r, p.rule, rr % p.c.Tq);
+            if (rr >= p.rows) rk[nb][e] = RowKeys{0x7fffffff, 0};
+            min_limit = min(min_limit, rk[nb][e].limit);
+            max_lo = max(max_lo, rk[nb][e].lo);
+          }
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) {
+          min_limit = min(min_limit, __shfl_xor_sync(0xffffffffu, min_limit, d));
+          max_lo = max(max_lo, __shfl_xor_sync(0xffffffffu, max_lo, d));
+        }
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        m[nb][0] = m[nb][1] = -INFINITY;
+        l[nb][0] = l[nb][1] = 0.0f;
+#pragma unroll
+        for (int a = 0; a < 8; ++a)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nb][a][e] = 0.0f;
+      }
+    }
+
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    load_next();
+
+    const int key0 = cx.key();
+    if (key0 < cx.t.len) {
+      const uint32_t kb = ring + stage * kStageBytes;
+      // S^T: lanes 0-15 address keys 0-15 of the lower 8 columns, lanes 16-31 of the upper.
+      float s[NB][2][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[nb][e >> 2][e & 3] = 0.0f;
+      {
+        const int row = lane & 15, up = lane >> 4;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          uint32_t a[4];
+          ldsm4(kb + row * (kHeadDim * 2) + (((2 * kk + up) ^ (row & 7)) << 4), a);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(s[nb][kk & 1], a, qf[nb][kk]);
+        }
+      }
+      // Scores of lane (g, t4): keys key0 + g (e = 0, 1) and + 8 (e = 2, 3); columns 2 t4 + (e & 1).
+      float x[NB][4];
+      bool over = false;
+      const bool masked = key0 + kSlice > min_limit ||
+                          (key0 < max_lo && key0 >= p.rule.glob * kTileKeys);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[nb][e] = (s[nb][0][e] + s[nb][1][e]) * p.scale_log2;
+          if (masked) {
+            const int key = key0 + g + (e >> 1) * 8;
+            const RowKeys k = rk[nb][e & 1];
+            if (key >= k.limit || (key < k.lo && key >= p.rule.glob * kTileKeys))
+              x[nb][e] = -INFINITY;
+          }
+          over |= x[nb][e] > m[nb][e & 1] + kRescaleLog2;
+        }
+      }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(x[nb][c], x[nb][c + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float mn = fmaxf(m[nb][c], mx);
+            const float f = mn == -INFINITY ? 1.0f : ptx::ex2(m[nb][c] - mn);
+            m[nb][c] = mn;
+            l[nb][c] *= f;
+#pragma unroll
+            for (int a = 0; a < 8; ++a) {
+              o[nb][a][c] *= f;
+              o[nb][a][c + 2] *= f;
+            }
+          }
+      }
+      uint32_t pf[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float pr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float mm = m[nb][e & 1];
+          pr[e] = ptx::ex2(x[nb][e] - (mm == -INFINITY ? 0.0f : mm));
+          l[nb][e & 1] += pr[e];
+        }
+        pf[nb][0] = movm_trans(pack16<BF16>(pr[0], pr[1]));
+        pf[nb][1] = movm_trans(pack16<BF16>(pr[2], pr[3]));
+      }
+      // O^T: 16 columns of d per step; lanes 0-7 / 8-15 address keys 0-7 of the lower / upper
+      // eight columns, lanes 16-31 keys 8-15.
+      {
+        const uint32_t vb = kb + kSliceBytes;
+        const int row = (lane & 7) + ((lane >> 4) << 3), up = (lane >> 3) & 1;
+#pragma unroll
+        for (int a = 0; a < 8; ++a) {
+          uint32_t f[4];
+          ldsm4_trans(vb + row * (kHeadDim * 2) + (((2 * a + up) ^ (row & 7)) << 4), f);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(o[nb][a], f, pf[nb]);
+        }
+      }
+    }
+
+    const bool done = cx.k + 1 == cx.t.n;
+    if (done || cx.at + cx.k + 1 >= end) {
+      // The item, or this warp's part of it, ends.  Rows go through shared memory: this slice's stage,
+      // which the next load_next refills only after this, or the room for a part that is kept.
+      const bool began = seg_k0 == 0;
+      const bool keep = !(done && began);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
+      // A part that goes on behind the share is the warp's last: every copy has landed by now, and it
+      // lies in the ring (stage 0); one that began before it has room of its own.
+      const int at_end = began ? 1 : 0;
+      float* rows = keep && !began ? &sh.rest_o[warp][0][0]
+                                   : reinterpret_cast<float*>(
+                                         sh.ring[warp][keep ? 0 : stage]);
+      if (keep && began) cp_async_wait<0>();
+      __syncwarp();
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float inv[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) inv[c] = keep ? 1.0f : l[nb][c] > 0.0f ? 1.0f / l[nb][c] : 0.0f;
+#pragma unroll
+        for (int a = 0; a < 8; ++a)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = nb * 8 + 2 * t4 + (e & 1), d = a * 16 + g + (e >> 1) * 8;
+            rows[r * kHeadDim + piece(r, d >> 2) * 4 + (d & 3)] = o[nb][a][e] * inv[e & 1];
+          }
+      }
+      const int item = cx.b * per_seq + cx.h;
+      if (keep) {
+        Part<NB>& pt = sh.part[warp][at_end];
+        if (g == 0)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              pt.m[nb * 8 + 2 * t4 + c] = m[nb][c];
+              pt.l[nb * 8 + 2 * t4 + c] = l[nb][c];
+            }
+        if (lane == 0) {
+          pt.item = item;
+          pt.first = cx.at / ln.quota;
+          pt.last = last_cta(ln, cx.at, units_of(cx.t.n, ln.align));
+          pt.live = min(p.rows - (cx.h % p.row_tiles) * R, R);
+          pt.q_row = q_row_of(cx.b, cx.h);
+        }
+      } else {
+        __syncwarp();
+        const long long q_row = q_row_of(cx.b, cx.h);
+        const int live = min(p.rows - (cx.h % p.row_tiles) * R, R);
+        const long long slot = part_slot(1, item, cta, true) * R;
+        if (g == 0)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int r = nb * 8 + 2 * t4 + c;
+              const float lg = l[nb][c] > 0.0f ? m[nb][c] + log2f(l[nb][c]) : -INFINITY;
+              if (r < live) {
+                if (p.all_partial) p.part_l[slot + r] = lg;
+                else if (p.lse != nullptr) p.lse[q_row + r] = lg * 0.69314718055994531f;
+              }
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (r >= live) continue;
+          const float4 v = reinterpret_cast<const float4*>(rows)[r * (kHeadDim / 4) + piece(r, lane)];
+          if (p.all_partial)
+            reinterpret_cast<float4*>(p.part_o)[(slot + r) * (kHeadDim / 4) + lane] = v;
+          else
+            store_row(p.o, nullptr, p.out_bf16, q_row + r, v, 0.0f, lane);
+        }
+        __syncwarp();
+      }
+      fresh = true;
+    }
+    advance(cx);
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // The warps' parts in the order of the line, one per lane; runs of one item are added up, a row per
+  // warp.  An item that lies across CTAs is left for whoever completes it.
+  struct Split {
+    int first, last, live;
+    long long q_row;
+  };
+  Split split[2] = {{0, -1, 0, 0}, {0, -1, 0, 0}};
+  int turn = 0;  // spreads the rows of the runs over the warps
+  const int my_item = lane < 2 * W ? sh.part[lane >> 1][lane & 1].item : -1;
+  const uint32_t there = __ballot_sync(0xffffffffu, my_item >= 0);
+  const uint32_t below = there & ((1u << lane) - 1u);
+  const int prev_item = __shfl_sync(0xffffffffu, my_item, below ? 31 - __clz(below) : 0);
+  uint32_t starts = __ballot_sync(0xffffffffu, my_item >= 0 && (below == 0 || prev_item != my_item));
+  while (starts != 0) {
+    const int e = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const uint32_t run = there & ~((1u << e) - 1u) & (starts ? (starts & (0u - starts)) - 1u : 0xffffffffu);
+    const Part<NB>& a = sh.part[e >> 1][e & 1];
+    const int first = a.first, last = a.last, live = a.live;
+    const bool split_here = first != last;
+    const long long q_row = a.q_row;
+    const long long slot = part_slot(p.all_partial, a.item, cta, first == cta) * R;
+    int r = warp;  // a split item's row r is always warp r % W's, which counts its parts below
+    if (!split_here) {
+      r -= turn;
+      if (r < 0) r += W;
+      turn = (turn + live) % W;
+    }
+    for (; r < live; r += W) {
+      const bool in = (run >> lane) & 1u;
+      const float m_e = in ? sh.part[lane >> 1][lane & 1].m[r] : -INFINITY;
+      float mx = m_e;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const float f = m_e == -INFINITY ? 0.0f : ptx::ex2(m_e - mx);
+      float sum = in ? sh.part[lane >> 1][lane & 1].l[r] * f : 0.0f;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      PartSum s;
+      s.clear();
+      for (uint32_t left = run; left != 0; left &= left - 1) {
+        const int x = __ffs(left) - 1;
+        const float* rows = (x & 1) ? reinterpret_cast<const float*>(sh.ring[x >> 1][0])
+                                    : &sh.rest_o[x >> 1][0][0];
+        s.add(reinterpret_cast<const float4*>(rows)[r * (kHeadDim / 4) + piece(r, lane)],
+              __shfl_sync(0xffffffffu, f, x));
+      }
+      s.sum = sum;
+      const float4 v = s.normal();
+      const float lg = s.log2_total(mx);
+      if (!split_here && !p.all_partial) {
+        store_row(p.o, p.lse, p.out_bf16, q_row + r, v, lg, lane);
+      } else {
+        reinterpret_cast<float4*>(p.part_o)[(slot + r) * (kHeadDim / 4) + lane] = v;
+        if (lane == 0) p.part_l[slot + r] = lg;
+      }
+    }
+    if (split_here) {
+      const Split x{first, last, live, q_row};
+      if (first == cta) split[1] = x;
+      else split[0] = x;
+    }
+  }
+  if (!p.all_partial && (split[0].last >= 0 || split[1].last >= 0)) {
+    // Asked for once, at the CTA's end: the fence and the counters cost a round trip to L2 each.
+    constexpr int kMine = (R + W - 1) / W;  // rows of a warp
+    int done[2][kMine];
+    __threadfence();
+    __syncwarp();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r = warp + i * W;
+        done[s][i] = -1;
+        if (lane == 0 && split[s].last >= 0 && r < split[s].live)
+          done[s][i] = atomicAdd(p.counters + split[s].first * kFewRows + r, 1);
+      }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r = warp + i * W;
+        const int n = __shfl_sync(0xffffffffu, done[s][i], 0);
+        if (n < 0 || n != split[s].last - split[s].first) continue;
+        __threadfence();
+        if (lane == 0) p.counters[split[s].first * kFewRows + r] = 0;
+        join_row(p, split[s].q_row + r, r, R, split[s].first, split[s].last, lane);
+      }
+  }
+  // Behind a shared prefix this kernel starts while the prefix's still runs, and must not end before
+  // it: the join waits for this kernel only.
+  pdl_wait();
+}
+
+}  // namespace few
+
+int few_setup() {
+  using namespace few;
+  const struct {
+    const void* kernel;
+    size_t smem;
+  } all[] = {{reinterpret_cast<const void*>(few_kernel<false, 1>), sizeof(Smem<1>)},
+             {reinterpret_cast<const void*>(few_kernel<true, 1>), sizeof(Smem<1>)},
+             {reinterpret_cast<const void*>(few_kernel<false, 2>), sizeof(Smem<2>)},
+             {reinterpret_cast<const void*>(few_kernel<true, 2>), sizeof(Smem<2>)}};
+  for (const auto& k : all)
+    if (cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(k.smem)) != cudaSuccess)
+      return BSATTN_E_CUDA;
+  return BSATTN_OK;
+}
+
+int few_launch(const FewCall& c, bool overlapped, cudaStream_t stream) {
+  using namespace few;
+  // The tokens of a page and head lie side by side.
+  const int packed = c.c.k_tok == kHeadDim * 2 && c.c.v_tok == kHeadDim * 2;
+  const Params p{c.c,        c.rule,        c.q,   c.o,      c.lse,    c.rows,    c.row_tiles, c.scale_log2,
+                 c.out_bf16, c.all_partial, packed, c.cum, c.part_o, c.part_l, c.counters};
+  void (*kernel)(Params) = c.R == 8 ? (c.in_bf16 ? few_kernel<true, 1> : few_kernel<false, 1>)
+                                    : (c.in_bf16 ? few_kernel<true, 2> : few_kernel<false, 2>);
+  const int threads = 32 * (c.R == 8 ? kWarpsOf<1> : kWarpsOf<2>);
+  const size_t smem = c.R == 8 ? sizeof(Smem<1>) : sizeof(Smem<2>);
+  return launch(kernel, dim3(static_cast<unsigned>(c.ctas)), threads, smem, overlapped, stream, p);
+}
+
+}  // namespace paged
+}  // namespace bsattn
