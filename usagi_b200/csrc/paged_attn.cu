@@ -16,11 +16,10 @@
 namespace bsattn {
 namespace paged {
 
-// Joins behind a shared prefix: every row of the call, W warps a row, over the pieces of its own
-// keys in the order of the line, then over those of the prefix.
+// Joins behind a shared prefix: every row of the call, over the parts of its own keys in the order of
+// the line, then over those of the prefix: o = sum_i o_i 2^(l_i - l), l = log2 sum 2^l_i.
 struct RowJoin {
-  int Hkv, rows;         // rows = G * Tq
-  long long total;       // B * Hq * Tq
+  int Hkv, rows, groups; // rows = G * Tq; groups = B * Hkv
   void* o;
   float* lse;
   int out_bf16;
@@ -33,14 +32,91 @@ struct RowJoin {
   int n_b, tiles_p, quota_p;
 };
 constexpr int kJoinWarps = 4;
+
+// Four rows of partial results in a warp: lane l has row l % 4 and the 16-byte pieces l / 4 + 8 i.
+struct Quad {
+  float4 acc[4];
+  float sum, mx;
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    sum = 0.0f;
+    mx = -INFINITY;
+  }
+  // Parts in their order; `at` is the lane's first 16-byte piece, `step` the distance of the next.
+  // Up to four at once, so that their loads overlap.
+  template <int N>
+  __device__ __forceinline__ void add(const float4* const (&at)[N], const float (&lg)[N], int step) {
+    float4 y[N][4];
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        y[c][i] = lg[c] > -INFINITY ? __ldcg(at[c] + i * step) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float top = mx;
+#pragma unroll
+    for (int c = 0; c < N; ++c) top = fmaxf(top, lg[c]);
+    if (top == -INFINITY) return;
+    scale(ptx::ex2(mx - top));
+    mx = top;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const float w = ptx::ex2(lg[c] - top);
+      sum += w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[i].x += y[c][i].x * w;
+        acc[i].y += y[c][i].y * w;
+        acc[i].z += y[c][i].z * w;
+        acc[i].w += y[c][i].w * w;
+      }
+    }
+  }
+  __device__ __forceinline__ void scale(float f) {
+    sum *= f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
+  }
+  // Every W-th part from `from` on, of `n`: part c's log2 sum at l[c * l_step], its rows c * o_step on.
+  __device__ __forceinline__ void add_all(const float* l, long long l_step, const float4* o,
+                                          long long o_step, int step, int from, int n, int W) {
+    for (int c0 = from; c0 < n; c0 += 4 * W) {
+      const float4* at[4];
+      float lg[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const long long x = c0 + c * W;
+        lg[c] = x < n ? __ldcg(l + x * l_step) : -INFINITY;
+        at[c] = o + x * o_step;
+      }
+      add(at, lg, step);
+    }
+  }
+  __device__ __forceinline__ void store(void* o, float* lse, int out_bf16, long long row, int piece) const {
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint2*>(o)[row * (kHeadDim / 4) + piece + 8 * i] =
+          make_uint2(pack_out(acc[i].x * inv, acc[i].y * inv, out_bf16),
+                     pack_out(acc[i].z * inv, acc[i].w * inv, out_bf16));
+    if (lse != nullptr && piece == 0)
+      lse[row] = sum > 0.0f ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+  }
+};
+
+// The rows of a (sequence, K/V head) go four by four; W warps share a quad when it has many parts.
 template <int W>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid_constant__ RowJoin p) {
-  __shared__ float4 so[kJoinWarps][32];
-  __shared__ float sl[kJoinWarps];
+  __shared__ float4 so[W > 1 ? kJoinWarps : 1][4][32];
+  __shared__ float sl[kJoinWarps][4], sm[kJoinWarps][4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = W == 1 ? static_cast<long long>(blockIdx.x) * kJoinWarps + warp : blockIdx.x;
-  if (row >= p.total) return;
-  const int bh = static_cast<int>(row / p.rows), rr = static_cast<int>(row - static_cast<long long>(bh) * p.rows);
+  const int quads = (p.rows + 3) >> 2;
+  const long long quad = W == 1 ? static_cast<long long>(blockIdx.x) * kJoinWarps + warp : blockIdx.x;
+  if (quad >= static_cast<long long>(p.groups) * quads) return;
+  const int bh = static_cast<int>(quad / quads);
+  const int rr = static_cast<int>(quad - static_cast<long long>(bh) * quads) * 4 + (lane & 3);
+  const int piece = lane >> 2;
   const int b = bh / p.Hkv, h = bh - b * p.Hkv;
   const int hr = h * p.row_tiles + rr / p.R, r = rr % p.R;
   const int heads = p.Hkv * p.row_tiles;
@@ -55,44 +131,49 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid
   const int s = c0 * heads + hr * n;
   const int first = s / ln.quota, own = last_cta(ln, s, n) - first + 1;
   const long long item = static_cast<long long>(b) * heads + hr;
-  const float *po[2] = {p.part_o, p.pre_o}, *pl[2] = {p.part_l, p.pre_l};
-  const long long at[2] = {(item + first) * p.R + r, (item_p + first_p) * 128 + rp};
-  const int step[2] = {p.R, 128}, count[2] = {own, pre};
-  float mx = -INFINITY;
+  const bool live = rr < p.rows;
+  Quad x;
+  x.clear();
+  if (live) {
+    const int from = W == 1 ? 0 : warp;
+    const long long at = (item + first) * p.R + r;
+    x.add_all(p.part_l + at, p.R, reinterpret_cast<const float4*>(p.part_o) + at * (kHeadDim / 4) + piece,
+              static_cast<long long>(p.R) * (kHeadDim / 4), 8, from, own, W);
+    const long long at_p = item_p + first_p;
+    x.add_all(p.pre_l + at_p * 128 + rp, 128,
+              reinterpret_cast<const float4*>(p.pre_o) + (at_p * (kHeadDim / 4) + piece) * 128 + rp,
+              128 * (kHeadDim / 4), 8 * 128, from, pre, W);
+  }
+  if (W > 1) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int c = lane; c < count[k]; c += 32)
-      mx = fmaxf(mx, pl[k][at[k] + static_cast<long long>(c) * step[k]]);
+    for (int i = 0; i < 4; ++i) so[W > 1 ? warp : 0][i][lane] = x.acc[i];
+    if (piece == 0) {
+      sl[warp][lane & 3] = x.sum;
+      sm[warp][lane & 3] = x.mx;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    float top = x.mx;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-  PartSum acc;
-  acc.clear();
-  if (mx > -INFINITY) {
+    for (int w = 1; w < W; ++w) top = fmaxf(top, sm[w][lane & 3]);
+    x.scale(top > -INFINITY ? ptx::ex2(x.mx - top) : 0.0f);
+    x.mx = top;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll 4
-      for (int c = W == 1 ? 0 : warp; c < count[k]; c += W) {
-        const long long x = at[k] + static_cast<long long>(c) * step[k];
-        acc.add(part_row(po[k], x, lane), ptx::ex2(pl[k][x] - mx));
+    for (int w = 1; w < W; ++w) {
+      const float f = sm[w][lane & 3] > -INFINITY ? ptx::ex2(sm[w][lane & 3] - top) : 0.0f;
+      x.sum += sl[w][lane & 3] * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 y = so[W > 1 ? w : 0][i][lane];
+        x.acc[i].x += y.x * f;
+        x.acc[i].y += y.y * f;
+        x.acc[i].z += y.z * f;
+        x.acc[i].w += y.w * f;
       }
     }
   }
-  if (W > 1) {
-    so[warp][lane] = acc.acc;
-    if (lane == 0) sl[warp] = acc.sum;
-    __syncthreads();
-    if (warp != 0) return;
-#pragma unroll
-    for (int w = 1; w < W; ++w) {
-      const float4 y = so[w][lane];
-      acc.acc.x += y.x;
-      acc.acc.y += y.y;
-      acc.acc.z += y.z;
-      acc.acc.w += y.w;
-      acc.sum += sl[w];
-    }
-  }
-  store_row(p.o, p.lse, p.out_bf16, row, acc.normal(), acc.log2_total(mx), lane);
+  if (live)
+    x.store(p.o, p.lse, p.out_bf16, static_cast<long long>(bh) * p.rows + rr, piece);
 }
 
 // Joins the items that the many-row kernel's line was cut in: at most one begins in each CTA and
@@ -109,32 +190,24 @@ struct CutJoin {
 };
 __global__ void __launch_bounds__(kJoinWarps * 32) join_cuts_kernel(const __grid_constant__ CutJoin p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = (blockIdx.y * kJoinWarps + warp) * 4 + (lane & 3), piece = lane >> 2;
   const int first = blockIdx.x;
   pdl_wait();
   const TileCut cut = p.cuts[first];
   if (cut.v < 0) return;
-  const int b = cut.v / p.rt.per_seq, t0 = (cut.v - b * p.rt.per_seq) * p.rt.n_t;
-  for (int k = 0; k < 4; ++k) {
-    const int r = blockIdx.y * 16 + warp * 4 + k;
-    const int g = r / p.rt.n_t, t = t0 + r - g * p.rt.n_t;
-    if (g >= p.rt.G || t >= p.Tq) continue;
-    float mx = -INFINITY;
-    for (int c = lane; c < cut.pieces; c += 32)
-      mx = fmaxf(mx, p.part_l[part_slot(0, 0, first + c, c == 0) * 128 + r]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    PartSum acc;
-  acc.clear();
-    if (mx > -INFINITY) {
-#pragma unroll 4
-      for (int c = 0; c < cut.pieces; ++c) {
-        const long long x = part_slot(0, 0, first + c, c == 0) * 128 + r;
-        acc.add(part_row(p.part_o, x, lane), ptx::ex2(p.part_l[x] - mx));
-      }
-    }
-    const long long row = ((static_cast<long long>(b) * p.Hkv + cut.h) * p.rt.G + g) * p.Tq + t;
-    store_row(p.o, p.lse, p.out_bf16, row, acc.normal(), acc.log2_total(mx), lane);
-  }
+  const int b = cut.v / p.rt.per_seq;
+  const int g = r / p.rt.n_t, t = (cut.v - b * p.rt.per_seq) * p.rt.n_t + r - g * p.rt.n_t;
+  if (g >= p.rt.G || t >= p.Tq) return;
+  Quad x;
+  x.clear();
+  // The piece that begins the item lies in slot 2 first + 1, the others in 2 (first + 1), + 2, ...
+  const float* l = p.part_l + r;
+  const float4* o = reinterpret_cast<const float4*>(p.part_o) + piece * 128 + r;
+  constexpr int kSlot = 128 * (kHeadDim / 4);
+  const long long head = 2ll * first + 1, rest = 2ll * first + 2;
+  x.add_all(l + head * 128, 0, o + head * kSlot, 0, 8 * 128, 0, 1, 1);
+  x.add_all(l + rest * 128, 256, o + rest * kSlot, 2 * kSlot, 8 * 128, 0, cut.pieces - 1, 1);
+  x.store(p.o, p.lse, p.out_bf16, ((static_cast<long long>(b) * p.Hkv + cut.h) * p.rt.G + g) * p.Tq + t, piece);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -352,7 +425,7 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     RowJoin j;
     j.Hkv = cache.Hkv;
     j.rows = s.rows;
-    j.total = static_cast<long long>(cache.B) * Hq * cache.Tq;
+    j.groups = cache.B * cache.Hkv;
     j.o = o;
     j.lse = lse;
     j.out_bf16 = out_bf16;
@@ -368,12 +441,12 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     j.tiles_p = s.tiles_p;
     const long long items_p = static_cast<long long>(s.rt.count) * cache.Hkv;
     j.quota_p = static_cast<int>((items_p * s.tiles_p + s.pieces_p - 1) / s.pieces_p);
-    // A row of many pieces is shared by four warps.
-    const unsigned all = static_cast<unsigned>(j.total);
+    // Rows of many parts are shared by four warps.
+    const unsigned quads = static_cast<unsigned>(j.groups) * static_cast<unsigned>((s.rows + 3) / 4);
     return s.pieces_p / items_p >= 8
-               ? launch(join_rows_kernel<kJoinWarps>, dim3(all), kJoinWarps * 32, 0, true, stream, j)
-               : launch(join_rows_kernel<1>, dim3((all + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32,
-                        0, true, stream, j);
+               ? launch(join_rows_kernel<kJoinWarps>, dim3(quads), kJoinWarps * 32, 0, true, stream, j)
+               : launch(join_rows_kernel<1>, dim3((quads + kJoinWarps - 1) / kJoinWarps),
+                        kJoinWarps * 32, 0, true, stream, j);
   } else if (!s.few) {
     CutJoin j;
     j.cuts = reinterpret_cast<const TileCut*>(base + s.cuts);

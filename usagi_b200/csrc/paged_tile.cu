@@ -22,8 +22,9 @@
 //   warps 4-11  softmax, two warpgroups, keys 0..63 and 64..127 of every tile: thread t owns row t.
 //               They exchange row maxima through shared memory; the running maximum moves only when
 //               passed by more than 2^8, and O is rescaled in tensor memory only then;
-//   warps 12-15 epilogue: o = O / l, to global memory (a whole item) or through a swizzled staging
-//               buffer and TMA stores into the partial buffer.
+//   warps 12-15 epilogue: o = O / l, to o (a whole item) or to the partial buffer, which is laid out
+//               [32 pieces of four columns][128 rows] so that the threads of a warp, one row each,
+//               write side by side.
 // Tensor memory: S[2] at columns 0 and 128 (P overwrites S), O[2] at 256 and 384.  Every wait is
 // bounded; on expiry all roles leave, copies and MMAs in flight are drained and the call reports
 // BSATTN_E_TIMEOUT.
@@ -39,7 +40,9 @@ namespace paged {
 namespace tile {
 
 constexpr int kRows = 128;
-constexpr int kStages = 2;  // of K and of V each
+// Two tiles of K and of V each, and two of Q.  A third of V in place of the second Q was measured: it
+// does not help where the keys come from HBM (that is what bounds it then) and costs 2 % elsewhere.
+constexpr int kStages = 2;
 constexpr int kTileBytes = kTileKeys * kHeadDim * 2;  // 32 KB
 constexpr int kHalfBytes = kTileBytes / 2;            // 128 rows x 64 columns, 128-byte swizzle
 constexpr int kThreads = 512;
@@ -62,13 +65,14 @@ struct Params {
   Rule rule;
   RowTiles rt;
   int prefix_len;
-  int page_size, box_rows, boxes;  // rows of one box, boxes per 64-column half of a tile
+  int page_size, box_rows, box_shift, boxes;  // rows of one box (log2), boxes per 64-column half of a tile
   void* o;
   float* lse;
   int Hq;
   float scale_log2;
   int out_bf16;
   TileCut* cuts;
+  float* part_o;
   float* part_l;
   unsigned long long timeout_ns;
   int test_wait;  // test hook: the Q K^T issuer first waits on a barrier that nothing signals
@@ -84,22 +88,31 @@ struct Seg {
   int whole;
 };
 
+// The key tiles of virtual sequence v: those its last live row sees, at least one.
+struct VTiles {
+  int b0, t0, n;
+  int len, n_glob, lo_block;
+  Rows r;
+};
+
 struct alignas(1024) Smem {
   uint8_t q[2][kTileBytes];
-  uint8_t kv[2][kStages][kTileBytes];  // K, V
-  uint8_t ostage[kHalfBytes];
+  uint8_t k[kStages][kTileBytes];
+  uint8_t v[kStages][kTileBytes];
   float xmax[2][2][kRows];
   float stats[2][3][kRows];
   uint64_t q_full[2], q_empty[2];
-  uint64_t kv_full[2][kStages], kv_empty[2][kStages];
+  uint64_t k_full[kStages], k_empty[kStages];
+  uint64_t v_full[kStages], v_empty[kStages];
   uint64_t s_full[2], p_rdy[2][2], pv_done[2], xchg[2][4];
   uint64_t o_full[2], o_free[2], stats_rdy[2];
   Seg segs[kRing];
   uint64_t seg_full[kRing], seg_empty[kRing];
-  uint64_t tail[2];  // copies of a tile whose rest is filled with zeros
+  uint64_t tail[2];  // copies of a tile (of K, of V) whose rest is filled with zeros
   uint64_t drain, unsignalled;
   int warp_sum[kThreads / 32];
-  int found[3];
+  VTiles found;      // where the CTA's piece of the line starts
+  int found_v, found_h, found_tile;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -112,12 +125,6 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* map, uint3
       "r"(w), "r"(u), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void tma_store_2d(const void* map, uint32_t src, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                   map), "r"(x), "r"(y), "r"(src)
-               : "memory");
-}
-
 // ---------------------------------------------------------------- waits
 __device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, Smem& sh, const Params& p) {
   const uint64_t t0 = ptx::globaltimer_ns();
@@ -153,12 +160,6 @@ __device__ __forceinline__ void wait_drain(uint32_t bar, uint32_t parity, const 
 }
 
 // ---------------------------------------------------------------- items
-// The key tiles of virtual sequence v: those its last live row sees, at least one.
-struct VTiles {
-  int b0, t0, n;
-  int len, n_glob, lo_block;
-  Rows r;
-};
 __device__ __forceinline__ VTiles vtiles(const Params& p, int v) {
   VTiles x;
   if (p.prefix_len > 0) {
@@ -247,6 +248,8 @@ struct Stream {
   int is_v, stage;
   uint32_t phase, issued, last_parity;  // bit per stage: a copy was issued, its phase
   uint32_t tail_phase, tail_busy;
+  uint64_t *full, *empty;
+  uint8_t* tiles;
 };
 
 // Page of this lane's box (lane / 2) of the tile at key0, or -1: past the end, or no such box.
@@ -262,10 +265,10 @@ __device__ __forceinline__ bool load_tile(Smem& sh, const Params& p, Stream& x, 
                                           const Seg& s, int j, int page) {
   const int lane = threadIdx.x & 31, box = lane >> 1, half = lane & 1;
   const bool lead = lane == 0;
-  if (!wait_warp(ptx::smem_u32(&sh.kv_empty[x.is_v][x.stage]), x.phase ^ 1u, sh, p)) return false;
-  const uint32_t full = ptx::smem_u32(&sh.kv_full[x.is_v][x.stage]);
+  if (!wait_warp(ptx::smem_u32(x.empty + x.stage), x.phase ^ 1u, sh, p)) return false;
+  const uint32_t full = ptx::smem_u32(x.full + x.stage);
   const uint32_t tail = ptx::smem_u32(&sh.tail[x.is_v]);
-  const uint32_t dst = ptx::smem_u32(sh.kv[x.is_v][x.stage]);
+  const uint32_t dst = ptx::smem_u32(x.tiles) + x.stage * kTileBytes;
   const int key0 = seg_key(s, j);
   const int have = s.load_end - key0;  // rows that hold a token
   const bool mine = box < p.boxes && box * p.box_rows < have;
@@ -291,11 +294,14 @@ __device__ __forceinline__ bool load_tile(Smem& sh, const Params& p, Stream& x, 
       x.tail_busy = 0;
     }
     // Lane l writes piece l % 8 of half (l / 8) % 2, rows l / 16, + 2, ...
-    for (int row = lane >> 4; row < kTileKeys; row += 2) {
-      const bool there = row < have && ((got >> ((row / p.box_rows) * 2)) & 1u);
-      if (!there)
-        ptx::sts128(dst + ((lane >> 3) & 1) * kHalfBytes + row * 128 + (lane & 7) * 16, 0, 0, 0, 0);
+    const uint32_t at = dst + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;
+    if (hole) {
+      for (int row = lane >> 4; row < min(have, kTileKeys); row += 2)
+        if (!((got >> ((row >> p.box_shift) * 2)) & 1u)) ptx::sts128(at + row * 128, 0, 0, 0, 0);
     }
+#pragma unroll 4
+    for (int row = max(have, 0) + (lane >> 4); row < kTileKeys; row += 2)
+      ptx::sts128(at + row * 128, 0, 0, 0, 0);
     ptx::fence_async_smem();
     __syncwarp();
     if (lead) ptx::mbar_arrive(full);
@@ -310,8 +316,7 @@ __device__ __forceinline__ bool load_tile(Smem& sh, const Params& p, Stream& x, 
 __device__ __forceinline__ void drain_stream(Smem& sh, const Params& p, const Stream& x) {
   if ((threadIdx.x & 31) == 0) {
     for (int i = 0; i < kStages; ++i)
-      if ((x.issued >> i) & 1u)
-        wait_drain(ptx::smem_u32(&sh.kv_full[x.is_v][i]), (x.last_parity >> i) & 1u, p);
+      if ((x.issued >> i) & 1u) wait_drain(ptx::smem_u32(x.full + i), (x.last_parity >> i) & 1u, p);
     if (x.tail_busy) wait_drain(ptx::smem_u32(&sh.tail[x.is_v]), x.tail_phase, p);
   }
   __syncwarp();
@@ -320,10 +325,10 @@ __device__ __forceinline__ void drain_stream(Smem& sh, const Params& p, const St
 __device__ void producer_k_role(Smem& sh, const CUtensorMap* tq, const CUtensorMap* tk, const Params& p,
                                 int begin, int end, int quota) {
   const bool lead = (threadIdx.x & 31) == 0;
-  uint32_t q_issued = 0, q_last = 0;
-  Stream x{0, 0, 0, 0, 0, 0, 0};
-  int v = sh.found[0], h = sh.found[1], tl = sh.found[2];
-  VTiles vt = vtiles(p, v);
+  int q_loads = 0;
+  Stream x{0, 0, 0, 0, 0, 0, 0, sh.k_full, sh.k_empty, sh.k[0]};
+  int v = sh.found_v, h = sh.found_h, tl = sh.found_tile;
+  VTiles vt = sh.found;
   int left = end - begin;
   Seg s, next;
   // The next segment of the line (n == 0: none).
@@ -356,18 +361,6 @@ __device__ void producer_k_role(Smem& sh, const CUtensorMap* tq, const CUtensorM
   bool ok = ring_write(sh, p, 0, s, lead);
   int page = box_page(p, s, 0);
   for (int k = 0; ok && s.n > 0; ++k) {
-    const int b = k & 1;
-    const uint32_t ph = (static_cast<uint32_t>(k) >> 1) & 1u;
-    ok = wait_warp(ptx::smem_u32(&sh.q_empty[b]), ph ^ 1u, sh, p);
-    if (!ok) break;
-    if (lead) {
-      const uint32_t full = ptx::smem_u32(&sh.q_full[b]);
-      ptx::mbar_expect_tx(full, 2 * p.rt.n_t * p.rt.G * p.rt.n_b * 128);
-      for (int z = 0; z < 2; ++z)
-        tma_load_5d(ptx::smem_u32(sh.q[b]) + z * kHalfBytes, tq, full, 0, s.t0, s.h * p.rt.G, s.b0, z);
-    }
-    q_issued |= 1u << b;
-    q_last = (q_last & ~(1u << b)) | (ph << b);
     for (int j = 0; ok && j < s.n; ++j) {
       const int now = page;
       const bool last = j + 1 == s.n;
@@ -377,21 +370,32 @@ __device__ void producer_k_role(Smem& sh, const CUtensorMap* tq, const CUtensorM
       } else {
         page = box_page(p, s, j + 1);
       }
-      ok = load_tile(sh, p, x, tk, s, j, now);
+      if (j == 0) {
+        const int qb = k & 1;
+        ok = wait_warp(ptx::smem_u32(&sh.q_empty[qb]), ((static_cast<uint32_t>(k) >> 1) & 1u) ^ 1u, sh, p);
+        if (ok && lead) {
+          const uint32_t full = ptx::smem_u32(&sh.q_full[qb]);
+          ptx::mbar_expect_tx(full, 2 * p.rt.n_t * p.rt.G * p.rt.n_b * 128);
+          for (int z = 0; z < 2; ++z)
+            tma_load_5d(ptx::smem_u32(sh.q[qb]) + z * kHalfBytes, tq, full, 0, s.t0, s.h * p.rt.G, s.b0, z);
+        }
+        if (ok) ++q_loads;
+      }
+      if (ok) ok = load_tile(sh, p, x, tk, s, j, now);
       if (ok && last) ok = ring_write(sh, p, k + 1, next, lead);
     }
     s = next;
   }
   drain_stream(sh, p, x);
   if (lead)
-    for (int b = 0; b < 2; ++b)
-      if ((q_issued >> b) & 1u) wait_drain(ptx::smem_u32(&sh.q_full[b]), (q_last >> b) & 1u, p);
+    for (int i = max(q_loads - 2, 0); i < q_loads; ++i)
+      wait_drain(ptx::smem_u32(&sh.q_full[i & 1]), (static_cast<uint32_t>(i) >> 1) & 1u, p);
   __syncwarp();
 }
 
 __device__ void producer_v_role(Smem& sh, const CUtensorMap* tv, const Params& p) {
   const bool lead = (threadIdx.x & 31) == 0;
-  Stream x{1, 0, 0, 0, 0, 0, 0};
+  Stream x{1, 0, 0, 0, 0, 0, 0, sh.v_full, sh.v_empty, sh.v[0]};
   bool ok = true;
   for (int k = 0; ok; ++k) {
     const int slot = k & (kRing - 1);
@@ -417,7 +421,7 @@ template <bool BF16>
 __device__ void mma_s_role(Smem& sh, const Params& p, uint32_t tmem) {
   constexpr uint32_t idesc = ptx::idesc_f16_f32(128, 128, false, BF16);
   const uint64_t q_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.q[0]), 16, 1024);
-  const uint64_t k_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.kv[0][0]), 16, 1024);
+  const uint64_t k_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.k[0]), 16, 1024);
   if (p.test_wait && !wait_one(ptx::smem_u32(&sh.unsignalled), 0, sh, p)) return;
   Walk x;
   walk_begin(x, sh, p);
@@ -427,7 +431,7 @@ __device__ void mma_s_role(Smem& sh, const Params& p, uint32_t tmem) {
     if (x.j == 0 &&
         !wait_one(ptx::smem_u32(&sh.q_full[qb]), (static_cast<uint32_t>(x.ii) >> 1) & 1u, sh, p))
       return;
-    if (!wait_one(ptx::smem_u32(&sh.kv_full[0][sb]), tph, sh, p)) return;
+    if (!wait_one(ptx::smem_u32(&sh.k_full[sb]), tph, sh, p)) return;
     if (x.t >= 2 &&  // P V(t-2) has read the P stored in S[sb]
         !wait_one(ptx::smem_u32(&sh.pv_done[sb]), tph ^ 1u, sh, p))
       return;
@@ -439,7 +443,7 @@ __device__ void mma_s_role(Smem& sh, const Params& p, uint32_t tmem) {
       const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
       ptx::mma_ss(tmem + sb * 128, qd + off, kd + off, idesc, kk > 0 ? 1u : 0u);
     }
-    ptx::tc_commit(ptx::smem_u32(&sh.kv_empty[0][sb]));
+    ptx::tc_commit(ptx::smem_u32(&sh.k_empty[sb]));
     ptx::tc_commit(ptx::smem_u32(&sh.s_full[sb]));
     if (x.j == x.s.n - 1) ptx::tc_commit(ptx::smem_u32(&sh.q_empty[qb]));
     walk_next(x, sh, p);
@@ -449,13 +453,13 @@ __device__ void mma_s_role(Smem& sh, const Params& p, uint32_t tmem) {
 template <bool BF16>
 __device__ void mma_pv_role(Smem& sh, const Params& p, uint32_t tmem) {
   constexpr uint32_t idesc = ptx::idesc_f16_f32(128, 128, true, BF16);
-  const uint64_t v_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.kv[1][0]), kHalfBytes, 1024);
+  const uint64_t v_desc0 = ptx::sdesc_sw128(ptx::smem_u32(sh.v[0]), kHalfBytes, 1024);
   Walk x;
   walk_begin(x, sh, p);
   while (x.valid) {
     const int ob = x.ii & 1, sb = x.t & 1;
     const uint32_t tph = (static_cast<uint32_t>(x.t) >> 1) & 1u;
-    if (!wait_one(ptx::smem_u32(&sh.kv_full[1][sb]), tph, sh, p)) return;
+    if (!wait_one(ptx::smem_u32(&sh.v_full[sb]), tph, sh, p)) return;
     if (x.j == 0 && x.ii >= 2 &&  // O[ob] read out by the epilogue of segment ii - 2
         !wait_one(ptx::smem_u32(&sh.o_free[ob]), ((static_cast<uint32_t>(x.ii) >> 1) + 1u) & 1u, sh, p))
       return;
@@ -467,7 +471,7 @@ __device__ void mma_pv_role(Smem& sh, const Params& p, uint32_t tmem) {
     for (int kk = 0; kk < kTileKeys / 16; ++kk)
       ptx::mma_ts(tmem + kOCol + ob * 128, tmem + sb * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
                   vd + static_cast<uint32_t>((kk * 2048) >> 4), idesc, (x.j > 0 || kk > 0) ? 1u : 0u);
-    ptx::tc_commit(ptx::smem_u32(&sh.kv_empty[1][sb]));
+    ptx::tc_commit(ptx::smem_u32(&sh.v_empty[sb]));
     ptx::tc_commit(ptx::smem_u32(&sh.pv_done[sb]));
     if (x.j == x.s.n - 1) ptx::tc_commit(ptx::smem_u32(&sh.o_full[ob]));
     walk_next(x, sh, p);
@@ -634,7 +638,6 @@ __device__ void softmax_role(Smem& sh, const Params& p, int half, uint32_t tmem)
 // ------------------------------------------------------------------------------------------
 // Epilogue warpgroup
 // ------------------------------------------------------------------------------------------
-__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ bool epi_any(bool v) {
   uint32_t r;
   asm volatile(
@@ -644,7 +647,7 @@ __device__ __forceinline__ bool epi_any(bool v) {
   return r != 0;
 }
 
-__device__ void epilogue_role(Smem& sh, const Params& p, uint32_t tmem, const CUtensorMap* tp) {
+__device__ void epilogue_role(Smem& sh, const Params& p, uint32_t tmem) {
   const int t = threadIdx.x - kEpiWarp0 * 32;
   const int wq = t >> 5;
   const uint32_t lane_addr = tmem + (static_cast<uint32_t>(wq * 32) << 16);
@@ -697,11 +700,10 @@ __device__ void epilogue_role(Smem& sh, const Params& p, uint32_t tmem, const CU
       const int slot_o = p.prefix_len > 0
                              ? sg.v * p.c.Hkv + sg.h + static_cast<int>(blockIdx.x)
                              : 2 * static_cast<int>(blockIdx.x) + (sg.tile0 == 0 ? 1 : 0);
-      const uint32_t stage = ptx::smem_u32(sh.ostage) + static_cast<uint32_t>(t) * 128u;
+      float4* const dst = reinterpret_cast<float4*>(p.part_o) +
+                          static_cast<long long>(slot_o) * (kRows * kHeadDim / 4) + t;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
-        if (t == 0) ptx::bulk_wait_read0();
-        epi_sync();
         uint32_t orow[32];
         ptx::tmem_ld32(o_addr + c * 32, orow);
         ptx::tmem_wait_ld();
@@ -712,14 +714,9 @@ __device__ void epilogue_role(Smem& sh, const Params& p, uint32_t tmem, const CU
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          ptx::sts128(stage + static_cast<uint32_t>(k ^ (t & 7)) * 16u, orow[4 * k], orow[4 * k + 1],
-                      orow[4 * k + 2], orow[4 * k + 3]);
-        ptx::fence_async_smem();
-        epi_sync();
-        if (t == 0) {
-          tma_store_2d(tp, ptx::smem_u32(sh.ostage), c * 32, slot_o * kRows);
-          ptx::bulk_commit();
-        }
+          dst[(c * 8 + k) * kRows] =
+              make_float4(__uint_as_float(orow[4 * k]), __uint_as_float(orow[4 * k + 1]),
+                          __uint_as_float(orow[4 * k + 2]), __uint_as_float(orow[4 * k + 3]));
       }
       p.part_l[static_cast<long long>(slot_o) * kRows + t] = lg;
     }
@@ -731,42 +728,52 @@ __device__ void epilogue_role(Smem& sh, const Params& p, uint32_t tmem, const CU
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tp,
-                const __grid_constant__ Params p) {
+                const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   Smem& sh = *reinterpret_cast<Smem*>(smem_raw + (((raw + 1023u) & ~1023u) - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
 
-  if (threadIdx.x == 0) {
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(&sh.tmem_base), kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  if (warp == 2) {
+    // Side by side on the lanes of a warp: one thread would take a microsecond.
     auto init = [&](uint64_t& bar, uint32_t n) { ptx::mbar_init(ptx::smem_u32(&bar), n); };
-    for (int b = 0; b < 2; ++b) {
-      init(sh.q_full[b], 1);
-      init(sh.q_empty[b], 1);
-      init(sh.s_full[b], 1);
-      init(sh.p_rdy[b][0], 128);
-      init(sh.p_rdy[b][1], 128);
-      init(sh.pv_done[b], 1);
-      init(sh.o_full[b], 1);
-      init(sh.o_free[b], 128);
-      init(sh.stats_rdy[b], 256);
-      for (int q = 0; q < 4; ++q) init(sh.xchg[b][q], 64);
+    if (lane < 2) {
+      init(sh.s_full[lane], 1);
+      init(sh.pv_done[lane], 1);
+      init(sh.o_full[lane], 1);
+      init(sh.o_free[lane], 128);
+      init(sh.stats_rdy[lane], 256);
+      init(sh.tail[lane], 1);
+      init(sh.q_full[lane], 1);
+      init(sh.q_empty[lane], 1);
+    } else if (lane < 6) {
+      init(sh.p_rdy[(lane - 2) >> 1][lane & 1], 128);
+      init(sh.xchg[0][lane - 2], 64);
+      init(sh.xchg[1][lane - 2], 64);
+    } else if (lane < 6 + kStages) {
+      init(sh.k_full[lane - 6], 1);
+      init(sh.k_empty[lane - 6], 1);
+      init(sh.v_full[lane - 6], 1);
+      init(sh.v_empty[lane - 6], 1);
+    } else if (lane >= 16 && lane < 16 + kRing) {
+      init(sh.seg_full[lane - 16], 1);
+      init(sh.seg_empty[lane - 16], kRingReaders);
+    } else if (lane == 31) {
+      init(sh.drain, 2);
+      init(sh.unsignalled, 1);
+      sh.abort_flag = 0;
     }
-    for (int i = 0; i < 2 * kStages; ++i) {
-      init(sh.kv_full[i / kStages][i % kStages], 1);
-      init(sh.kv_empty[i / kStages][i % kStages], 1);
-    }
-    for (int i = 0; i < kRing; ++i) {
-      init(sh.seg_full[i], 1);
-      init(sh.seg_empty[i], kRingReaders);
-    }
-    init(sh.tail[0], 1);
-    init(sh.tail[1], 1);
-    init(sh.drain, 2);
-    init(sh.unsignalled, 1);
-    sh.abort_flag = 0;
     ptx::fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::tma_prefetch_desc(&tq);
+    ptx::tma_prefetch_desc(&tk);
+    ptx::tma_prefetch_desc(&tv);
   }
 
   // This CTA's piece of the line (as in the few-row kernel).
@@ -774,7 +781,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int v0 = min(static_cast<int>(threadIdx.x) * chunk, p.rt.count);
   const int v1 = min(v0 + chunk, p.rt.count);
   int mine = 0;
-  for (int v = v0; v < v1; ++v) mine += vtiles(p, v).n;
+  VTiles vt;  // of v0, the only one in most calls
+  for (int v = v0; v < v1; ++v) {
+    const VTiles y = vtiles(p, v);
+    if (v == v0) vt = y;
+    mine += y.n;
+  }
   int incl = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -793,32 +805,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int begin = min(static_cast<int>(blockIdx.x) * quota, line);
   const int end = min(begin + quota, line);
   for (int v = v0; v < v1; ++v) {
-    const int n = vtiles(p, v).n;
+    if (v > v0) vt = vtiles(p, v);
+    const int n = vt.n;
     const int rel = begin - before * p.c.Hkv;
     if (rel >= 0 && rel < n * p.c.Hkv) {
-      sh.found[0] = v;
-      sh.found[1] = rel / n;
-      sh.found[2] = rel % n;
+      sh.found = vt;
+      sh.found_v = v;
+      sh.found_h = rel / n;
+      sh.found_tile = rel % n;
     }
     before += n;
   }
   if (threadIdx.x == 0 && p.prefix_len == 0) p.cuts[blockIdx.x] = TileCut{-1, 0, 0, 0};
-  if (warp == 0 && lane == 0) {
-    ptx::tma_prefetch_desc(&tq);
-    ptx::tma_prefetch_desc(&tk);
-    ptx::tma_prefetch_desc(&tv);
-    ptx::tma_prefetch_desc(&tp);
-  }
-  __syncthreads();
-  if (begin >= end) return;  // the whole CTA
-  if (warp == 1) {
-    ptx::tmem_alloc(ptx::smem_u32(&sh.tmem_base), kTmemCols);
-    ptx::tmem_relinquish();
-  }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
+  if (begin >= end) {  // the whole CTA
+    if (warp == 1) ptx::tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
 
   if (warp >= kSoftmaxWarp0 && warp < kEpiWarp0) {
     ptx::setmaxnreg_inc<kSoftmaxRegs>();
@@ -836,8 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     ptx::setmaxnreg_dec<kEpilogueRegs>();
-    epilogue_role(sh, p, tmem, &tp);
-    if (threadIdx.x == kEpiWarp0 * 32) ptx::bulk_wait0();
+    epilogue_role(sh, p, tmem);
   }
   __syncwarp();
   ptx::tmem_wait_ld();
@@ -914,7 +919,9 @@ int tile_launch(const TileCall& call, int page_size, cudaStream_t stream) {
   Params p;
   p.box_rows = std::min(page_size, kTileKeys);
   p.boxes = kTileKeys / p.box_rows;
-  CUtensorMap tq, tk, tv, tp;
+  p.box_shift = 0;
+  while ((1 << p.box_shift) < p.box_rows) ++p.box_shift;
+  CUtensorMap tq, tk, tv;
   int rc;
   {
     const cuuint64_t tok = kHeadDim * 2, head = tok * c.Tq, seq = head * call.Hq;
@@ -937,13 +944,6 @@ int tile_launch(const TileCall& call, int page_size, cudaStream_t stream) {
     const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(p.box_rows), 1, 1, 1};
     if ((rc = encode(i ? &tv : &tk, type, 5, i ? c.v : c.k, dims, strides, box)) != BSATTN_OK) return rc;
   }
-  {
-    const cuuint64_t dims[2] = {kHeadDim, static_cast<cuuint64_t>(call.slots) * kRows};
-    const cuuint64_t strides[1] = {kHeadDim * sizeof(float)};
-    const cuuint32_t box[2] = {32, kRows};
-    if ((rc = encode(&tp, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, call.part_o, dims, strides, box)) != BSATTN_OK)
-      return rc;
-  }
   p.c = c;
   p.rule = call.rule;
   p.rt = rt;
@@ -955,14 +955,15 @@ int tile_launch(const TileCall& call, int page_size, cudaStream_t stream) {
   p.scale_log2 = call.scale_log2;
   p.out_bf16 = call.out_bf16;
   p.cuts = call.cuts;
+  p.part_o = call.part_o;
   p.part_l = call.part_l;
   p.timeout_ns = launch_timeout_ns();
   p.test_wait = launch_test_wait();
   const unsigned grid = static_cast<unsigned>(call.pieces);
   if (call.in_bf16)
-    tile_kernel<true><<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, tp, p);
+    tile_kernel<true><<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, p);
   else
-    tile_kernel<false><<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, tp, p);
+    tile_kernel<false><<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? BSATTN_OK : BSATTN_E_CUDA;
 }
 

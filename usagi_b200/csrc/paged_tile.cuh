@@ -34,7 +34,7 @@ struct TileCall {
   int pieces;      // CTAs
   long long slots; // partial outputs of 128 rows
   TileCut* cuts;   // [pieces], without a prefix
-  float* part_o;   // [slots, 128, 128]
+  float* part_o;   // [slots][32 pieces of four columns][128 rows]
   float* part_l;   // [slots, 128], log2
 };
 
