@@ -75,21 +75,35 @@ def test_window_and_global_blocks(window, glob, Tq, Hq):
     check_attention(o, lse, attention(q, c, None, window, glob))
 
 
-# (prefix, own lens, Hq, Hkv, Tq, q_lens, page, dtype, layout)
+def _cycle(values, n):
+    return [values[i % len(values)] for i in range(n)]
+
+
+# (prefix, own lens, Hq, Hkv, Tq, q_lens, page, dtype, layout).  A prefix is read once when that saves
+# 128 MB (512 bytes a token and head for every sequence but one); the first seven save less.
 SHARED = {
     "small": (64, [1, 7, 30], 8, 2, 1, None, 16, F16, "hnd"),
     "no_prefix": (0, [100, 40], 4, 2, 1, None, 32, BF16, "hnd"),
-    "ends_inside_a_tile": (336, [1, 200, 129], 8, 2, 1, None, 16, BF16, "nhd"),
-    "whole_tiles": (512, [3] * 9, 16, 2, 1, None, 128, F16, "hnd"),
-    "odd_group_many": (272, list(range(1, 60)), 6, 2, 1, None, 16, F16, "hnd"),
-    "group7": (400, list(range(1, 40)), 7, 1, 1, None, 16, BF16, "hnd"),
     "drafts": (320, [5, 6, 70, 9, 33], 8, 2, 5, [5, 2, 0, 4, 5], 64, F16, "nhd"),
     "chunks": (256, [70, 200], 4, 2, 70, [70, 33], 32, BF16, "hnd"),
     "long_chunks": (256, [300], 2, 1, 300, None, 64, F16, "hnd"),
     "one_sequence": (1280, [1], 4, 4, 1, None, 64, F16, "hnd"),
-    "wide": (2048, [1 + b % 17 for b in range(130)], 4, 1, 1, None, 64, BF16, "hnd"),
     "shorter_than_the_prefix": (256, [-256, -100, -1, 0, 1, 40], 8, 2, 1, None, 64, F16, "hnd"),
-    "rows_end_inside_the_prefix": (256, [-100, 3, 2], 4, 2, 8, [8, 8, 1], 64, BF16, "hnd"),
+    "once_ends_inside_a_tile": (2064, _cycle([1, 200, 129], 130), 8, 1, 1, None, 16, BF16, "nhd"),
+    "once_whole_tiles": (2048, [3] * 67, 16, 2, 1, None, 128, F16, "hnd"),
+    "once_odd_group": (2096, list(range(1, 67)), 6, 2, 1, None, 16, F16, "hnd"),
+    "once_group7": (2064, list(range(1, 131)), 7, 1, 1, None, 16, BF16, "hnd"),
+    "once_group16": (2080, _cycle([1, 140, 33], 130), 16, 1, 1, None, 32, F16, "nhd"),
+    "once_equal_heads": (1040, _cycle([5, 60], 66), 4, 4, 1, None, 16, BF16, "hnd"),
+    "once_drafts": (2112, _cycle([5, 6, 70, 9, 33], 130), 4, 1, 5, _cycle([5, 2, 0, 4, 5], 130), 64,
+                    F16, "nhd"),
+    "once_rows33": (2064, _cycle([11, 40], 130), 3, 1, 11, _cycle([11, 3], 130), 16, BF16, "hnd"),
+    "once_rows64": (2048, [70] * 130, 4, 1, 16, None, 256, F16, "hnd"),
+    "once_shorter": (4096, _cycle([-4096, -3000, -1, 0, 1, 40, -90], 66), 4, 1, 1, None, 64, F16,
+                     "hnd"),
+    "once_rows_end_inside": (4096, _cycle([-100, 3, 2, -1, -4090], 66), 4, 1, 8,
+                             _cycle([8, 8, 1, 0, 8], 66), 64, BF16, "hnd"),
+    "once_few_long_rows": (32768, [40, 1, 7], 8, 4, 1, None, 64, F16, "hnd"),
 }
 
 
@@ -117,25 +131,32 @@ def test_scores_far_apart():
     q = _q(2, 8, 1, F16, 42, gain=4.0)
     o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV))
     check_attention(o, lse, attention(q, c))
-    o2, lse2 = ub.shared_prefix_attn_fwd(q[:1].to(DEV).contiguous(), *[
-        x[:1] if i > 1 else x for i, x in enumerate(c.to(DEV))], prefix_len=1024)
-    check_attention(o2, lse2, [x[:1] for x in attention(q, c)])
+    # more rows on the same keys
+    q = _q(2, 8, 7, F16, 43, gain=4.0)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV))
+    check_attention(o, lse, attention(q, c))
+    # and one of the sequences as a prefix that 130 rows share
+    args = [x[:1].expand(130, *x.shape[1:]) if i > 1 else x for i, x in enumerate(c.to(DEV))]
+    q = _q(130, 8, 1, F16, 44, gain=4.0)
+    o, lse = ub.shared_prefix_attn_fwd(q.to(DEV), *args, prefix_len=1024)
+    c.table, c.lens = c.table[:1].expand(130, -1), [c.lens[0]] * 130
+    check_attention(o, lse, attention(q, c))
     ub.check_errors(DEV)
 
 
-@pytest.mark.parametrize("prefix", [0, 256])
-def test_options(prefix):
+@pytest.mark.parametrize("prefix,B,Tq", [(0, 2, 1), (0, 2, 3), (256, 2, 3), (2048, 66, 2)])
+def test_options(prefix, B, Tq):
     """Scale, output type, given outputs, no lse, int64 metadata, a strided table and q."""
-    c = Cache([300, 500], 2, 64, BF16, 51, DEV, prefix=prefix)
-    q = _q(2, 4, 3, BF16, 52)
+    c = Cache(_cycle([prefix + 44, prefix + 244], B), 2, 64, BF16, 51, DEV, prefix=prefix)
+    q = _q(B, 4, Tq, BF16, 52)
     kp, vp, table, lens = c.to(DEV)
     kw = dict(prefix_len=prefix) if prefix else {}
     fn = ub.shared_prefix_attn_fwd if prefix else ub.paged_attn_fwd
     qs = q.transpose(1, 2).contiguous().to(DEV).transpose(1, 2)
-    wide = torch.full((2, 2 * table.shape[1]), -1, dtype=torch.int32, device=DEV)
+    wide = torch.full((B, 2 * table.shape[1]), -1, dtype=torch.int32, device=DEV)
     wide[:, :table.shape[1]] = table
-    out = torch.empty(2, 4, 3, 128, device=DEV, dtype=F16)
-    lse = torch.empty(2, 4, 3, device=DEV)
+    out = torch.empty(B, 4, Tq, 128, device=DEV, dtype=F16)
+    lse = torch.empty(B, 4, Tq, device=DEV)
     o, l2 = fn(qs, kp, vp, wide[:, :table.shape[1]], lens.long(), scale=0.05, out_dtype=F16,
                out=out, lse_out=lse, **kw)
     assert o is out and l2 is lse
@@ -244,44 +265,51 @@ def _expect_page_error():
     ub.check_errors(DEV)  # cleared
 
 
-@pytest.mark.parametrize("prefix", [0, 128])
-@pytest.mark.parametrize("Tq", [1, 40])
-def test_bad_pages_and_lengths_are_reported(prefix, Tq):
+@pytest.mark.parametrize("prefix,B,Tq", [(0, 3, 1), (0, 3, 40), (128, 3, 1), (2048, 66, 3)])
+def test_bad_pages_and_lengths_are_reported(prefix, B, Tq):
     """Out-of-range table entries, lengths and row counts are found and reported; the sequences
     that are in order keep their results."""
-    c = Cache([200, 190, 180], 2, 16, F16, 81, DEV, prefix=prefix)
-    q = _q(3, 4, Tq, F16, 82).to(DEV)
+    lens_ = _cycle([prefix + 200, prefix + 190, prefix + 180], B)
+    c = Cache(lens_, 2, 16, F16, 81, DEV, prefix=prefix)
+    q = _q(B, 4, Tq, F16, 82).to(DEV)
     kp, vp, table, lens = c.to(DEV)
     fn = (lambda *a, **k: ub.shared_prefix_attn_fwd(*a, prefix_len=prefix, **k)) if prefix \
         else ub.paged_attn_fwd
     ref = fn(q, kp, vp, table, lens)
     ub.check_errors(DEV)
     want = attention(q.cpu(), c)
+    others = [b for b in range(B) if b != 1]
 
-    def in_order(o, lse, *which):
-        for b in which:
-            check_attention(o[b:b + 1], lse[b:b + 1], [x[b:b + 1] for x in want])
+    def in_order(o, lse, which):
+        check_attention(o[which], lse[which], [x[which] for x in want])
 
+    in_order(*ref, list(range(B)))
     for value in (-1, kp.shape[0], 2 ** 31 - 1):
         bad = table.clone()
-        bad[1, 9] = value
+        bad[1, prefix // 16 + 9] = value
         o, lse = fn(q, kp, vp, bad, lens)
         _expect_page_error()
-        for b in (0, 2):
+        for b in others:
             assert torch.equal(o[b], ref[0][b]) and torch.equal(lse[b], ref[1][b])
     for value in (-5, table.shape[1] * 16 + 1, 2 ** 31 - 1):
         bad = lens.clone()
-        bad[0] = value
+        bad[1] = value
         # the pages a longer length reaches exist in the table's width only
         ok = table.clamp(min=0)
         o, lse = fn(q, kp.nan_to_num(), vp.nan_to_num(), ok, bad)
         _expect_page_error()
-        in_order(o, lse, 1, 2)
+        in_order(o, lse, others)
     for value in (-1, Tq + 1, 2 ** 31 - 1):
-        ql = torch.tensor([Tq, value, Tq], dtype=torch.int32, device=DEV)
+        ql = torch.full((B,), Tq, dtype=torch.int32, device=DEV)
+        ql[1] = value
         o, lse = fn(q, kp, vp, table, lens, q_lens=ql)
         _expect_page_error()
-        in_order(o, lse, 0, 2)
+        in_order(o, lse, others)
+    if prefix:
+        bad = table.clone()
+        bad[0, 5] = kp.shape[0]
+        fn(q, kp, vp, bad, lens)
+        _expect_page_error()
 
 
 def test_append_reports_bad_pages_and_writes_nothing_there():
@@ -301,41 +329,41 @@ def test_append_reports_bad_pages_and_writes_nothing_there():
     _expect_page_error()
 
 
-def test_results_do_not_depend_on_the_run():
-    c = Cache([5000, 3, 777, 1200], 2, 32, BF16, 91, DEV)
-    q = _q(4, 8, 1, BF16, 92).to(DEV)
+def _three_calls(seed):
+    """A call for each of the ways through the attention kernels, with its arguments."""
+    c = Cache([5000 + seed, 3, 777, 1200], 2, 32, BF16, 91 + seed, DEV)
+    one, many = _q(4, 8, 1, BF16, 92 + seed).to(DEV), _q(4, 8, 9, BF16, 93 + seed).to(DEV)
     args = c.to(DEV)
-    first = ub.paged_attn_fwd(q, *args)
-    shared = ub.shared_prefix_attn_fwd(q[:1].contiguous(), *args[:2], args[2][:1], args[3][:1],
-                                       prefix_len=4096)
+    p = Cache(_cycle([2048 + 40 + seed, 2048 + 7], 66), 2, 64, BF16, 94 + seed, DEV, prefix=2048)
+    shared, pargs = _q(66, 4, 1, BF16, 95 + seed).to(DEV), p.to(DEV)
+    return [lambda: ub.paged_attn_fwd(one, *args), lambda: ub.paged_attn_fwd(many, *args),
+            lambda: ub.shared_prefix_attn_fwd(shared, *pargs, prefix_len=2048)]
+
+
+def test_results_do_not_depend_on_the_run():
+    calls = _three_calls(0)
+    first = [f() for f in calls]
     for _ in range(5):
-        o, lse = ub.paged_attn_fwd(q, *args)
-        assert torch.equal(o, first[0]) and torch.equal(lse, first[1])
-        o, lse = ub.shared_prefix_attn_fwd(q[:1].contiguous(), *args[:2], args[2][:1], args[3][:1],
-                                           prefix_len=4096)
-        assert torch.equal(o, shared[0]) and torch.equal(lse, shared[1])
+        for f, w in zip(calls, first):
+            o, lse = f()
+            assert torch.equal(o, w[0]) and torch.equal(lse, w[1])
     ub.check_errors(DEV)
 
 
 def test_two_graphs_side_by_side():
     """Two graphs captured on one stream and replayed at once on two: nothing is shared."""
     side = torch.cuda.Stream(DEV)
-    sets = []
-    for s in range(2):
-        c = Cache([4000 + 100 * s, 900], 2, 32, F16, 101 + s, DEV, prefix=512)
-        q = _q(2, 4, 1, F16, 103 + s).to(DEV)
-        sets.append((q, c.to(DEV)))
     side.wait_stream(torch.cuda.current_stream(DEV))
     want, outs, graphs = [], [], []
     with torch.cuda.stream(side):
-        for q, a in sets:
-            want.append([*ub.paged_attn_fwd(q, *a), *ub.shared_prefix_attn_fwd(q, *a, prefix_len=512)])
+        sets = [_three_calls(s) for s in range(2)]
+        for calls in sets:
+            want.append([x for f in calls for x in f()])
         side.synchronize()
-        for q, a in sets:
+        for calls in sets:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=side):
-                outs.append([*ub.paged_attn_fwd(q, *a),
-                             *ub.shared_prefix_attn_fwd(q, *a, prefix_len=512)])
+                outs.append([x for f in calls for x in f()])
             graphs.append(graph)
     streams = [torch.cuda.Stream(DEV) for _ in range(2)]
     for rep in range(20):
@@ -346,12 +374,36 @@ def test_two_graphs_side_by_side():
         for s, graph in zip(streams, graphs):
             with torch.cuda.stream(s):
                 graph.replay()
+        # eager calls of the same sizes between the replays, on a third stream
+        eager = [x for f in sets[0] for x in f()]
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert all(torch.equal(x, y) for x, y in zip(o, w)), rep
+        assert all(torch.equal(x, y) for x, y in zip(eager, want[0])), rep
     with torch.cuda.stream(side):
         ub.check_errors(DEV)
+    ub.check_errors(DEV)
     del graphs
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams: each stream has its own scratch and counters."""
+    sets = [_three_calls(s) for s in range(2)]
+    want = [[x for f in calls for x in f()] for calls in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    for rep in range(10):
+        outs = [[], []]
+        for _ in range(3):
+            for s, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    outs[s] = [x for f in sets[s] for x in f()]
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(x, y) for x, y in zip(o, w)), rep
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            ub.check_errors(DEV)
 
 
 def test_offsets_past_32_bits():
@@ -369,8 +421,9 @@ def test_offsets_past_32_bits():
     want = attention(q, c)
     o, lse = ub.paged_attn_fwd(q.to(DEV), kp, vp, table, lens)
     check_attention(o, lse, want)
-    o, lse = ub.shared_prefix_attn_fwd(q.to(DEV), kp, vp, table, lens, prefix_len=18 * page)
-    check_attention(o, lse, want)
+    many = _q(1, 16, 9, F16, 114)
+    o, lse = ub.paged_attn_fwd(many.to(DEV), kp, vp, table, lens)
+    check_attention(o, lse, attention(many, c))
     x = torch.randn(1, Hkv, 1, 128, generator=torch.Generator().manual_seed(113)).half().to(DEV)
     ub.paged_kv_append(kp, vp, table, lens, x, x)
     at = table[0, (L - 1) // page].item(), (L - 1) % page
@@ -421,11 +474,7 @@ def test_prefill_then_decode(window, glob):
 def test_wait_timeout_is_reported_and_context_survives():
     """The many-row kernel's waits are bounded: with the test hook its Q K^T issuers wait on a barrier
     that nothing signals, the bound runs out on every SM, and the host reads the status."""
-    c = Cache([900, 500], 2, 32, F16, 131, DEV, prefix=256)
-    args = c.to(DEV)
-    calls = [lambda q=_q(2, 4, 40, F16, 132).to(DEV): ub.paged_attn_fwd(q, *args),
-             lambda q=_q(2, 4, 1, F16, 133).to(DEV): ub.shared_prefix_attn_fwd(q, *args,
-                                                                            prefix_len=256)]
+    calls = _three_calls(0)[1:]
     want = [f() for f in calls]
     ub.check_errors(DEV)
     lib = _lib.load()

@@ -2,7 +2,7 @@
 // of partial results.
 //
 // Rows of q that share a K/V head (G = Hq / Hkv query heads, Tq tokens) go together:
-//   * up to 16 rows: the few-row kernel (paged_few.cu), which is bound by memory;
+//   * up to 8 rows: the few-row kernel (paged_few.cu), which is bound by memory;
 //   * more: the many-row kernel (paged_tile.cu), tiles of 128 rows on the tensor cores;
 //   * behind a shared prefix: the prefix's keys by the many-row kernel, over the stacked rows of the
 //     whole batch, the sequences' own keys by the few-row kernel at the same time, and a join of both.
@@ -290,6 +290,11 @@ struct Shape {
 };
 
 constexpr int kStackedRows = 64; // more rows of one sequence fill a tile without its neighbours
+// A prefix is read once when that saves at least this much reading; below, three launches and a join
+// cost more than the bytes, which L2 serves.  Measured, one pass over everything against prefix once,
+// 32 query heads on 8: 8 sequences behind 4,096 tokens (117 MB saved) 24.8 and 25.3 us, 16 behind 4,096
+// (252 MB) 36.8 and 27.3, 64 behind 1,024 (264 MB) 38.2 and 25.8, 16 behind 1,024 (63 MB) 18.6 and 22.1.
+constexpr long long kSharedBytes = 128ll << 20;
 
 static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size, int prefix_len,
                     int sms, Shape* s) {
@@ -298,7 +303,8 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
   const long long rows = static_cast<long long>(G) * Tq;
   if (rows * B * Hkv > (1ll << 31) - 1) return BSATTN_E_SHAPE;
   s->rows = static_cast<int>(rows);
-  s->prefix = prefix_len > 0 && rows <= kStackedRows;
+  const long long saved = static_cast<long long>(B - 1) * prefix_len * Hkv * (4 * kHeadDim);
+  s->prefix = prefix_len > 0 && rows <= kStackedRows && saved >= kSharedBytes;
   s->few = s->prefix || rows <= kFewRows || G > 128;
   s->k0 = s->prefix ? prefix_len : 0;
   s->all_partial = s->prefix;
@@ -307,8 +313,8 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
   const long long tiles = (static_cast<long long>(max_pages) * page_size + step - 1) / step + 1;
   long long items;
   if (s->few) {
-    s->R = rows <= 8 ? 8 : kFewRows;
-    s->row_tiles = static_cast<int>((rows + s->R - 1) / s->R);
+    s->R = kFewRows;
+    s->row_tiles = static_cast<int>((rows + kFewRows - 1) / kFewRows);
     s->count = B;
     items = static_cast<long long>(B) * Hkv * s->row_tiles;
   } else {
@@ -408,7 +414,6 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     f.o = o;
     f.lse = lse;
     f.rows = s.rows;
-    f.R = s.R;
     f.row_tiles = s.row_tiles;
     f.scale_log2 = scale_log2;
     f.in_bf16 = bf16;

@@ -39,9 +39,7 @@ constexpr int kSliceBytes = kSlice * kHeadDim * 2;  // 4 KB of K or of V
 constexpr int kStageBytes = 2 * kSliceBytes;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kAlign = 32;  // units of a CTA in a small call
-// With 16 rows per tile a warp's outputs take twice the room, so fewer warps fit.
-template <int NB>
-constexpr int kWarpsOf = NB == 1 ? 8 : 6;
+constexpr int kWarps = 8, kThreads = kWarps * 32;
 
 struct Params {
   Cache c;
@@ -59,9 +57,8 @@ struct Params {
 };
 
 // What a warp leaves of an item that is not its own alone: which item, and the rows' maxima and sums.
-template <int NB>
 struct Part {
-  float m[8 * NB], l[8 * NB];
+  float m[kFewRows], l[kFewRows];
   int item;           // b * per_seq + h; < 0: none
   int first, last;    // the CTAs it lies in
   int live;           // its rows
@@ -105,12 +102,11 @@ struct Cursor {
   }
 };
 
-template <int NB>
 struct Smem {
-  uint8_t ring[kWarpsOf<NB>][kStages][kStageBytes];
-  float rest_o[kWarpsOf<NB>][8 * NB][kHeadDim];  // of the item that began before the warp's share
-  Part<NB> part[kWarpsOf<NB>][2];                // that one, and the one that goes on behind the share
-  unsigned long long warp_sum[kWarpsOf<NB>];
+  uint8_t ring[kWarps][kStages][kStageBytes];
+  float rest_o[kWarps][kFewRows][kHeadDim];    // of the item that began before the warp's share
+  Part part[kWarps][2];                        // that one, and the one that goes on behind the share
+  unsigned long long warp_sum[kWarps];
   Cursor found;
 };
 
@@ -152,11 +148,11 @@ __device__ __noinline__ void join_row(const Params& p, long long row, int r, int
   store_row(p.o, p.lse, p.out_bf16, row, s.normal(), s.log2_total(mx), lane);
 }
 
-template <bool BF16, int NB>
-__global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_constant__ Params p) {
-  constexpr int W = kWarpsOf<NB>, kThreads = W * 32, R = 8 * NB;
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant__ Params p) {
+  constexpr int W = kWarps, R = kFewRows;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  Smem<NB>& sh = *reinterpret_cast<Smem<NB>*>(smem_raw);
+  Smem& sh = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int per_seq = p.c.Hkv * p.row_tiles;
@@ -224,8 +220,8 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
   }
 
   // This warp's share, and its first slice.
-  const int share = (cta_end - cta_begin + W - 1) / W;
-  const int begin = min(cta_begin + warp * share, cta_end), end = min(begin + share, cta_end);
+  const int units = cta_end - cta_begin;
+  const int begin = cta_begin + units * warp / W, end = cta_begin + units * (warp + 1) / W;
   auto next_item = [&](Cursor& x) {
     x.at += units_of(x.t.n, ln.align);
     x.k = 0;
@@ -301,34 +297,26 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
     const int head = h / p.row_tiles;
     return (static_cast<long long>(b) * p.c.Hkv + head) * p.rows + (h - head * p.row_tiles) * R;
   };
-  auto load_q = [&](int b, int h, uint32_t(&f)[NB][8][2]) {
-    const int left = p.rows - (h % p.row_tiles) * R;
+  auto load_q = [&](int b, int h, uint32_t(&f)[8][2]) {
+    const bool live = g < p.rows - (h % p.row_tiles) * R;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + (q_row_of(b, h) + g) * (kHeadDim / 2) + t4;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) +
-                            (q_row_of(b, h) + nb * 8 + g) * (kHeadDim / 2) + t4;
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        f[nb][kk][0] = nb * 8 + g < left ? __ldg(src + kk * 8) : 0u;
-        f[nb][kk][1] = nb * 8 + g < left ? __ldg(src + kk * 8 + 4) : 0u;
-      }
+    for (int kk = 0; kk < 8; ++kk) {
+      f[kk][0] = live ? __ldg(src + kk * 8) : 0u;
+      f[kk][1] = live ? __ldg(src + kk * 8 + 4) : 0u;
     }
   };
 
-  // Per-lane state: columns (rows of q) 8 nb + 2 t4 and + 1.
-  uint32_t qf[NB][8][2];
-  float o[NB][8][4];
-  float m[NB][2], l[NB][2];
-  RowKeys rk[NB][2];
+  // Per-lane state: columns (rows of q) 2 t4 and + 1.  The next item's q is fetched while this one is
+  // computed.
+  uint32_t qf[8][2], qn[8][2];
+  float o[8][4], m[2], l[2];
+  RowKeys rk[2];
   int min_limit = 0, max_lo = 0;
   bool fresh = true;
   int seg_k0 = 0;
   int stage = 0;
-  // With registers to spare (NB == 1) the next item's rows are fetched while this one is computed.
-  constexpr bool kAhead = NB == 1;
-  uint32_t qn[kAhead ? NB : 1][8][2];
-  if constexpr (kAhead)
-    if (valid(cx)) load_q(cx.b, cx.h, qn);
+  if (valid(cx)) load_q(cx.b, cx.h, qn);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load_next();
   if (lane == 0) sh.part[warp][0].item = sh.part[warp][1].item = -1;
@@ -338,52 +326,42 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
     if (fresh) {
       fresh = false;
       seg_k0 = cx.k;
-      if constexpr (kAhead) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          qf[0][kk][0] = qn[0][kk][0];
-          qf[0][kk][1] = qn[0][kk][1];
-        }
-        const bool roll = cx.h + 1 == per_seq;
-        if (cx.at + units_of(cx.t.n, ln.align) < end) load_q(cx.b + roll, roll ? 0 : cx.h + 1, qn);
-      } else {
-        load_q(cx.b, cx.h, qf);
+      for (int kk = 0; kk < 8; ++kk) {
+        qf[kk][0] = qn[kk][0];
+        qf[kk][1] = qn[kk][1];
       }
+      const bool roll = cx.h + 1 == per_seq;
+      if (cx.at + units_of(cx.t.n, ln.align) < end) load_q(cx.b + roll, roll ? 0 : cx.h + 1, qn);
       if (p.c.Tq == 1) {
         const RowKeys k = row_keys(cx.t.r, p.rule, 0);
         min_limit = k.limit;
         max_lo = k.lo;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) rk[nb][0] = rk[nb][1] = k;
+        rk[0] = rk[1] = k;
       } else {
         min_limit = 0x7fffffff;
         max_lo = 0;
         const int row0 = (cx.h % p.row_tiles) * R;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int rr = row0 + nb * 8 + 2 * t4 + e;
-            rk[nb][e] = row_keys(cx.t.r, p.rule, rr % p.c.Tq);
-            if (rr >= p.rows) rk[nb][e] = RowKeys{0x7fffffff, 0};
-            min_limit = min(min_limit, rk[nb][e].limit);
-            max_lo = max(max_lo, rk[nb][e].lo);
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int rr = row0 + 2 * t4 + e;
+          rk[e] = row_keys(cx.t.r, p.rule, rr % p.c.Tq);
+          if (rr >= p.rows) rk[e] = RowKeys{0x7fffffff, 0};
+          min_limit = min(min_limit, rk[e].limit);
+          max_lo = max(max_lo, rk[e].lo);
+        }
 #pragma unroll
         for (int d = 1; d < 4; d <<= 1) {
           min_limit = min(min_limit, __shfl_xor_sync(0xffffffffu, min_limit, d));
           max_lo = max(max_lo, __shfl_xor_sync(0xffffffffu, max_lo, d));
         }
       }
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.0f;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        m[nb][0] = m[nb][1] = -INFINITY;
-        l[nb][0] = l[nb][1] = 0.0f;
+      for (int a = 0; a < 8; ++a)
 #pragma unroll
-        for (int a = 0; a < 8; ++a)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nb][a][e] = 0.0f;
-      }
+        for (int e = 0; e < 4; ++e) o[a][e] = 0.0f;
     }
 
     cp_async_wait<kStages - 2>();
@@ -394,72 +372,58 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
     if (key0 < cx.t.len) {
       const uint32_t kb = ring + stage * kStageBytes;
       // S^T: lanes 0-15 address keys 0-15 of the lower 8 columns, lanes 16-31 of the upper.
-      float s[NB][2][4];
+      float s[2][4];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[nb][e >> 2][e & 3] = 0.0f;
+      for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] = 0.0f;
       {
         const int row = lane & 15, up = lane >> 4;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
           uint32_t a[4];
           ldsm4(kb + row * (kHeadDim * 2) + (((2 * kk + up) ^ (row & 7)) << 4), a);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(s[nb][kk & 1], a, qf[nb][kk]);
+          mma16816<BF16>(s[kk & 1], a, qf[kk]);
         }
       }
       // Scores of lane (g, t4): keys key0 + g (e = 0, 1) and + 8 (e = 2, 3); columns 2 t4 + (e & 1).
-      float x[NB][4];
+      float x[4];
       bool over = false;
       const bool masked = key0 + kSlice > min_limit ||
                           (key0 < max_lo && key0 >= p.rule.glob * kTileKeys);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[nb][e] = (s[nb][0][e] + s[nb][1][e]) * p.scale_log2;
-          if (masked) {
-            const int key = key0 + g + (e >> 1) * 8;
-            const RowKeys k = rk[nb][e & 1];
-            if (key >= k.limit || (key < k.lo && key >= p.rule.glob * kTileKeys))
-              x[nb][e] = -INFINITY;
-          }
-          over |= x[nb][e] > m[nb][e & 1] + kRescaleLog2;
+      for (int e = 0; e < 4; ++e) {
+        x[e] = (s[0][e] + s[1][e]) * p.scale_log2;
+        if (masked) {
+          const int key = key0 + g + (e >> 1) * 8;
+          const RowKeys k = rk[e & 1];
+          if (key >= k.limit || (key < k.lo && key >= p.rule.glob * kTileKeys)) x[e] = -INFINITY;
         }
+        over |= x[e] > m[e & 1] + kRescaleLog2;
       }
       if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(x[c], x[c + 2]);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(x[nb][c], x[nb][c + 2]);
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float mn = fmaxf(m[c], mx);
+          const float f = mn == -INFINITY ? 1.0f : ptx::ex2(m[c] - mn);
+          m[c] = mn;
+          l[c] *= f;
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float mn = fmaxf(m[nb][c], mx);
-            const float f = mn == -INFINITY ? 1.0f : ptx::ex2(m[nb][c] - mn);
-            m[nb][c] = mn;
-            l[nb][c] *= f;
-#pragma unroll
-            for (int a = 0; a < 8; ++a) {
-              o[nb][a][c] *= f;
-              o[nb][a][c + 2] *= f;
-            }
+          for (int a = 0; a < 8; ++a) {
+            o[a][c] *= f;
+            o[a][c + 2] *= f;
           }
-      }
-      uint32_t pf[NB][2];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float pr[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float mm = m[nb][e & 1];
-          pr[e] = ptx::ex2(x[nb][e] - (mm == -INFINITY ? 0.0f : mm));
-          l[nb][e & 1] += pr[e];
         }
-        pf[nb][0] = movm_trans(pack16<BF16>(pr[0], pr[1]));
-        pf[nb][1] = movm_trans(pack16<BF16>(pr[2], pr[3]));
       }
+      float pr[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mm = m[e & 1];
+        pr[e] = ptx::ex2(x[e] - (mm == -INFINITY ? 0.0f : mm));
+        l[e & 1] += pr[e];
+      }
+      const uint32_t pf[2] = {movm_trans(pack16<BF16>(pr[0], pr[1])), movm_trans(pack16<BF16>(pr[2], pr[3]))};
       // O^T: 16 columns of d per step; lanes 0-7 / 8-15 address keys 0-7 of the lower / upper
       // eight columns, lanes 16-31 keys 8-15.
       {
@@ -469,8 +433,7 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
         for (int a = 0; a < 8; ++a) {
           uint32_t f[4];
           ldsm4_trans(vb + row * (kHeadDim * 2) + (((2 * a + up) ^ (row & 7)) << 4), f);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(o[nb][a], f, pf[nb]);
+          mma16816<BF16>(o[a], f, pf);
         }
       }
     }
@@ -482,11 +445,9 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
       const bool began = seg_k0 == 0;
       const bool keep = !(done && began);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], d);
+        for (int d = 4; d < 32; d <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
       // A part that goes on behind the share is the warp's last: every copy has landed by now, and it
       // lies in the ring (stage 0); one that began before it has room of its own.
       const int at_end = began ? 1 : 0;
@@ -495,30 +456,25 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
                                          sh.ring[warp][keep ? 0 : stage]);
       if (keep && began) cp_async_wait<0>();
       __syncwarp();
+      float inv[2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float inv[2];
+      for (int c = 0; c < 2; ++c) inv[c] = keep ? 1.0f : l[c] > 0.0f ? 1.0f / l[c] : 0.0f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) inv[c] = keep ? 1.0f : l[nb][c] > 0.0f ? 1.0f / l[nb][c] : 0.0f;
+      for (int a = 0; a < 8; ++a)
 #pragma unroll
-        for (int a = 0; a < 8; ++a)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = nb * 8 + 2 * t4 + (e & 1), d = a * 16 + g + (e >> 1) * 8;
-            rows[r * kHeadDim + piece(r, d >> 2) * 4 + (d & 3)] = o[nb][a][e] * inv[e & 1];
-          }
-      }
+        for (int e = 0; e < 4; ++e) {
+          const int r = 2 * t4 + (e & 1), d = a * 16 + g + (e >> 1) * 8;
+          rows[r * kHeadDim + piece(r, d >> 2) * 4 + (d & 3)] = o[a][e] * inv[e & 1];
+        }
       const int item = cx.b * per_seq + cx.h;
       if (keep) {
-        Part<NB>& pt = sh.part[warp][at_end];
+        Part& pt = sh.part[warp][at_end];
         if (g == 0)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              pt.m[nb * 8 + 2 * t4 + c] = m[nb][c];
-              pt.l[nb * 8 + 2 * t4 + c] = l[nb][c];
-            }
+          for (int c = 0; c < 2; ++c) {
+            pt.m[2 * t4 + c] = m[c];
+            pt.l[2 * t4 + c] = l[c];
+          }
         if (lane == 0) {
           pt.item = item;
           pt.first = cx.at / ln.quota;
@@ -533,16 +489,14 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
         const long long slot = part_slot(1, item, cta, true) * R;
         if (g == 0)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int r = nb * 8 + 2 * t4 + c;
-              const float lg = l[nb][c] > 0.0f ? m[nb][c] + log2f(l[nb][c]) : -INFINITY;
-              if (r < live) {
-                if (p.all_partial) p.part_l[slot + r] = lg;
-                else if (p.lse != nullptr) p.lse[q_row + r] = lg * 0.69314718055994531f;
-              }
+          for (int c = 0; c < 2; ++c) {
+            const int r = 2 * t4 + c;
+            const float lg = l[c] > 0.0f ? m[c] + log2f(l[c]) : -INFINITY;
+            if (r < live) {
+              if (p.all_partial) p.part_l[slot + r] = lg;
+              else if (p.lse != nullptr) p.lse[q_row + r] = lg * 0.69314718055994531f;
             }
+          }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           if (r >= live) continue;
@@ -578,18 +532,17 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
     const int e = __ffs(starts) - 1;
     starts &= starts - 1;
     const uint32_t run = there & ~((1u << e) - 1u) & (starts ? (starts & (0u - starts)) - 1u : 0xffffffffu);
-    const Part<NB>& a = sh.part[e >> 1][e & 1];
+    const Part& a = sh.part[e >> 1][e & 1];
     const int first = a.first, last = a.last, live = a.live;
     const bool split_here = first != last;
     const long long q_row = a.q_row;
     const long long slot = part_slot(p.all_partial, a.item, cta, first == cta) * R;
-    int r = warp;  // a split item's row r is always warp r % W's, which counts its parts below
+    int r = warp;  // a split item's row r is always warp r's, which counts its parts below
     if (!split_here) {
-      r -= turn;
-      if (r < 0) r += W;
-      turn = (turn + live) % W;
+      r = (warp - turn) & (W - 1);
+      turn += live;
     }
-    for (; r < live; r += W) {
+    if (r < live) {
       const bool in = (run >> lane) & 1u;
       const float m_e = in ? sh.part[lane >> 1][lane & 1].m[r] : -INFINITY;
       float mx = m_e;
@@ -625,31 +578,24 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
     }
   }
   if (!p.all_partial && (split[0].last >= 0 || split[1].last >= 0)) {
-    // Asked for once, at the CTA's end: the fence and the counters cost a round trip to L2 each.
-    constexpr int kMine = (R + W - 1) / W;  // rows of a warp
-    int done[2][kMine];
+    // Row r of either item is warp r's.  Asked for once, at the CTA's end: the fence and the counters
+    // cost a round trip to L2 each.
+    static_assert(R == W, "a row for every warp");
+    int done[2] = {-1, -1};
     __threadfence();
     __syncwarp();
 #pragma unroll
     for (int s = 0; s < 2; ++s)
+      if (lane == 0 && split[s].last >= 0 && warp < split[s].live)
+        done[s] = atomicAdd(p.counters + split[s].first * R + warp, 1);
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int r = warp + i * W;
-        done[s][i] = -1;
-        if (lane == 0 && split[s].last >= 0 && r < split[s].live)
-          done[s][i] = atomicAdd(p.counters + split[s].first * kFewRows + r, 1);
-      }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int r = warp + i * W;
-        const int n = __shfl_sync(0xffffffffu, done[s][i], 0);
-        if (n < 0 || n != split[s].last - split[s].first) continue;
-        __threadfence();
-        if (lane == 0) p.counters[split[s].first * kFewRows + r] = 0;
-        join_row(p, split[s].q_row + r, r, R, split[s].first, split[s].last, lane);
-      }
+    for (int s = 0; s < 2; ++s) {
+      const int n = __shfl_sync(0xffffffffu, done[s], 0);
+      if (n < 0 || n != split[s].last - split[s].first) continue;
+      __threadfence();
+      if (lane == 0) p.counters[split[s].first * R + warp] = 0;
+      join_row(p, split[s].q_row + warp, warp, R, split[s].first, split[s].last, lane);
+    }
   }
   // Behind a shared prefix this kernel starts while the prefix's still runs, and must not end before
   // it: the join waits for this kernel only.
@@ -660,16 +606,11 @@ __global__ void __launch_bounds__(kWarpsOf<NB> * 32, 1) few_kernel(const __grid_
 
 int few_setup() {
   using namespace few;
-  const struct {
-    const void* kernel;
-    size_t smem;
-  } all[] = {{reinterpret_cast<const void*>(few_kernel<false, 1>), sizeof(Smem<1>)},
-             {reinterpret_cast<const void*>(few_kernel<true, 1>), sizeof(Smem<1>)},
-             {reinterpret_cast<const void*>(few_kernel<false, 2>), sizeof(Smem<2>)},
-             {reinterpret_cast<const void*>(few_kernel<true, 2>), sizeof(Smem<2>)}};
-  for (const auto& k : all)
-    if (cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(k.smem)) != cudaSuccess)
+  const void* kernels[] = {reinterpret_cast<const void*>(few_kernel<false>),
+                           reinterpret_cast<const void*>(few_kernel<true>)};
+  for (const void* k : kernels)
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(sizeof(Smem))) != cudaSuccess)
       return BSATTN_E_CUDA;
   return BSATTN_OK;
 }
@@ -678,13 +619,10 @@ int few_launch(const FewCall& c, bool overlapped, cudaStream_t stream) {
   using namespace few;
   // The tokens of a page and head lie side by side.
   const int packed = c.c.k_tok == kHeadDim * 2 && c.c.v_tok == kHeadDim * 2;
-  const Params p{c.c,        c.rule,        c.q,   c.o,      c.lse,    c.rows,    c.row_tiles, c.scale_log2,
+  const Params p{c.c,        c.rule,        c.q,    c.o,   c.lse,    c.rows,   c.row_tiles, c.scale_log2,
                  c.out_bf16, c.all_partial, packed, c.cum, c.part_o, c.part_l, c.counters};
-  void (*kernel)(Params) = c.R == 8 ? (c.in_bf16 ? few_kernel<true, 1> : few_kernel<false, 1>)
-                                    : (c.in_bf16 ? few_kernel<true, 2> : few_kernel<false, 2>);
-  const int threads = 32 * (c.R == 8 ? kWarpsOf<1> : kWarpsOf<2>);
-  const size_t smem = c.R == 8 ? sizeof(Smem<1>) : sizeof(Smem<2>);
-  return launch(kernel, dim3(static_cast<unsigned>(c.ctas)), threads, smem, overlapped, stream, p);
+  return launch(c.in_bf16 ? few_kernel<true> : few_kernel<false>, dim3(static_cast<unsigned>(c.ctas)),
+                kThreads, sizeof(Smem), overlapped, stream, p);
 }
 
 }  // namespace paged

@@ -7,7 +7,7 @@
 namespace bsattn {
 namespace paged {
 
-constexpr int kFewRows = 16;   // rows of a tile of rows at most
+constexpr int kFewRows = 8;    // rows of a tile of rows
 constexpr int kSlice = 16;     // keys a warp takes at a time
 constexpr int kMaxSms = 160;   // CTAs of a call at most (a B200 has 148 SMs)
 
@@ -17,13 +17,13 @@ struct FewCall {
   const void* q;
   void* o;
   float* lse;
-  int rows, R, row_tiles;  // rows = G * Tq, in row_tiles tiles of R (8 or 16)
+  int rows, row_tiles;     // rows = G * Tq, in tiles of kFewRows
   float scale_log2;
   int in_bf16, out_bf16;
   int all_partial;         // behind a shared prefix: no piece is a whole result
   int ctas;
   // Scratch: for the join behind a prefix, the sequences' places on the line [B + 1], the line's
-  // quota and alignment; partial outputs and their log2 sums, `slots` of R rows.
+  // quota and alignment; partial outputs and their log2 sums, slots of kFewRows rows.
   int* cum;
   float* part_o;
   float* part_l;

@@ -43,6 +43,9 @@ __all__ = ["paged_kv_append", "paged_attn_fwd", "shared_prefix_attn_fwd", "rope_
 _PACK = _lib.PAGED_CALL.pack
 _STRIDES9 = struct.Struct("@9q").pack
 _HALF = (torch.float16, torch.bfloat16)
+_PAGE_SIZES = frozenset(1 << i for i in range(4, 11))
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def rope_inv_freq(rot_dim: int = HEAD_DIM, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -55,28 +58,30 @@ def _index(t: torch.Tensor, name: str, dev, shape) -> torch.Tensor:
     """``t`` as int32 on ``dev`` with a contiguous last dimension."""
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.dtype != torch.int32 or t.device != dev:
+    if t.dtype is not torch.int32 or t.device != dev:
         t = t.to(device=dev, dtype=torch.int32)
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    if not t.is_contiguous() and t.stride(-1) != 1:
         t = t.contiguous()
     return t
 
 
 def _rows(t: torch.Tensor, name: str, dev, dtype, shape):
-    """A [B, H, T, 128] input as the kernels read it in place (16-byte rows and strides), and its
-    strides."""
+    """A [B, H, T, 128] input as the kernels read it in place (16-byte rows and strides), with its
+    strides and address."""
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if t.dtype != dtype or t.device != dev:
+    if t.dtype is not dtype or t.device != dev:
         raise TypeError(f"{name} must be {dtype} on {dev} like the pages, got {t.dtype} on "
                         f"{t.device}")
-    st = t.stride()
-    if st[3] != 1 or (st[0] | st[1] | st[2]) & 7 or t.data_ptr() & 15:
+    s0, s1, s2, s3 = t.stride()
+    at = t.data_ptr()
+    if s3 != 1 or (s0 | s1 | s2) & 7 or at & 15:
         t = t.contiguous()
         if t.data_ptr() & 15:
             t = t.clone()
-        st = t.stride()
-    return t, st
+        s0, s1, s2, s3 = t.stride()
+        at = t.data_ptr()
+    return t, s0, s1, s2, at
 
 
 def _cache(k_pages, v_pages, block_table, seq_lens, q_lens, B):
@@ -87,15 +92,15 @@ def _cache(k_pages, v_pages, block_table, seq_lens, q_lens, B):
         raise ValueError(f"k_pages and v_pages must be [n_pages, Hkv, page_size, {HEAD_DIM}] of one "
                          f"shape, got {tuple(shape)}, {tuple(v_pages.shape)}")
     dev, dtype = k_pages.device, k_pages.dtype
-    if dtype not in _HALF or v_pages.dtype != dtype:
+    if dtype not in _HALF or v_pages.dtype is not dtype:
         raise TypeError("k_pages and v_pages must both be float16 or both bfloat16, got "
                         f"{dtype}, {v_pages.dtype}")
-    if dev.type != "cuda" or v_pages.device != dev:
+    if not k_pages.is_cuda or v_pages.device != dev:
         raise ValueError("the paged cache needs CUDA tensors on one device (there is no CPU path)")
     n_pages, Hkv, page_size, _ = shape
     if n_pages == 0 or Hkv == 0:
         raise ValueError(f"the cache has no pages or no heads: {tuple(shape)}")
-    if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+    if page_size not in _PAGE_SIZES:
         raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
     k0, k1, k2, k3 = k_pages.stride()
     v0, v1, v2, v3 = v_pages.stride()
@@ -103,14 +108,18 @@ def _cache(k_pages, v_pages, block_table, seq_lens, q_lens, B):
     if k3 != 1 or v3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & 7 or (kp | vp) & 15:
         raise ValueError("k_pages and v_pages must be 16-byte aligned, with a contiguous last "
                          "dimension and strides that are multiples of 8")
-    if block_table.dim() != 2 or block_table.shape[1] == 0:
-        raise ValueError(f"block_table must be [B, max_pages], got {tuple(block_table.shape)}")
-    max_pages = block_table.shape[1]
+    tshape = block_table.shape
+    if len(tshape) != 2 or tshape[1] == 0:
+        raise ValueError(f"block_table must be [B, max_pages], got {tuple(tshape)}")
+    max_pages = tshape[1]
     table = _index(block_table, "block_table", dev, (B, max_pages))
     sl = _index(seq_lens, "seq_lens", dev, (B,))
-    ql = None if q_lens is None else _index(q_lens, "q_lens", dev, (B,))
-    head = (kp, vp, k0, k1, k2, v0, v1, v2, table.data_ptr(), table.stride(0), sl.data_ptr(),
-            0 if ql is None else ql.data_ptr(), max_pages, n_pages, page_size, B)
+    ql, qp = None, 0
+    if q_lens is not None:
+        ql = _index(q_lens, "q_lens", dev, (B,))
+        qp = ql.data_ptr()
+    head = (kp, vp, k0, k1, k2, v0, v1, v2, table.data_ptr(), table.stride(0), sl.data_ptr(), qp,
+            max_pages, n_pages, page_size, B)
     return dev, dtype, Hkv, max_pages, page_size, head, (table, sl, ql)
 
 
@@ -146,18 +155,19 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     B, _, Tq, _ = shape
     dev, dtype, Hkv, _, _, head, keep = _cache(k_pages, v_pages, block_table, seq_lens, q_lens, B)
     rows = (B, Hkv, Tq, HEAD_DIM)
-    k, ks = _rows(k, "k", dev, dtype, rows)
-    v, vs = _rows(v, "v", dev, dtype, rows)
-    Hq, qs, qp, qo = 0, (0, 0, 0), None, None
+    k, k0, k1, k2, kp = _rows(k, "k", dev, dtype, rows)
+    v, v0, v1, v2, vp = _rows(v, "v", dev, dtype, rows)
+    Hq = q0 = q1 = q2 = 0
+    qp = qo = None
     if q is not None:
         Hq = q.shape[1] if q.dim() == 4 else 0
         if Hq == 0:
             raise ValueError(f"q must be [{B}, Hq, {Tq}, {HEAD_DIM}], got {tuple(q.shape)}")
-        q, qs = _rows(q, "q", dev, dtype, (B, Hq, Tq, HEAD_DIM))
-        qp = q.data_ptr()
+        rows = (B, Hq, Tq, HEAD_DIM)
+        q, q0, q1, q2, qp = _rows(q, "q", dev, dtype, rows)
         if q_out is None:
-            q_out = q.new_empty((B, Hq, Tq, HEAD_DIM))
-        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.device != dev \
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif q_out.shape != rows or q_out.dtype is not dtype or q_out.device != dev \
                 or not q_out.is_contiguous() or q_out.data_ptr() & 15:
             raise ValueError("q_out has the wrong shape, dtype, device, layout or alignment")
         qo = q_out.data_ptr()
@@ -165,7 +175,7 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
         raise ValueError("q_out needs q")
     rot, inv = 0, None
     if inv_freq is not None:
-        if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != dev:
+        if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float64 or inv_freq.device != dev:
             raise TypeError("inv_freq must be float64 [rot_dim / 2] on the device of the pages")
         rot = 2 * inv_freq.shape[0]
         if rot % 16 or not 0 < rot <= HEAD_DIM:
@@ -174,26 +184,27 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
         inv = inv_freq.data_ptr()
     if B == 0 or Tq == 0:
         return q_out
-    if torch._C._cuda_getDevice() != dev.index:
-        with torch.cuda.device(dev):
-            return _append(dev, dtype, head, Hq, Hkv, Tq, qp, k, v, qs, ks, vs, qo, inv, rot,
-                           interleaved, q_out)
-    return _append(dev, dtype, head, Hq, Hkv, Tq, qp, k, v, qs, ks, vs, qo, inv, rot, interleaved,
-                   q_out)
+    flags = _lib.IN_BF16 if dtype is torch.bfloat16 else 0
 
+    def launch():
+        stream = _raw_stream(dev.index)
+        ws = _workspace(dev, stream)
+        return _lib.load().bsattn_paged_append(
+            _PACK(*head, Hq, Hkv, Tq, flags, ws.data_ptr(), 4 * ws.numel(), stream), qp, kp, vp,
+            _STRIDES9(q0, q1, q2, k0, k1, k2, v0, v1, v2), qo, inv, rot, 1 if interleaved else 0)
 
-def _append(dev, dtype, head, Hq, Hkv, Tq, qp, k, v, qs, ks, vs, qo, inv, rot, interleaved, q_out):
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    ws = _workspace(dev, stream)
-    call = _PACK(*head, Hq, Hkv, Tq, _lib.IN_BF16 if dtype == torch.bfloat16 else 0, ws.data_ptr(),
-                 4 * ws.numel(), stream)
-    rc = _lib.load().bsattn_paged_append(
-        call, qp, k.data_ptr(), v.data_ptr(),
-        _STRIDES9(qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), qo, inv, rot,
-        1 if interleaved else 0)
+    rc = _on(dev, launch)
     if rc != 0:
         raise BsattnError(rc, "bsattn_paged_append")
     return q_out
+
+
+def _on(dev, launch) -> int:
+    """``launch()`` with ``dev`` current."""
+    if _current_device() == dev.index:
+        return launch()
+    with torch.cuda.device(dev):
+        return launch()
 
 
 def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -251,7 +262,7 @@ def _attn(q, k_pages, v_pages, block_table, seq_lens, q_lens, window, global_blo
     B, Hq, Tq, _ = shape
     dev, dtype, Hkv, max_pages, page_size, head, keep = _cache(k_pages, v_pages, block_table,
                                                                seq_lens, q_lens, B)
-    if q.dtype != dtype or q.device != dev:
+    if q.dtype is not dtype or q.device != dev:
         raise TypeError(f"q must be {dtype} on {dev} like the pages, got {q.dtype} on {q.device}")
     if Hq == 0 or Hq % Hkv:
         raise ValueError(f"Hq must be a multiple of Hkv, got {Hq} and {Hkv}")
@@ -263,61 +274,62 @@ def _attn(q, k_pages, v_pages, block_table, seq_lens, q_lens, window, global_blo
     if q.data_ptr() & 15:
         q = q.clone()
     if out is None:
-        out = torch.empty_like(q, dtype=out_dtype)
-    elif out.shape != shape or out.dtype != out_dtype or out.device != dev \
+        out = torch.empty_like(q) if out_dtype is dtype else torch.empty_like(q, dtype=out_dtype)
+    elif out.shape != shape or out.dtype is not out_dtype or out.device != dev \
             or not out.is_contiguous() or out.data_ptr() & 15:
         raise ValueError("out has the wrong shape, dtype, device, layout or alignment")
-    lse = None
+    lse, lp = None, None
     if return_lse:
         lse = lse_out
         if lse is None:
             lse = q.new_empty((B, Hq, Tq), dtype=torch.float32)
-        elif lse.shape != (B, Hq, Tq) or lse.dtype != torch.float32 or lse.device != dev \
+        elif lse.shape != (B, Hq, Tq) or lse.dtype is not torch.float32 or lse.device != dev \
                 or not lse.is_contiguous():
             raise ValueError("lse_out has the wrong shape, dtype, device or layout")
+        lp = lse.data_ptr()
     if B == 0 or Tq == 0:
         return out, lse
-    flags = (_lib.IN_BF16 if dtype == torch.bfloat16 else 0) | \
-        (_lib.OUT_BF16 if out_dtype == torch.bfloat16 else 0)
-    rule = (window, global_blocks, prefix_len, 0.0 if scale is None else float(scale))
-    if torch._C._cuda_getDevice() != dev.index:
-        with torch.cuda.device(dev):
-            _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags, rule)
-    else:
-        _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags, rule)
+    flags = (_lib.IN_BF16 if dtype is torch.bfloat16 else 0) | \
+        (_lib.OUT_BF16 if out_dtype is torch.bfloat16 else 0)
+
+    def launch():
+        stream = _raw_stream(dev.index)
+        ws = _workspace(dev, stream)
+        need = _scratch_bytes(dev.index, B, Hq, Hkv, Tq, max_pages, page_size, prefix_len)
+        scratch, counters = _room(dev, stream, need)
+        return _lib.load().bsattn_paged_fwd(
+            _PACK(*head, Hq, Hkv, Tq, flags, ws.data_ptr(), 4 * ws.numel(), stream), q.data_ptr(),
+            out.data_ptr(), lp, window, global_blocks, prefix_len,
+            0.0 if scale is None else scale, scratch.data_ptr(), need, counters.data_ptr())
+
+    rc = _on(dev, launch)
+    if rc != 0:
+        raise BsattnError(rc, "bsattn_paged_fwd")
     return out, lse
 
 
-_counter_lock = threading.Lock()
-_counter_sets: dict = {}
+_room_lock = threading.Lock()
+_rooms: dict = {}
+_KEPT = 32 << 20  # bytes of scratch that a stream keeps
 
 
-def _counters(dev, stream) -> torch.Tensor:
-    """The counters of a call: one set per CUDA stream, whose calls follow one another; a captured
-    call gets its own, zeroed by the graph, since graphs of one stream may be replayed at once."""
+def _room(dev, stream, need):
+    """(scratch, counters) of a call.  The calls of one CUDA stream follow one another, so a stream
+    keeps its own; a captured call gets new ones, which belong to the graph (the counters zeroed by
+    it), since graphs captured on one stream may be replayed at the same time."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(_lib.load().bsattn_paged_counters(), dtype=torch.int32, device=dev)
+        return (torch.empty(need, dtype=torch.uint8, device=dev),
+                torch.zeros(_lib.load().bsattn_paged_counters(), dtype=torch.int32, device=dev))
     key = (dev.index, stream)
-    t = _counter_sets.get(key)
-    if t is None:
-        with _counter_lock:
-            t = _counter_sets.get(key)
-            if t is None:
-                t = torch.zeros(_lib.load().bsattn_paged_counters(), dtype=torch.int32, device=dev)
-                _counter_sets[key] = t
-    return t
-
-
-def _launch(dev, head, q, out, lse, B, Hq, Hkv, Tq, max_pages, page_size, flags, rule):
-    index = dev.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    ws = _workspace(dev, stream)
-    need = _scratch_bytes(index, B, Hq, Hkv, Tq, max_pages, page_size, rule[2])
-    # From the caching allocator, for this call only: in a captured graph it belongs to the graph.
-    scratch = q.new_empty(need, dtype=torch.uint8)
-    call = _PACK(*head, Hq, Hkv, Tq, flags, ws.data_ptr(), 4 * ws.numel(), stream)
-    rc = _lib.load().bsattn_paged_fwd(call, q.data_ptr(), out.data_ptr(),
-                                      None if lse is None else lse.data_ptr(), *rule,
-                                      scratch.data_ptr(), need, _counters(dev, stream).data_ptr())
-    if rc != 0:
-        raise BsattnError(rc, "bsattn_paged_fwd")
+    room = _rooms.get(key)
+    if room is None or room[0].numel() < min(need, _KEPT):
+        with _room_lock:
+            room = _rooms.get(key)
+            if room is None or room[0].numel() < min(need, _KEPT):
+                counters = room[1] if room is not None else torch.zeros(
+                    _lib.load().bsattn_paged_counters(), dtype=torch.int32, device=dev)
+                room = _rooms[key] = (torch.empty(min(max(need, 4 << 20), _KEPT),
+                                                  dtype=torch.uint8, device=dev), counters)
+    if need > _KEPT:
+        return torch.empty(need, dtype=torch.uint8, device=dev), room[1]
+    return room
