@@ -312,6 +312,80 @@ def test_bad_pages_and_lengths_are_reported(prefix, B, Tq):
         _expect_page_error()
 
 
+def test_refusals():
+    """What the calls refuse before a launch, with the exception it raises."""
+    c = Cache([40, 33], 2, 16, F16, 84, DEV)
+    kp, vp, table, lens = c.to(DEV)
+    q, k = _q(2, 4, 1, F16, 85).to(DEV), _q(2, 2, 1, F16, 86).to(DEV)
+    inv = ub.rope_inv_freq(128, device=DEV)
+    attn = lambda q=q, kp=kp, vp=vp, table=table, lens=lens, **kw: \
+        ub.paged_attn_fwd(q, kp, vp, table, lens, **kw)  # noqa: E731
+    append = lambda k=k, v=k, kp=kp, table=table, lens=lens, **kw: \
+        ub.paged_kv_append(kp, vp, table, lens, k, v, **kw)  # noqa: E731
+    shared = lambda n: ub.shared_prefix_attn_fwd(q, kp, vp, table, lens, prefix_len=n)  # noqa: E731
+    tall = torch.zeros(2, 2, 8, 128, dtype=F16, device=DEV)
+    odd = torch.zeros(6, 2, 24, 128, dtype=F16, device=DEV)
+    for error, calls in ((ValueError, [
+            lambda: attn(q=q[0]), lambda: attn(q=q[:1]), lambda: attn(q=q[:, :3].contiguous()),
+            lambda: attn(q=q[..., :64].contiguous()), lambda: attn(kp=kp[:, :1], vp=vp),
+            lambda: attn(kp=tall, vp=tall), lambda: attn(kp=odd, vp=odd),
+            lambda: attn(kp=kp[..., ::2], vp=vp[..., ::2]), lambda: attn(kp=kp[:0], vp=vp[:0]),
+            lambda: attn(table=table[0]), lambda: attn(table=table[:1]), lambda: attn(lens=lens[:1]),
+            lambda: attn(q_lens=lens[:1]), lambda: attn(out=q[:1]), lambda: attn(out=q.float()),
+            lambda: attn(lse_out=torch.zeros(2, 4, device=DEV)), lambda: attn(window=0),
+            lambda: attn(global_blocks=1), lambda: attn(window=2, global_blocks=-1),
+            lambda: attn(window=2 ** 40), lambda: shared(24), lambda: shared(-16),
+            lambda: shared(16 * (table.shape[1] + 1)), lambda: shared(2 ** 40),
+            lambda: append(k=k[0]), lambda: append(k=k[:1]), lambda: append(v=q),
+            lambda: append(q=q[:1]), lambda: append(q_out=q), lambda: append(q=q, q_out=k),
+            lambda: append(q=q, q_out=torch.zeros(2, 4, 1, 256, dtype=F16, device=DEV)[..., :128]),
+            lambda: append(q=q, inv_freq=inv[:4]), lambda: append(q=q, inv_freq=inv[:12]),
+            lambda: append(inv_freq=torch.zeros(72, dtype=torch.float64, device=DEV))]),
+            (TypeError, [
+            lambda: attn(q=q.bfloat16()), lambda: attn(q=q.cpu()), lambda: attn(vp=vp.bfloat16()),
+            lambda: attn(kp=kp.float(), vp=vp.float(), q=q.float()),
+            lambda: attn(out_dtype=torch.float32), lambda: attn(out_dtype=16), lambda: attn(q=None),
+            lambda: attn(scale="1"), lambda: append(v=k.bfloat16()), lambda: append(q=q.bfloat16()),
+            lambda: append(k=k.cpu()), lambda: append(inv_freq=inv.float()),
+            lambda: append(inv_freq=inv.cpu()), lambda: append(inv_freq=inv[None])])):
+        for i, call in enumerate(calls):
+            with pytest.raises(error):
+                call()
+                pytest.fail(f"{error.__name__} call {i} was accepted")
+    with pytest.raises(ub.BsattnError) as err:  # windows past the C ABI's bound
+        attn(window=(1 << 24) + 1)
+    assert err.value.code == _lib.E_SHAPE
+    # empty batches and no rows are no error
+    o, lse = attn(q=q[:0], table=table[:0], lens=lens[:0])
+    assert o.shape == (0, 4, 1, 128) and lse.shape == (0, 4, 1)
+    o, lse = attn(q=q[:, :, :0])
+    assert o.shape == (2, 4, 0, 128)
+    assert append(k=k[:, :, :0], v=k[:, :, :0], q=q[:, :, :0]).shape == (2, 4, 0, 128)
+    ub.check_errors(DEV)
+
+
+def test_first_call_on_a_stream_inside_capture_is_refused():
+    """As for the prefill calls: the stream's error word has to exist before a capture."""
+    from usagi_b200 import api
+    c = Cache([40], 2, 16, F16, 87, DEV)
+    args, q = c.to(DEV), _q(1, 4, 1, F16, 88).to(DEV)
+    fresh = torch.cuda.Stream(DEV)
+    fresh.wait_stream(torch.cuda.current_stream(DEV))
+    api._workspaces.pop((DEV.index, fresh.cuda_stream), None)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside graph capture"):
+        with torch.cuda.graph(graph, stream=fresh):
+            ub.paged_attn_fwd(q, *args)
+    del graph
+
+
+def test_gradients_are_not_recorded():
+    c = Cache([40], 2, 16, F16, 89, DEV)
+    args, q = c.to(DEV), _q(1, 4, 1, F16, 90).to(DEV).requires_grad_()
+    o, lse = ub.paged_attn_fwd(q, *args)
+    assert not o.requires_grad and not lse.requires_grad
+
+
 def test_append_reports_bad_pages_and_writes_nothing_there():
     c = Cache([40, 40], 1, 16, F16, 83, DEV)
     kp, vp, table, lens = c.to(DEV)

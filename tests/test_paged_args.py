@@ -8,10 +8,21 @@ import torch
 import usagi_b200 as ub
 from usagi_b200 import _lib
 
+class Call(ctypes.Structure):
+    """bsattn_paged_call of include/bsattn.h."""
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+                ("page_strides", ctypes.c_int64 * 6), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("seq_lens", ctypes.c_void_p),
+                ("q_lens", ctypes.c_void_p)] + [(n, ctypes.c_int32) for n in (
+                    "max_pages", "n_pages", "page_size", "B", "Hq", "Hkv", "Tq", "dtype_flags")] + \
+               [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                ("stream", ctypes.c_void_p)]
+
+
 def _record(a):
-    return _lib.PAGED_CALL.pack(a["kp"], a["vp"], *a["st"], a["table"], a["ts"], a["sl"], a["ql"],
-                                a["mp"], a["np"], a["ps"], a["B"], a["Hq"], a["Hkv"], a["Tq"],
-                                a["flags"], a["ws"], a["wsb"], 0)
+    return ctypes.byref(Call(a["kp"], a["vp"], (ctypes.c_int64 * 6)(*a["st"]), a["table"], a["ts"],
+                             a["sl"], a["ql"], a["mp"], a["np"], a["ps"], a["B"], a["Hq"], a["Hkv"],
+                             a["Tq"], a["flags"], a["ws"], a["wsb"], None))
 
 
 CACHE = dict(kp=16, vp=16, st=[128] * 6, table=16, ts=4, mp=4, np=8, ps=16, sl=16, ql=0, B=1, Hq=2,
@@ -28,7 +39,7 @@ def _fwd(**kw):
 def _append(**kw):
     a = dict(CACHE, q=16, k=16, v=16, ins=[128] * 9, qo=16, inv=16, rot=128)
     a.update(kw)
-    ins = None if a["ins"] is None else bytes((ctypes.c_int64 * 9)(*a["ins"]))
+    ins = None if a["ins"] is None else (ctypes.c_int64 * 9)(*a["ins"])
     return _lib.load().bsattn_paged_append(_record(a), a["q"], a["k"], a["v"], ins, a["qo"],
                                            a["inv"], a["rot"], 0)
 
@@ -73,7 +84,7 @@ def test_append_arguments():
 def test_null_call_record():
     lib = _lib.load()
     assert lib.bsattn_paged_fwd(None, 16, 16, None, 0, 0, 0, 0.0, 16, 1 << 20, 16) == _lib.E_NULL
-    assert lib.bsattn_paged_append(None, 16, 16, 16, bytes(72), 16, None, 0, 0) == _lib.E_NULL
+    assert lib.bsattn_paged_append(None, 16, 16, 16, (ctypes.c_int64 * 9)(), 16, None, 0, 0) == _lib.E_NULL
 
 
 def test_error_code_has_a_text():
@@ -101,10 +112,11 @@ def test_python_side():
         ub.paged_attn_fwd(q, kp, kp, table, lens, window=0)
     with pytest.raises(ValueError, match="window"):
         ub.paged_attn_fwd(q, kp, kp, table, lens, global_blocks=1)
-    with pytest.raises(ValueError, match="whole pages"):
-        ub.shared_prefix_attn_fwd(q, kp, kp, table, lens, prefix_len=24)
-    with pytest.raises(ValueError, match="holds"):
-        ub.shared_prefix_attn_fwd(q, kp, kp, table, lens, prefix_len=80)
+    for bad in (None, 3, kp.numpy()):
+        with pytest.raises(TypeError, match="tensor"):
+            ub.paged_attn_fwd(bad, kp, kp, table, lens)
+        with pytest.raises(TypeError, match="tensor"):
+            ub.paged_attn_fwd(q, kp, bad, table, lens)
 
 
 def test_inv_freq():

@@ -5,7 +5,6 @@ There is no fallback: if the library is missing or does not export the ABI, load
 from __future__ import annotations
 
 import ctypes
-import struct
 import threading
 from pathlib import Path
 
@@ -65,14 +64,14 @@ SIGNATURES = {
     "bsattn_ipc_close": (_c_int, [_c_void_p, ctypes.c_uint64]),
     "bsattn_peer_copy": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),
     "bsattn_paged_append": (_c_int, [
-        ctypes.c_char_p,                          # PAGED_CALL
+        _c_void_p,                                # bsattn_paged_call (host)
         _c_void_p, _c_void_p, _c_void_p,          # q, k, v
-        ctypes.c_char_p, _c_void_p,               # in_strides (host int64[9]), q_out
+        _c_void_p, _c_void_p,                     # in_strides (host int64[9]), q_out
         _c_void_p, _c_int, _c_int,                # inv_freq, rot_dim, interleaved
     ]),
     "bsattn_paged_scratch_bytes": (_c_int, [_c_int] * 7 + [ctypes.POINTER(_c_size_t)]),
     "bsattn_paged_fwd": (_c_int, [
-        ctypes.c_char_p,                          # PAGED_CALL
+        _c_void_p,                                # bsattn_paged_call (host)
         _c_void_p, _c_void_p, _c_void_p,          # q, o, lse
         _c_int, _c_int, _c_int, ctypes.c_float,   # window, global_blocks, prefix_len, scale
         _c_void_p, _c_size_t, _c_void_p,          # scratch, bytes, counters
@@ -88,10 +87,6 @@ SIGNATURES = {
         _c_void_p, _c_void_p,                     # status (device or pinned host int*), stream
     ]),
 }
-
-# bsattn_paged_call: k_pages, v_pages, page_strides[6], block_table, table_stride, seq_lens, q_lens,
-# max_pages, n_pages, page_size, B, Hq, Hkv, Tq, dtype_flags, workspace, workspace_bytes, stream
-PAGED_CALL = struct.Struct("@PP6qPqPP8iPNP")
 
 # error codes (include/bsattn.h)
 OK = 0

@@ -28,6 +28,14 @@ SOURCES = ["bsattn_fwd.cu", "csr_build.cu", "peer.cu", "paged_append.cu", "paged
            "paged_few.cu", "paged_tile.cu"]
 HEADERS = ["sm100_ptx.cuh", "paged_common.cuh", "paged_few.cuh", "paged_tile.cuh"]
 
+# The Python side of the paged-cache calls: a CPython module of its own, compiled against torch, which
+# reaches the kernel library through the addresses that _lib gives it.
+BINDING_NAME = "_paged_binding.so"
+BINDING_PATH = PKG_DIR / BINDING_NAME
+BINDING_STAMP_PATH = PKG_DIR / (BINDING_NAME + ".sha256")
+BINDING_SOURCE = CSRC / "paged_binding.cpp"
+BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo",
@@ -71,8 +79,58 @@ def needs_build() -> bool:
     return STAMP_PATH.read_text().strip() != source_hash()
 
 
+def binding_hash() -> str:
+    """sha256 over what the binding is built from: flags, sources, torch's and Python's versions."""
+    import torch
+    h = hashlib.sha256()
+    h.update(" ".join([*BINDING_FLAGS, torch.__version__, sys.version]).encode())
+    for f in (BINDING_SOURCE, INCLUDE / "bsattn.h"):
+        h.update(f.read_bytes())
+    return h.hexdigest()
+
+
+def binding_needs_build() -> bool:
+    """As :func:`needs_build`, for the binding."""
+    if not BINDING_PATH.exists() or not BINDING_STAMP_PATH.exists():
+        return True
+    return BINDING_STAMP_PATH.read_text().strip() != binding_hash()
+
+
+def _run(cmd, verbose: bool) -> str:
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    return res.stderr
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile ``csrc/paged_binding.cpp`` into ``usagi_b200/_paged_binding.so``; returns its path."""
+    if not force and not binding_needs_build():
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).parent
+    nvcc = Path(_nvcc()).resolve()
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    _run([os.environ.get("CXX") or "g++", *BINDING_FLAGS,
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-isystem", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+          "-isystem", str(nvcc.parent.parent / "include"), str(BINDING_SOURCE), "-o", str(tmp),
+          "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"],
+         verbose)
+    digest = binding_hash()
+    os.replace(tmp, BINDING_PATH)
+    BINDING_STAMP_PATH.write_text(digest + "\n")
+    return BINDING_PATH
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compile ``csrc/*.cu`` into ``usagi_b200/libbsattn.so``; returns the library path."""
+    """Compile ``csrc/*.cu`` into ``usagi_b200/libbsattn.so`` and the binding next to it; returns the
+    library path."""
+    build_binding(force, verbose)
     if not force and not needs_build():
         return LIB_PATH
     cmd = [_nvcc(), *NVCC_FLAGS]
@@ -80,13 +138,9 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         cmd += ["-Xptxas", "-v"]
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd += ["-o", str(tmp)] + [str(CSRC / s) for s in SOURCES]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    stderr = _run(cmd, verbose)
     if verbose or ptxas_info:
-        sys.stdout.write(res.stderr)
+        sys.stdout.write(stderr)
     digest = source_hash()
     os.replace(tmp, LIB_PATH)
     STAMP_PATH.write_text(digest + "\n")
