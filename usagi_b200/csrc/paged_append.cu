@@ -72,6 +72,8 @@ template <bool BF16>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ float2 cs[kTok][kHeadDim / 2];
   __shared__ int s_pos[kTok], s_page[kTok], s_b[kTok], s_t[kTok];
+  pdl_wait();
+  pdl_trigger();
   const long long tok0 = static_cast<long long>(blockIdx.x) * kTok;
   const long long tokens = static_cast<long long>(p.c.B) * p.c.Tq;
   const int half = p.rot / 2;
@@ -211,10 +213,6 @@ extern "C" int bsattn_paged_append(const bsattn_paged_call* call, const void* q,
   p.heads_per_block = static_cast<int>((heads + split - 1) / split);
   const dim3 grid(static_cast<unsigned>(bx),
                   static_cast<unsigned>((heads + p.heads_per_block - 1) / p.heads_per_block));
-  cudaStream_t s = static_cast<cudaStream_t>(call->stream);
-  if (call->dtype_flags & BSATTN_IN_BF16)
-    append_kernel<true><<<grid, kAppendThreads, 0, s>>>(p);
-  else
-    append_kernel<false><<<grid, kAppendThreads, 0, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? BSATTN_OK : BSATTN_E_CUDA;
+  return launch((call->dtype_flags & BSATTN_IN_BF16) ? append_kernel<true> : append_kernel<false>, grid,
+                kAppendThreads, 0, static_cast<cudaStream_t>(call->stream), p);
 }

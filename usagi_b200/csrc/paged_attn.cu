@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid
   const int first_p = static_cast<int>(sp / p.quota_p);
   const int pre = static_cast<int>((sp + p.tiles_p - 1) / p.quota_p) - first_p + 1;
   pdl_wait();
+  pdl_trigger();
   const int c0 = p.cum[b], n = p.cum[b + 1] - c0;
   const Line ln{p.cum[p.B + 1], p.cum[p.B + 2]};
   const int s = c0 * heads + hr * n;
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_cuts_kernel(const __grid
   const int r = (blockIdx.y * kJoinWarps + warp) * 4 + (lane & 3), piece = lane >> 2;
   const int first = blockIdx.x;
   pdl_wait();
+  pdl_trigger();
   const TileCut cut = p.cuts[first];
   if (cut.v < 0) return;
   const int b = cut.v / p.rt.per_seq;
@@ -424,7 +426,7 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     f.part_o = reinterpret_cast<float*>(base + s.part_o);
     f.part_l = reinterpret_cast<float*>(base + s.part_l);
     f.counters = counters;
-    if ((rc = few_launch(f, s.prefix, stream)) != BSATTN_OK) return rc;
+    if ((rc = few_launch(f, stream)) != BSATTN_OK) return rc;
   }
   if (s.prefix) {
     RowJoin j;
@@ -449,9 +451,9 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     // Rows of many parts are shared by four warps.
     const unsigned quads = static_cast<unsigned>(j.groups) * static_cast<unsigned>((s.rows + 3) / 4);
     return s.pieces_p / items_p >= 8
-               ? launch(join_rows_kernel<kJoinWarps>, dim3(quads), kJoinWarps * 32, 0, true, stream, j)
+               ? launch(join_rows_kernel<kJoinWarps>, dim3(quads), kJoinWarps * 32, 0, stream, j)
                : launch(join_rows_kernel<1>, dim3((quads + kJoinWarps - 1) / kJoinWarps),
-                        kJoinWarps * 32, 0, true, stream, j);
+                        kJoinWarps * 32, 0, stream, j);
   } else if (!s.few) {
     CutJoin j;
     j.cuts = reinterpret_cast<const TileCut*>(base + s.cuts);
@@ -465,7 +467,7 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     j.part_l = reinterpret_cast<const float*>(base + s.part_l);
     const unsigned groups = static_cast<unsigned>((s.rt.n_t * s.rt.G + 15) / 16);
     return launch(join_cuts_kernel, dim3(static_cast<unsigned>(s.pieces), groups), kJoinWarps * 32, 0,
-                  true, stream, j);
+                  stream, j);
   }
   return BSATTN_OK;
 }

@@ -151,8 +151,10 @@ __device__ __forceinline__ float2 unpack16(uint32_t v) {
   if constexpr (BF16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
   return __half22float2(*reinterpret_cast<__half2*>(&v));
 }
-// Programmatic launch: the next kernel of the stream may start its own setup; it waits for this
-// one's results with pdl_wait.
+// Programmatic launch.  Every kernel here is launched so that it may begin while its predecessor on the
+// stream still runs, and waits for that one's end and results (pdl_wait) before it touches memory: what
+// is saved is the launch, a microsecond or two of a call that takes ten.  It lets its own successor
+// begin (pdl_trigger) only after that wait, so whoever comes next finds everything before it complete.
 __device__ __forceinline__ void pdl_trigger() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
@@ -164,11 +166,9 @@ __device__ __forceinline__ void pdl_wait() {
 // Number of SMs of the current device (checked to be sm_100).
 int device_sms(int* sms);
 
-// Launches a kernel of one parameter record; overlapped: it may start while its predecessor on the
-// stream still runs, and waits for its results with pdl_wait.
+// Launches a kernel of one parameter record, to begin while its predecessor still runs.
 template <class P>
-inline int launch(void (*kernel)(P), dim3 grid, int threads, size_t smem, bool overlapped,
-                  cudaStream_t stream, const P& p) {
+inline int launch(void (*kernel)(P), dim3 grid, int threads, size_t smem, cudaStream_t stream, const P& p) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -178,7 +178,7 @@ inline int launch(void (*kernel)(P), dim3 grid, int threads, size_t smem, bool o
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = overlapped ? 1 : 0;
+  cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess) return BSATTN_OK;
   cudaGetLastError();
   return BSATTN_E_CUDA;

@@ -156,6 +156,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int per_seq = p.c.Hkv * p.row_tiles;
+  // Behind a shared prefix this kernel runs beside the prefix's, whose inputs are its own: it waits for
+  // that one at its end, so that the join may wait for this one only.
+  if (!p.all_partial) pdl_wait();
   pdl_trigger();
 
   // The line: every thread adds up some sequences, in plain units and (upper half) aligned ones.
@@ -215,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   }
   __syncthreads();
   if (cta_begin >= cta_end) {
-    pdl_wait();
+    if (p.all_partial) pdl_wait();
     return;
   }
 
@@ -554,12 +557,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       PartSum s;
       s.clear();
-      for (uint32_t left = run; left != 0; left &= left - 1) {
-        const int x = __ffs(left) - 1;
-        const float* rows = (x & 1) ? reinterpret_cast<const float*>(sh.ring[x >> 1][0])
-                                    : &sh.rest_o[x >> 1][0][0];
-        s.add(reinterpret_cast<const float4*>(rows)[r * (kHeadDim / 4) + piece(r, lane)],
-              __shfl_sync(0xffffffffu, f, x));
+#pragma unroll
+      for (int w = 0; w < W; ++w) {  // a warp has at most one part of an item
+        const uint32_t which = (run >> (2 * w)) & 3u;
+        const float fx = __shfl_sync(0xffffffffu, f, 2 * w + (which >> 1));
+        if (which == 0) continue;
+        const float* rows = which > 1 ? reinterpret_cast<const float*>(sh.ring[w][0]) : &sh.rest_o[w][0][0];
+        s.add(reinterpret_cast<const float4*>(rows)[r * (kHeadDim / 4) + piece(r, lane)], fx);
       }
       s.sum = sum;
       const float4 v = s.normal();
@@ -597,9 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       join_row(p, split[s].q_row + warp, warp, R, split[s].first, split[s].last, lane);
     }
   }
-  // Behind a shared prefix this kernel starts while the prefix's still runs, and must not end before
-  // it: the join waits for this kernel only.
-  pdl_wait();
+  if (p.all_partial) pdl_wait();
 }
 
 }  // namespace few
@@ -615,14 +617,14 @@ int few_setup() {
   return BSATTN_OK;
 }
 
-int few_launch(const FewCall& c, bool overlapped, cudaStream_t stream) {
+int few_launch(const FewCall& c, cudaStream_t stream) {
   using namespace few;
   // The tokens of a page and head lie side by side.
   const int packed = c.c.k_tok == kHeadDim * 2 && c.c.v_tok == kHeadDim * 2;
   const Params p{c.c,        c.rule,        c.q,    c.o,   c.lse,    c.rows,   c.row_tiles, c.scale_log2,
                  c.out_bf16, c.all_partial, packed, c.cum, c.part_o, c.part_l, c.counters};
   return launch(c.in_bf16 ? few_kernel<true> : few_kernel<false>, dim3(static_cast<unsigned>(c.ctas)),
-                kThreads, sizeof(Smem), overlapped, stream, p);
+                kThreads, sizeof(Smem), stream, p);
 }
 
 }  // namespace paged

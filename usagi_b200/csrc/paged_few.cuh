@@ -31,7 +31,7 @@ struct FewCall {
 };
 
 int few_setup();
-int few_launch(const FewCall& call, bool overlapped, cudaStream_t stream);
+int few_launch(const FewCall& call, cudaStream_t stream);
 
 // The line.  An item is (sequence, K/V head, tile of rows): its slices of 16 keys, one unit each, and
 // kItemUnits for what its end costs.  The line of all items is cut into pieces of `quota` units, one

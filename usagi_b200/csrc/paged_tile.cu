@@ -725,20 +725,20 @@ __device__ void epilogue_role(Smem& sh, const Params& p, uint32_t tmem) {
   }
 }
 
+struct Launch {
+  CUtensorMap q, k, v;
+  Params p;
+};
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
-    tile_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
+    tile_kernel(const __grid_constant__ Launch l) {
+  const CUtensorMap &tq = l.q, &tk = l.k, &tv = l.v;
+  const Params& p = l.p;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   Smem& sh = *reinterpret_cast<Smem*>(smem_raw + (((raw + 1023u) & ~1023u) - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
-
-  if (warp == 1) {
-    ptx::tmem_alloc(ptx::smem_u32(&sh.tmem_base), kTmemCols);
-    ptx::tmem_relinquish();
-  }
   if (warp == 2) {
     // Side by side on the lanes of a warp: one thread would take a microsecond.
     auto init = [&](uint64_t& bar, uint32_t n) { ptx::mbar_init(ptx::smem_u32(&bar), n); };
@@ -776,6 +776,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::tma_prefetch_desc(&tv);
   }
 
+  pdl_wait();
+  pdl_trigger();
+  // Tensor memory only now: a predecessor that still has to allocate its own on this SM must not find
+  // it taken by a kernel that waits for it.
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(&sh.tmem_base), kTmemCols);
+    ptx::tmem_relinquish();
+  }
   // This CTA's piece of the line (as in the few-row kernel).
   const int chunk = (p.rt.count + kThreads - 1) / kThreads;
   const int v0 = min(static_cast<int>(threadIdx.x) * chunk, p.rt.count);
@@ -959,12 +967,9 @@ int tile_launch(const TileCall& call, int page_size, cudaStream_t stream) {
   p.part_l = call.part_l;
   p.timeout_ns = launch_timeout_ns();
   p.test_wait = launch_test_wait();
-  const unsigned grid = static_cast<unsigned>(call.pieces);
-  if (call.in_bf16)
-    tile_kernel<true><<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, p);
-  else
-    tile_kernel<false><<<grid, kThreads, kSmemBytes, stream>>>(tq, tk, tv, p);
-  return cudaGetLastError() == cudaSuccess ? BSATTN_OK : BSATTN_E_CUDA;
+  const Launch l{tq, tk, tv, p};
+  return launch(call.in_bf16 ? tile_kernel<true> : tile_kernel<false>,
+                dim3(static_cast<unsigned>(call.pieces)), kThreads, kSmemBytes, stream, l);
 }
 
 }  // namespace paged
