@@ -38,7 +38,12 @@ constexpr int kStages = 3;
 constexpr int kSliceBytes = kSlice * kHeadDim * 2;  // 4 KB of K or of V
 constexpr int kStageBytes = 2 * kSliceBytes;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kAlign = 32;  // units of a CTA in a small call
+// When to give every item CTAs of its own (Line::align).  A part of at least kPartUnits units, since
+// joining parts takes 3 us and a CTA 16 units in 1.5; up to kWholeUnits an item is not cut at all (512
+// keys: 9.4 us, cut in two 11.2); and rather than cutting the line in equal pieces as long as a part is
+// no more than kCutUnits units longer than such a piece, of which most CTAs hold two (16 heads, 8,192
+// keys: 20.2 us in parts of 64 units, 23.8 in pieces of 56).
+constexpr int kPartUnits = 16, kWholeUnits = 32, kCutUnits = 16;
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 
 struct Params {
@@ -106,7 +111,7 @@ struct Smem {
   uint8_t ring[kWarps][kStages][kStageBytes];
   float rest_o[kWarps][kFewRows][kHeadDim];    // of the item that began before the warp's share
   Part part[kWarps][2];                        // that one, and the one that goes on behind the share
-  unsigned long long warp_sum[kWarps];
+  int warp_sum[2][kWarps], longest[kWarps];
   Cursor found;
 };
 
@@ -156,50 +161,70 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int per_seq = p.c.Hkv * p.row_tiles;
-  // Behind a shared prefix this kernel runs beside the prefix's, whose inputs are its own: it waits for
-  // that one at its end, so that the join may wait for this one only.
+  // Behind a shared prefix this kernel runs beside the prefix's (paged_attn.cu says how).
   if (!p.all_partial) pdl_wait();
   pdl_trigger();
 
-  // The line: every thread adds up some sequences, in plain units and (upper half) aligned ones.
-  const int chunk = (p.c.B + kThreads - 1) / kThreads;
-  const int b0 = min(static_cast<int>(threadIdx.x) * chunk, p.c.B);
+  // The line.  Up to 32 sequences every warp lays out by itself, one per lane, with no barrier; more of
+  // them the block's threads, some each.
+  const bool alone = p.c.B <= 32;
+  const int chunk = alone ? 1 : (p.c.B + kThreads - 1) / kThreads;
+  const int b0 = min((alone ? lane : static_cast<int>(threadIdx.x)) * chunk, p.c.B);
   const int b1 = min(b0 + chunk, p.c.B);
-  unsigned long long mine = 0;
-  Slices t0;  // of sequence b0; the only one in most calls
+  int mine = 0, longest = 0;
+  Slices t0 = {};  // of sequence b0; the only one in most calls
   for (int b = b0; b < b1; ++b) {
     const Slices t = slices_of(p, b);
     if (b == b0) t0 = t;
-    const int n = t.n;
-    mine += static_cast<unsigned>(units_of(n, 0)) +
-            (static_cast<unsigned long long>(units_of(n, kAlign)) << 32);
+    mine += units_of(t.n, 0);
+    longest = max(longest, t.n);
   }
-  unsigned long long incl = mine;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  // What lies before this thread's sequences, and in all.
+  auto sums = [&](int x, int* shared, int& before, int& total) {
+    int incl = x;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const unsigned long long up = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += up;
-  }
-  if (lane == 31) sh.warp_sum[warp] = incl;
-  __syncthreads();
-  unsigned long long total2 = 0, before2 = incl - mine;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    if (w < warp) before2 += sh.warp_sum[w];
-    total2 += sh.warp_sum[w];
-  }
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    before = incl - x;
+    total = __shfl_sync(0xffffffffu, incl, 31);
+    if (alone) return;
+    if (lane == 0) {
+      shared[warp] = total;
+      sh.longest[warp] = longest;
+    }
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < W; ++w) {
+      if (w < warp) before += shared[w];
+      total += shared[w];
+      longest = max(longest, sh.longest[w]);
+    }
+  };
+  int before, total;
+  sums(mine, sh.warp_sum[0], before, total);
   const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
-  Line ln;
-  ln.align = static_cast<long long>(total2 >> 32) * per_seq <= static_cast<long long>(ctas) * kAlign
-                 ? kAlign : 0;
-  const int total = static_cast<int>(ln.align ? total2 >> 32 : total2 & 0xffffffffu);
-  int before = static_cast<int>(ln.align ? before2 >> 32 : before2 & 0xffffffffu);
+  const int line_plain = total * per_seq, quota_plain = (line_plain + ctas - 1) / ctas;
+  Line ln{quota_plain, 0};
+  const int spare = max(ctas - p.c.B * per_seq, 1);  // CTAs behind one for every item
+  if (ctas >= p.c.B * per_seq) {
+    // Two part lengths that fit: each item in as many parts as there are CTAs for every item, or as many
+    // as its length gives beside one CTA of its own.
+    const int each = ctas / (p.c.B * per_seq);
+    const int fit = min((longest + each - 1) / each, (line_plain + spare - 1) / spare);
+    const int align = longest <= kWholeUnits ? kWholeUnits : max(fit, kPartUnits);
+    if (align <= max(quota_plain, kPartUnits) + kCutUnits) ln = Line{align, align};
+  }
+  if (ln.align > 0) sums(b0 < b1 ? units_of(t0.n, ln.align) : 0, sh.warp_sum[1], before, total);
   const int line = total * per_seq;
-  ln.quota = ln.align ? kAlign : (line + ctas - 1) / ctas;
   const int cta_begin =
       static_cast<int>(min(static_cast<long long>(cta) * ln.quota, static_cast<long long>(line)));
   const int cta_end = min(cta_begin + ln.quota, line);
   // The item that holds the CTA's first unit.
+  Cursor ld = {};
+  bool here = false;
   for (int b = b0; b < b1; ++b) {
     if (b > b0) t0 = slices_of(p, b);
     const int n = units_of(t0.n, ln.align);
@@ -207,7 +232,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     const int rel = cta_begin - before * per_seq;
     if (rel >= 0 && rel < n * per_seq) {
       const int h = rel / n;
-      sh.found = Cursor{b, h, 0, before * per_seq + h * n, t0};
+      ld = Cursor{b, h, 0, before * per_seq + h * n, t0};
+      here = true;
     }
     before += n;
   }
@@ -216,14 +242,25 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     p.cum[p.c.B + 1] = ln.quota;
     p.cum[p.c.B + 2] = ln.align;
   }
-  __syncthreads();
+  if (alone) {
+    const uint32_t at = __ballot_sync(0xffffffffu, here);
+    int* const words = reinterpret_cast<int*>(&ld);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(Cursor) / sizeof(int)); ++i)
+      words[i] = __shfl_sync(0xffffffffu, words[i], at ? __ffs(at) - 1 : 0);
+  } else {
+    if (here) sh.found = ld;
+    __syncthreads();
+    ld = sh.found;
+  }
   if (cta_begin >= cta_end) {
-    if (p.all_partial) pdl_wait();
+    if (p.all_partial && blockIdx.x == 0) pdl_wait();
     return;
   }
 
   // This warp's share, and its first slice.
-  const int units = cta_end - cta_begin;
+  const int stop = ln.align > 0 ? min(cta_end, ld.at + ld.t.n) : cta_end;
+  const int units = stop - cta_begin;
   const int begin = cta_begin + units * warp / W, end = cta_begin + units * (warp + 1) / W;
   auto next_item = [&](Cursor& x) {
     x.at += units_of(x.t.n, ln.align);
@@ -232,7 +269,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     x.h = 0;
     if (++x.b < p.c.B) x.t = slices_of(p, x.b);
   };
-  Cursor ld = sh.found;
   while (ld.at < end && ld.at + ld.t.n <= begin) next_item(ld);
   ld.k = max(begin - ld.at, 0);
   auto valid = [&](const Cursor& x) { return x.at + x.k < end; };
@@ -601,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       join_row(p, split[s].q_row + warp, warp, R, split[s].first, split[s].last, lane);
     }
   }
-  if (p.all_partial) pdl_wait();
+  if (p.all_partial && blockIdx.x == 0) pdl_wait();
 }
 
 }  // namespace few

@@ -36,8 +36,8 @@ int few_launch(const FewCall& call, cudaStream_t stream);
 // The line.  An item is (sequence, K/V head, tile of rows): its slices of 16 keys, one unit each, and
 // kItemUnits for what its end costs.  The line of all items is cut into pieces of `quota` units, one
 // per CTA, and those into equal shares for its warps; a warp takes the slices that begin in its share.
-// When the call is so small that every item can begin a CTA of its own (align > 0: items are rounded
-// up to whole pieces of that many units), few items are cut at all and none shares a CTA.
+// When there are CTAs enough for every item to have its own, that may be better than equal pieces
+// (align > 0: items are rounded up to whole pieces of that many units, and no CTA holds two).
 constexpr int kItemUnits = 1;
 struct Line {
   int quota, align;

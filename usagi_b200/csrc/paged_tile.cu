@@ -776,6 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::tma_prefetch_desc(&tv);
   }
 
+  const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
   pdl_wait();
   pdl_trigger();
   // Tensor memory only now: a predecessor that still has to allocate its own on this SM must not find
@@ -809,8 +810,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     total += sh.warp_sum[w];
   }
   const int line = total * p.c.Hkv;
-  const int quota = (line + gridDim.x - 1) / gridDim.x;
-  const int begin = min(static_cast<int>(blockIdx.x) * quota, line);
+  const int quota = (line + ctas - 1) / ctas;
+  const int begin = min(cta * quota, line);
   const int end = min(begin + quota, line);
   for (int v = v0; v < v1; ++v) {
     if (v > v0) vt = vtiles(p, v);
@@ -824,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     before += n;
   }
-  if (threadIdx.x == 0 && p.prefix_len == 0) p.cuts[blockIdx.x] = TileCut{-1, 0, 0, 0};
+  if (threadIdx.x == 0 && p.prefix_len == 0) p.cuts[cta] = TileCut{-1, 0, 0, 0};
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
