@@ -16,8 +16,8 @@
 namespace bsattn {
 namespace paged {
 
-// Joins behind a shared prefix: every row of the call, over the parts of its own keys in the order of
-// the line, then over those of the prefix: o = sum_i o_i 2^(l_i - l), l = log2 sum 2^l_i.
+// Joins behind a shared prefix: every row of the call, over the parts of the prefix in the order of its
+// line, then over those of its own keys: o = sum_i o_i 2^(l_i - l), l = log2 sum 2^l_i.
 struct RowJoin {
   int Hkv, rows, groups; // rows = G * Tq; groups = B * Hkv
   void* o;
@@ -43,16 +43,9 @@ struct Quad {
     sum = 0.0f;
     mx = -INFINITY;
   }
-  // Parts in their order; `at` is the lane's first 16-byte piece, `step` the distance of the next.
-  // Up to four at once, so that their loads overlap.
+  // Parts in their order: their pieces and log2 sums.
   template <int N>
-  __device__ __forceinline__ void add(const float4* const (&at)[N], const float (&lg)[N], int step) {
-    float4 y[N][4];
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        y[c][i] = lg[c] > -INFINITY ? __ldcg(at[c] + i * step) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __device__ __forceinline__ void add(const float4 (&y)[N][4], const float (&lg)[N]) {
     float top = mx;
 #pragma unroll
     for (int c = 0; c < N; ++c) top = fmaxf(top, lg[c]);
@@ -78,19 +71,26 @@ struct Quad {
     for (int i = 0; i < 4; ++i)
       acc[i] = make_float4(acc[i].x * f, acc[i].y * f, acc[i].z * f, acc[i].w * f);
   }
-  // Every W-th part from `from` on, of `n`: part c's log2 sum at l[c * l_step], its rows c * o_step on.
+  // Every W-th part from `from` on, of `n`: part c's log2 sum at l[c * l_step], the lane's first piece
+  // of it at o[c * o_step], the others `step` apart.  Four at once, so that their loads overlap.
   __device__ __forceinline__ void add_all(const float* l, long long l_step, const float4* o,
                                           long long o_step, int step, int from, int n, int W) {
     for (int c0 = from; c0 < n; c0 += 4 * W) {
-      const float4* at[4];
+      float4 y[4][4];
       float lg[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const long long x = c0 + c * W;
-        lg[c] = x < n ? __ldcg(l + x * l_step) : -INFINITY;
-        at[c] = o + x * o_step;
+        lg[c] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[c][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (x < n) {
+          lg[c] = __ldcg(l + x * l_step);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[c][i] = __ldcg(o + x * o_step + i * step);
+        }
       }
-      add(at, lg, step);
+      add(y, lg);
     }
   }
   __device__ __forceinline__ void store(void* o, float* lse, int out_bf16, long long row, int piece) const {
@@ -127,23 +127,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_rows_kernel(const __grid
   const int pre = static_cast<int>((sp + p.tiles_p - 1) / p.quota_p) - first_p + 1;
   pdl_wait();
   pdl_trigger();
+  // The prefix's parts first: where the own ones lie has to be read.
   const int c0 = p.cum[b], n = p.cum[b + 1] - c0;
   const Line ln{p.cum[p.B + 1], p.cum[p.B + 2]};
-  const int s = c0 * heads + hr * n;
-  const int first = s / ln.quota, own = last_cta(ln, s, n) - first + 1;
-  const long long item = static_cast<long long>(b) * heads + hr;
   const bool live = rr < p.rows;
+  const int from = W == 1 ? 0 : warp;
   Quad x;
   x.clear();
   if (live) {
-    const int from = W == 1 ? 0 : warp;
-    const long long at = (item + first) * p.R + r;
-    x.add_all(p.part_l + at, p.R, reinterpret_cast<const float4*>(p.part_o) + at * (kHeadDim / 4) + piece,
-              static_cast<long long>(p.R) * (kHeadDim / 4), 8, from, own, W);
     const long long at_p = item_p + first_p;
     x.add_all(p.pre_l + at_p * 128 + rp, 128,
               reinterpret_cast<const float4*>(p.pre_o) + (at_p * (kHeadDim / 4) + piece) * 128 + rp,
               128 * (kHeadDim / 4), 8 * 128, from, pre, W);
+    const int s = c0 * heads + hr * n;
+    const int first = s / ln.quota, own = last_cta(ln, s, n) - first + 1;
+    const long long at = (static_cast<long long>(b) * heads + hr + first) * p.R + r;
+    x.add_all(p.part_l + at, p.R, reinterpret_cast<const float4*>(p.part_o) + at * (kHeadDim / 4) + piece,
+              static_cast<long long>(p.R) * (kHeadDim / 4), 8, from, own, W);
   }
   if (W > 1) {
 #pragma unroll
