@@ -64,6 +64,49 @@ def test_attention_over_the_cache(name):
     check_attention(o, lse, attention(q, c, q_lens))
 
 
+@pytest.mark.parametrize("name", ["odd_group", "group9_over_eight_rows", "group16", "drafts",
+                                  "drafts_ragged", "more_rows_than_tokens", "group32_rows", "chunk_odd",
+                                  "rows17"])
+def test_in_a_wide_table(name):
+    """What a call may hold decides the kernel for more than 8 rows a head; the table's unused width
+    counts for that and changes nothing else."""
+    lens, Hq, Hkv, Tq, q_lens, page, dtype, layout = DECODE[name]
+    c = Cache(lens, Hkv, page, dtype, 11, DEV, layout, width_extra=70016 // page)
+    q = _q(len(lens), Hq, Tq, dtype, 12)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV), q_lens=_ql(q_lens))
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c, q_lens))
+
+
+@pytest.mark.parametrize("Hq,Hkv,Tq,B", [(32, 8, 4, 4), (4, 1, 32, 3), (14, 2, 9, 2), (16, 16, 64, 1),
+                                         (128, 1, 1, 1), (5, 5, 27, 7)])
+@pytest.mark.parametrize("window,glob", [(None, 0), (1, 1)])
+def test_small_calls_of_many_rows(Hq, Hkv, Tq, B, window, glob):
+    c = Cache(_cycle([333, 90, 5, 256], B), Hkv, 16, BF16, 13, DEV)
+    q = _q(B, Hq, Tq, BF16, 14)
+    q_lens = _cycle([Tq, max(Tq - 3, 0), 1], B)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV), q_lens=_ql(q_lens), window=window,
+                               global_blocks=glob)
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c, q_lens, window or 0, glob))
+
+
+@pytest.mark.parametrize("Tq", [1, 5, 40, 200])
+def test_pages_outside_the_window_need_not_exist(Tq):
+    """Pages wholly outside the blocks that any row sees are not read: their entries may be anything."""
+    lens, page, window, glob = [1000, 1283, 700], 64, 2, 1
+    c = Cache(lens, 2, page, F16, 23, DEV)
+    q = _q(3, 4, Tq, F16, 24)
+    kp, vp, table, sl = c.to(DEV)
+    for b, n in enumerate(lens):
+        lo = (max(n - Tq, 0) // 128 - window + 1) * 128
+        table[b, glob * 128 // page:max(lo, 0) // page] = -1
+    assert (table[:, 2:6] == -1).any()
+    o, lse = ub.paged_attn_fwd(q.to(DEV), kp, vp, table, sl, window=window, global_blocks=glob)
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c, None, window, glob))
+
+
 @pytest.mark.parametrize("window,glob", [(1, 0), (2, 1), (3, 4), (64, 2)])
 @pytest.mark.parametrize("Tq,Hq", [(1, 8), (5, 4), (200, 2)])
 def test_window_and_global_blocks(window, glob, Tq, Hq):
@@ -265,12 +308,13 @@ def _expect_page_error():
     ub.check_errors(DEV)  # cleared
 
 
-@pytest.mark.parametrize("prefix,B,Tq", [(0, 3, 1), (0, 3, 40), (128, 3, 1), (2048, 66, 3)])
-def test_bad_pages_and_lengths_are_reported(prefix, B, Tq):
+@pytest.mark.parametrize("prefix,B,Tq,width", [(0, 3, 1, 1), (0, 3, 40, 1), (0, 3, 40, 2200),
+                                               (128, 3, 1, 1), (2048, 66, 3, 1)])
+def test_bad_pages_and_lengths_are_reported(prefix, B, Tq, width):
     """Out-of-range table entries, lengths and row counts are found and reported; the sequences
     that are in order keep their results."""
     lens_ = _cycle([prefix + 200, prefix + 190, prefix + 180], B)
-    c = Cache(lens_, 2, 16, F16, 81, DEV, prefix=prefix)
+    c = Cache(lens_, 2, 16, F16, 81, DEV, prefix=prefix, width_extra=width)
     q = _q(B, 4, Tq, F16, 82).to(DEV)
     kp, vp, table, lens = c.to(DEV)
     fn = (lambda *a, **k: ub.shared_prefix_attn_fwd(*a, prefix_len=prefix, **k)) if prefix \

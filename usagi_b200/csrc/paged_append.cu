@@ -208,7 +208,8 @@ extern "C" int bsattn_paged_append(const bsattn_paged_call* call, const void* q,
   p.Hq = Hq;
   const long long bx = (tokens + kTok - 1) / kTok;
   // One pass of the block's 16 row slots over kTok tokens covers 8 heads; with few tokens the
-  // heads are split over blocks down to that, so that every SM has work.
+  // heads are split over blocks down to that, so that every SM has work (one token of 48 heads: 2.4 us,
+  // in one block 3.6).
   long long split = std::min<long long>((heads + 7) / 8, std::max<long long>(1, 4ll * sms / bx));
   p.heads_per_block = static_cast<int>((heads + split - 1) / split);
   const dim3 grid(static_cast<unsigned>(bx),

@@ -2,8 +2,8 @@
 // of partial results.
 //
 // Rows of q that share a K/V head (G = Hq / Hkv query heads, Tq tokens) go together:
-//   * up to 8 rows: the few-row kernel (paged_few.cu), which is bound by memory;
-//   * more: the many-row kernel (paged_tile.cu), tiles of 128 rows on the tensor cores;
+//   * up to 8 rows, and more in small calls: the few-row kernel (paged_few.cu), which is bound by memory;
+//   * else the many-row kernel (paged_tile.cu), tiles of 128 rows on the tensor cores;
 //   * behind a shared prefix: the prefix's keys by the many-row kernel, over the stacked rows of the
 //     whole batch, the sequences' own keys by the few-row kernel beside it, and a join of both.
 #include <algorithm>
@@ -291,11 +291,24 @@ struct Shape {
   size_t cum, cuts, part_o, part_l, pre_o, pre_l, bytes;  // offsets into the scratch
 };
 
-constexpr int kStackedRows = 64; // more rows of one sequence fill a tile without its neighbours
+// More than 8 rows go to the few-row kernel as well, eight at a time over the same keys, when every such
+// item has a CTA of its own, there are no more than kSmallTiles for a K/V head, and a cache as large as the
+// page table allows is read in no more than kSmallBytes: it starts 3 us sooner and needs no join kernel.
+// Few-row and many-row kernel within that: 32 query heads on 8, 8 tokens, 1,000 keys (16 MB) 12.9 and 14.3
+// us; 64 on 8, 3 tokens, 4 sequences of 512 keys (24 MB) 12.1 and 16.0; 64 on 4, 8,192 keys (32 MB) 16.3 and
+// 22.3.  Outside: 32 on 8, 5 tokens, 4 sequences of 1,000 keys (48 MB) 18.1 and 17.4; 32 on 2, 16 tokens, 600
+// keys (32 for a head) 13.5 and 12.9; 32 on 8, 64 tokens, 200 keys (256 items) 16.6 and 13.3.
+// At 8 rows (64 on 8) the few-row kernel is ahead at any size: 8,192 keys 16.9 and 22.1, 32 sequences of
+// 4,096 keys 96.5 and 97.4.
+constexpr int kSmallTiles = 16;
+constexpr long long kSmallBytes = 32ll << 20;
+// More rows of one sequence fill a tile without its neighbours.  At 64 rows (32 sequences of 16 tokens, 32
+// heads on 8, behind 8,192 tokens) stacked 97 us, one sequence after the other 154.
+constexpr int kStackedRows = 64;
 // A prefix is read once when that saves at least this much reading; below, three launches and a join
 // cost more than the bytes, which L2 serves.  Measured, one pass over everything against prefix once,
-// 32 query heads on 8: 8 sequences behind 4,096 tokens (117 MB saved) 24.8 and 25.3 us, 16 behind 4,096
-// (252 MB) 36.8 and 27.3, 64 behind 1,024 (264 MB) 38.2 and 25.8, 16 behind 1,024 (63 MB) 18.6 and 22.1.
+// 32 query heads on 8: 8 sequences behind 4,096 tokens (117 MB saved) 24.5 and 23.4 us, 16 behind 4,096
+// (252 MB) 36.4 and 26.2, 64 behind 1,024 (264 MB) 38.4 and 26.3, 16 behind 1,024 (63 MB) 15.8 and 19.5.
 constexpr long long kSharedBytes = 128ll << 20;
 
 static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size, int prefix_len,
@@ -307,7 +320,10 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
   s->rows = static_cast<int>(rows);
   const long long saved = static_cast<long long>(B - 1) * prefix_len * Hkv * (4 * kHeadDim);
   s->prefix = prefix_len > 0 && rows <= kStackedRows && saved >= kSharedBytes;
-  s->few = s->prefix || rows <= kFewRows || G > 128;
+  const long long row_tiles = (rows + kFewRows - 1) / kFewRows;
+  const bool small = row_tiles <= kSmallTiles && row_tiles * B * Hkv <= sms &&
+                     row_tiles * B * Hkv * max_pages * page_size * (4 * kHeadDim) <= kSmallBytes;
+  s->few = s->prefix || rows <= kFewRows || small || G > 128;
   s->k0 = s->prefix ? prefix_len : 0;
   s->all_partial = s->prefix;
   // Most tiles one item can have.
@@ -316,7 +332,7 @@ static int shape_of(int B, int Hq, int Hkv, int Tq, int max_pages, int page_size
   long long items;
   if (s->few) {
     s->R = kFewRows;
-    s->row_tiles = static_cast<int>((rows + kFewRows - 1) / kFewRows);
+    s->row_tiles = static_cast<int>(row_tiles);
     s->count = B;
     items = static_cast<long long>(B) * Hkv * s->row_tiles;
   } else {
@@ -429,7 +445,8 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
   // Behind a prefix the few-row kernel takes the SMs as the other leaves them: it does not wait for it
   // to begin with (its inputs are there, the other has waited for them), but one of its CTAs holds it
   // open until the other has ended, so that the join may wait for it alone.  (Running both from the
-  // start, half of each one's CTAs at a time, was measured: 118 us against 108 at shared_wide's sizes.)
+  // start, half of each one's CTAs at a time, was measured: 118 us against 108 for 256 sequences behind
+  // 8,192 tokens.)
   if ((s.prefix || !s.few) && (rc = tile_launch(t, page_size, stream)) != BSATTN_OK) return rc;
   if (s.few && (rc = few_launch(f, stream)) != BSATTN_OK) return rc;
   if (s.prefix) {
@@ -452,7 +469,8 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     j.tiles_p = s.tiles_p;
     const long long items_p = static_cast<long long>(s.rt.count) * cache.Hkv;
     j.quota_p = static_cast<int>((items_p * s.tiles_p + s.pieces_p - 1) / s.pieces_p);
-    // Rows of many parts are shared by four warps.
+    // Rows of many parts are shared by four warps (18 parts: 70 us for the call against 78; 5 parts: 110
+    // against 105).
     const unsigned quads = static_cast<unsigned>(j.groups) * static_cast<unsigned>((s.rows + 3) / 4);
     return s.pieces_p / items_p >= 8
                ? launch(join_rows_kernel<kJoinWarps>, dim3(quads), kJoinWarps * 32, 0, stream, j)

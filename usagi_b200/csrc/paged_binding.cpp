@@ -1,7 +1,7 @@
 // paged_binding.cpp -- the Python side of the paged-cache calls, in C++.
 //
 // A decode step's call is a few microseconds of GPU time, and checking nine tensors' shapes, types and
-// strides from Python takes three times that (16 us a call against 7 here), so the checks of
+// strides from Python takes three times that (16 us a call against 6 here), so the checks of
 // usagi_b200/paged.py are made here, against the CPython interface.  The C ABI itself is reached
 // through the addresses that the package's one loaded library gives (init), so there is one library
 // and one set of kernels.
