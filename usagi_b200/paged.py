@@ -14,11 +14,15 @@ The cache is plain tensors that the caller owns:
   from 16 to 1024.  Any strides that are multiples of 8 with a contiguous last dimension: a
   ``[n_pages, page_size, Hkv, 128]`` cache is passed as ``pages.transpose(1, 2)``.
 * ``block_table``: int ``[B, max_pages]``, the pages of each sequence in order.  Entries behind a
-  sequence's length are not read and may be anything.
+  sequence's length are not read and may be anything, and so may, with a window, the entries of pages
+  that no row of the call sees.
 * ``seq_lens``: int ``[B]``, tokens of each sequence, the new ones of this call included.
 * ``q_lens``: int ``[B]`` or None, how many of the Tq rows of each sequence are live (None: all).
   Row t < q_lens[b] is the token at position ``seq_lens[b] - q_lens[b] + t``; the rows behind them are
   padding.
+
+Slots that hold no token may hold anything.  Values that are held must be finite: those that one row
+of a call sees reach the others as well, with weight 0, and 0 times NaN is NaN.
 
 A page table entry, a length or a row count out of range is found on the device, never used as an
 address, and raised by :func:`usagi_b200.check_errors` (code ``E_PAGE``).
@@ -84,7 +88,8 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     rot_dim values of every row of k and q are turned by position * inv_freq[i], pairs
     (x_i, x_{i + rot_dim/2}) or, ``interleaved``, (x_2i, x_{2i+1}); angles are formed in 64 bits.  Only
     the slots of live rows are written.  Returns the rotated q, contiguous, with zeros in padding
-    rows (``q_out`` when given; it may be q itself if that is contiguous), or None without q.
+    rows (``q_out`` when given; it may be q itself if that is contiguous), or None without q.  Sequences
+    must not share a page that new tokens go to.
     """
     return (_binding or _load()).append(k_pages, v_pages, block_table, seq_lens, k, v, q, q_lens,
                                         inv_freq, interleaved, q_out)
@@ -125,8 +130,8 @@ def shared_prefix_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
                            lse_out: Optional[torch.Tensor] = None, return_lse: bool = True
                            ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """:func:`paged_attn_fwd` for a batch whose sequences all begin with the same ``prefix_len``
-    tokens (a system prompt, a document): whole pages, the same ones at the front of every row of
-    ``block_table``.  Where it pays they are read once for the whole batch, through the row of sequence
+    tokens (a system prompt, a document): whole pages, all held, the same ones at the front of every row
+    of ``block_table`` (also in the rows of shorter sequences).  Where it pays they are read once for the whole batch, through the row of sequence
     0, with the rows of all sequences stacked on the tensor cores.  Same arguments and same result as
     :func:`paged_attn_fwd` without a window; a sequence may also be shorter than the prefix.
     """
