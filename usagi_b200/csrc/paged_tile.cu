@@ -525,12 +525,19 @@ __device__ void softmax_role(Smem& sh, const Params& p, int half, uint32_t tmem)
     if (sg.n == 0) break;
     const int ob = ii & 1;
     const RowKeys rk = row_of(p, sg, t).k;
+    // Nobody reads what becomes of a warp's rows if none of them is live.
+    const bool dead = __all_sync(0xffffffffu, rk.limit <= 0);
     float m_run = kNoMax, l_run = 0.0f;
     for (int j = 0; j < sg.n; ++j, ++tile) {
       const int sb = tile & 1;
       const uint32_t s_addr = lane_addr + sb * 128 + half * 64;
       if (!wait_warp(ptx::smem_u32(&sh.s_full[sb]), (static_cast<uint32_t>(tile) >> 1) & 1u, sh, p))
         return;
+      if (dead) {
+        ptx::mbar_arrive(ptx::smem_u32(&sh.xchg[sb][wq]));
+        ptx::mbar_arrive(ptx::smem_u32(&sh.p_rdy[sb][half]));
+        continue;
+      }
       ptx::tc_fence_after();
       uint32_t sr[64];
       ptx::tmem_ld32(s_addr + 0, sr + 0);
