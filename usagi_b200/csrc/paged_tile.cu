@@ -250,7 +250,11 @@ struct Stream {
   uint32_t tail_phase, tail_busy;
   uint64_t *full, *empty;
   uint8_t* tiles;
+  uint32_t lane_at;  // where this lane's box lies in a tile
 };
+__device__ __forceinline__ uint32_t lane_box_at(const Params& p) {
+  return (threadIdx.x & 1) * kHalfBytes + ((threadIdx.x & 31) >> 1) * p.box_rows * 128;
+}
 
 // Page of this lane's box (lane / 2) of the tile at key0, or -1: past the end, or no such box.
 __device__ __forceinline__ int box_page(const Params& p, const Seg& s, int j) {
@@ -261,50 +265,65 @@ __device__ __forceinline__ int box_page(const Params& p, const Seg& s, int j) {
   return __ldg(p.c.table + b * p.c.table_stride + (key >> p.c.page_shift));
 }
 
-__device__ __forceinline__ bool load_tile(Smem& sh, const Params& p, Stream& x, const CUtensorMap* map,
-                                          const Seg& s, int j, int page) {
+// A tile with rows that must be zero: of V behind the sequence's end, of both where there is no page.
+__device__ __forceinline__ bool load_ragged(Smem& sh, const Params& p, Stream& x, const CUtensorMap* map, int key0,
+                                         int have, int h, int page, uint32_t dst) {
   const int lane = threadIdx.x & 31, box = lane >> 1, half = lane & 1;
   const bool lead = lane == 0;
-  if (!wait_warp(ptx::smem_u32(x.empty + x.stage), x.phase ^ 1u, sh, p)) return false;
   const uint32_t full = ptx::smem_u32(x.full + x.stage);
   const uint32_t tail = ptx::smem_u32(&sh.tail[x.is_v]);
-  const uint32_t dst = ptx::smem_u32(x.tiles) + x.stage * kTileBytes;
-  const int key0 = seg_key(s, j);
-  const int have = s.load_end - key0;  // rows that hold a token
   const bool mine = box < p.boxes && box * p.box_rows < have;
   if (mine) page = page_checked(p.c, page);
   const bool get = mine && page >= 0;
   const uint32_t got = __ballot_sync(0xffffffffu, get);
   const bool hole = __any_sync(0xffffffffu, mine && !get);
   const uint32_t bytes = __popc(got) * p.box_rows * 128;
-  // Rows that must be zero: of V behind the end, of both where there is no page.
   const bool fill = hole || (x.is_v && have < kTileKeys);
   const uint32_t bar = fill ? tail : full;
   if (lead && bytes > 0) ptx::mbar_expect_tx(bar, bytes);
   if (lead && bytes == 0 && !fill) ptx::mbar_arrive(bar);
   __syncwarp();
   if (get)
-    tma_load_5d(dst + half * kHalfBytes + box * p.box_rows * 128, map, bar, 0,
-                key0 & (p.page_size - 1) & ~(p.box_rows - 1), s.h, page, half);
-  if (fill) {
-    if (bytes > 0) {
-      x.tail_busy = 1;
-      if (!wait_warp(tail, x.tail_phase, sh, p)) return false;
-      x.tail_phase ^= 1u;
-      x.tail_busy = 0;
-    }
-    // Lane l writes piece l % 8 of half (l / 8) % 2, rows l / 16, + 2, ...
-    const uint32_t at = dst + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;
-    if (hole) {
-      for (int row = lane >> 4; row < min(have, kTileKeys); row += 2)
-        if (!((got >> ((row >> p.box_shift) * 2)) & 1u)) ptx::sts128(at + row * 128, 0, 0, 0, 0);
-    }
+    tma_load_5d(dst + half * kHalfBytes + box * p.box_rows * 128, map, bar, 0, key0 & (p.page_size - 1), h, page,
+                half);
+  if (!fill) return true;
+  if (bytes > 0) {
+    x.tail_busy = 1;
+    if (!wait_warp(tail, x.tail_phase, sh, p)) return false;
+    x.tail_phase ^= 1u;
+    x.tail_busy = 0;
+  }
+  // Lane l writes piece l % 8 of half (l / 8) % 2, rows l / 16, + 2, ...
+  const uint32_t at = dst + ((lane >> 3) & 1) * kHalfBytes + (lane & 7) * 16;
+  if (hole) {
+    for (int row = lane >> 4; row < min(have, kTileKeys); row += 2)
+      if (!((got >> ((row >> p.box_shift) * 2)) & 1u)) ptx::sts128(at + row * 128, 0, 0, 0, 0);
+  }
 #pragma unroll 4
-    for (int row = max(have, 0) + (lane >> 4); row < kTileKeys; row += 2)
-      ptx::sts128(at + row * 128, 0, 0, 0, 0);
-    ptx::fence_async_smem();
+  for (int row = max(have, 0) + (lane >> 4); row < kTileKeys; row += 2)
+    ptx::sts128(at + row * 128, 0, 0, 0, 0);
+  ptx::fence_async_smem();
+  __syncwarp();
+  if (lead) ptx::mbar_arrive(full);
+  return true;
+}
+
+__device__ __forceinline__ bool load_tile(Smem& sh, const Params& p, Stream& x, const CUtensorMap* map,
+                                          const Seg& s, int j, int page) {
+  const int lane = threadIdx.x & 31;
+  const int key0 = seg_key(s, j), have = s.load_end - key0;  // rows that hold a token
+  const bool mine = (lane >> 1) < p.boxes;
+  const bool whole = __all_sync(0xffffffffu, have >= kTileKeys && (!mine || static_cast<unsigned>(page) <
+                                                                           static_cast<unsigned>(p.c.n_pages)));
+  if (!wait_warp(ptx::smem_u32(x.empty + x.stage), x.phase ^ 1u, sh, p)) return false;
+  const uint32_t dst = ptx::smem_u32(x.tiles) + x.stage * kTileBytes;
+  if (whole) {
+    const uint32_t full = ptx::smem_u32(x.full + x.stage);
+    if (lane == 0) ptx::mbar_expect_tx(full, kTileBytes);
     __syncwarp();
-    if (lead) ptx::mbar_arrive(full);
+    if (mine) tma_load_5d(dst + x.lane_at, map, full, 0, key0 & (p.page_size - 1), s.h, page, lane & 1);
+  } else if (!load_ragged(sh, p, x, map, key0, have, s.h, page, dst)) {
+    return false;
   }
   x.issued |= 1u << x.stage;
   x.last_parity = (x.last_parity & ~(1u << x.stage)) | (x.phase << x.stage);
@@ -326,7 +345,7 @@ __device__ void producer_k_role(Smem& sh, const CUtensorMap* tq, const CUtensorM
                                 int begin, int end, int quota) {
   const bool lead = (threadIdx.x & 31) == 0;
   int q_loads = 0;
-  Stream x{0, 0, 0, 0, 0, 0, 0, sh.k_full, sh.k_empty, sh.k[0]};
+  Stream x{0, 0, 0, 0, 0, 0, 0, sh.k_full, sh.k_empty, sh.k[0], lane_box_at(p)};
   int v = sh.found_v, h = sh.found_h, tl = sh.found_tile;
   VTiles vt = sh.found;
   int left = end - begin;
@@ -395,7 +414,7 @@ __device__ void producer_k_role(Smem& sh, const CUtensorMap* tq, const CUtensorM
 
 __device__ void producer_v_role(Smem& sh, const CUtensorMap* tv, const Params& p) {
   const bool lead = (threadIdx.x & 31) == 0;
-  Stream x{1, 0, 0, 0, 0, 0, 0, sh.v_full, sh.v_empty, sh.v[0]};
+  Stream x{1, 0, 0, 0, 0, 0, 0, sh.v_full, sh.v_empty, sh.v[0], lane_box_at(p)};
   bool ok = true;
   for (int k = 0; ok; ++k) {
     const int slot = k & (kRing - 1);
