@@ -443,7 +443,7 @@ static int launch_paged(const void* q, const Cache& cache, Rule rule, int prefix
     f.counters = counters;
   }
   // Behind a prefix the few-row kernel takes the SMs as the other leaves them: it does not wait for it
-  // to begin with (its inputs are there, the other has waited for them), but one of its CTAs holds it
+  // to begin with (its inputs are there, the other has waited for them), but its last CTA holds it
   // open until the other has ended, so that the join may wait for it alone.  (Running both from the
   // start, half of each one's CTAs at a time, was measured: 118 us against 108 for 256 sequences behind
   // 8,192 tokens.)

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     ld = sh.found;
   }
   if (cta_begin >= cta_end) {
-    if (p.all_partial && blockIdx.x == 0) pdl_wait();
+    if (p.all_partial && blockIdx.x + 1 == gridDim.x) pdl_wait();
     return;
   }
 
@@ -288,6 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   const int lr = lane >> 4, lc = lane & 15;
   const uint32_t ld_dst = lr * (kHeadDim * 2) + ((lc ^ lr) << 4);
   int ld_stage = 0;
+  // Behind a prefix this leaves its keys and the partial results in L2: 256 sequences behind 8,192 tokens
+  // 107 us without it, 100 with it; 64 behind 32,768 81 and 78.
+  const uint64_t pol = evict_first_policy();
   auto load_next = [&]() {
     if (valid(ld)) {
       const int key = ld.key();
@@ -306,8 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
           for (int i = 0; i < kSlice / 2; ++i) {
             const uint32_t d = (dst ^ ((2 * i & 7) << 4)) + 2 * i * (kHeadDim * 2);
-            cp_async16(d, ks + i * (kHeadDim * 4));
-            cp_async16(d + kSliceBytes, vs + i * (kHeadDim * 4));
+            cp_async16(d, ks + i * (kHeadDim * 4), pol);
+            cp_async16(d + kSliceBytes, vs + i * (kHeadDim * 4), pol);
           }
         } else {
           const char *ka[kSlice / 2], *va[kSlice / 2];
@@ -320,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
           for (int i = 0; i < kSlice / 2; ++i) {
             const uint32_t d = (dst ^ ((2 * i & 7) << 4)) + 2 * i * (kHeadDim * 2);
             const uint32_t bytes = 2 * i < have ? 16u : 0u;
-            cp_async16(d, ka[i], bytes);
-            cp_async16(d + kSliceBytes, va[i], bytes);
+            cp_async16(d, ka[i], bytes, pol);
+            cp_async16(d + kSliceBytes, va[i], bytes, pol);
           }
         }
       }
@@ -637,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
       join_row(p, split[s].q_row + warp, warp, R, split[s].first, split[s].last, lane);
     }
   }
-  if (p.all_partial && blockIdx.x == 0) pdl_wait();
+  if (p.all_partial && blockIdx.x + 1 == gridDim.x) pdl_wait();
 }
 
 }  // namespace few
