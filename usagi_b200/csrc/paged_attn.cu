@@ -195,6 +195,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_cuts_kernel(const __grid
   const int first = blockIdx.x;
   pdl_wait();
   pdl_trigger();
+  // The piece that begins the item lies in slot 2 first + 1, the others in 2 (first + 1), + 2, ...: the first
+  // two are asked for before it is known whether there is an item.
+  constexpr int kSlot = 128 * (kHeadDim / 4);
+  const float* l = p.part_l + (2ll * first + 1) * 128 + r;
+  const float4* o = reinterpret_cast<const float4*>(p.part_o) + (2ll * first + 1) * kSlot + piece * 128 + r;
+  float4 y[2][4];
+  float lg[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const bool there = first + c < static_cast<int>(gridDim.x);
+    lg[c] = there ? __ldcg(l + c * 128) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      y[c][i] = there ? __ldcg(o + c * kSlot + i * (8 * 128)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
   const TileCut cut = p.cuts[first];
   if (cut.v < 0) return;
   const int b = cut.v / p.rt.per_seq;
@@ -202,13 +217,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_cuts_kernel(const __grid
   if (g >= p.rt.G || t >= p.Tq) return;
   Quad x;
   x.clear();
-  // The piece that begins the item lies in slot 2 first + 1, the others in 2 (first + 1), + 2, ...
-  const float* l = p.part_l + r;
-  const float4* o = reinterpret_cast<const float4*>(p.part_o) + piece * 128 + r;
-  constexpr int kSlot = 128 * (kHeadDim / 4);
-  const long long head = 2ll * first + 1, rest = 2ll * first + 2;
-  x.add_all(l + head * 128, 0, o + head * kSlot, 0, 8 * 128, 0, 1, 1);
-  x.add_all(l + rest * 128, 256, o + rest * kSlot, 2 * kSlot, 8 * 128, 0, cut.pieces - 1, 1);
+  x.add(y, lg);
+  x.add_all(l + 3 * 128, 256, o + 3 * kSlot, 2 * kSlot, 8 * 128, 0, cut.pieces - 2, 1);
   x.store(p.o, p.lse, p.out_bf16, ((static_cast<long long>(b) * p.Hkv + cut.h) * p.rt.G + g) * p.Tq + t, piece);
 }
 
