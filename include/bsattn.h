@@ -213,7 +213,8 @@ BSATTN_API int bsattn_peer_copy(void* dst, const void* src, size_t bytes, void* 
  * A page table entry outside [0, n_pages), a length outside the table or a live row count outside
  * [0, Tq] is reported as BSATTN_E_PAGE through bsattn_check_error and never used as an address:
  * the length or count is forced into range, the entry's tokens are not written, and are read as
- * zeros.  Slots that hold no token of a sequence are never used, whatever their bits are. */
+ * zeros.  Slots that hold no token of a sequence are never used, whatever their bits are; values that
+ * are held must be finite, since one that a row's mask excludes may still enter it with weight 0. */
 typedef struct bsattn_paged_call {
   void* k_pages;              /* fp16 or bf16 [n_pages, Hkv, page_size, 128], 16-byte aligned      */
   void* v_pages;
@@ -241,7 +242,7 @@ typedef struct bsattn_paged_call {
  * padding rows), are turned: pair i = (x_i, x_{i + rot_dim/2}), or (x_2i, x_{2i+1}) when interleaved, by
  * position * inv_freq[i].  inv_freq NULL: no rotation.  Hq == 0: no q.  q_out may be q itself when q is
  * contiguous.  in_strides[9] (host) = elements between batches, heads and tokens of q, k, v.  Two rows
- * of one call in the same slot (a page in two places of the table) leave one of them there. */
+ * of one call must not share a slot (a page in two places of the table): parts of both could be left. */
 BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q, const void* k,
                                    const void* v, const int64_t* in_strides, void* q_out,
                                    const double* inv_freq, int rot_dim, int interleaved);
