@@ -423,6 +423,29 @@ def test_first_call_on_a_stream_inside_capture_is_refused():
     del graph
 
 
+def test_wide_integers_and_floats_as_indexes():
+    """64-bit metadata whose low 32 bits look right is out of range; floats are refused."""
+    c = Cache([40, 33], 2, 16, F16, 87, DEV)
+    (kp, vp, table, lens), q = c.to(DEV), _q(2, 4, 1, F16, 88)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), kp, vp, table.long(), lens.long(),
+                               q_lens=torch.ones(2, dtype=torch.int64, device=DEV))
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c))
+    for far in (2 ** 32, -2 ** 32):
+        ub.paged_attn_fwd(q.to(DEV), kp, vp, table.long() + far, lens)
+        _expect_page_error()
+        ub.paged_attn_fwd(q.to(DEV), kp, vp, table, lens.long() + far)
+        _expect_page_error()
+        ub.paged_attn_fwd(q.to(DEV), kp, vp, table, lens,
+                          q_lens=torch.full((2,), 1 + far, dtype=torch.int64, device=DEV))
+        _expect_page_error()
+    for bad in (dict(block_table=table.float()), dict(seq_lens=lens.half()), dict(q_lens=lens > 0)):
+        kw = dict(block_table=table, seq_lens=lens, q_lens=None)
+        kw.update(bad)
+        with pytest.raises(TypeError, match="integers"):
+            ub.paged_attn_fwd(q.to(DEV), kp, vp, **kw)
+
+
 def test_gradients_are_not_recorded():
     c = Cache([40], 2, 16, F16, 89, DEV)
     args, q = c.to(DEV), _q(1, 4, 1, F16, 90).to(DEV).requires_grad_()

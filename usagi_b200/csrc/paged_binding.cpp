@@ -82,6 +82,10 @@ at::Tensor index_tensor(const at::Tensor& t, const char* name, c10::Device dev, 
     refuse(PyExc_ValueError, std::string(name) + ": expected shape " + shape_text(shape) + ", got " +
                                  shape_text(t.sizes()));
   at::Tensor x = t;
+  if (!at::isIntegralType(x.scalar_type(), false))
+    refuse(PyExc_TypeError, std::string(name) + " must hold integers");
+  // What 32 bits do not hold stays out of range, where the kernels find it.
+  if (x.scalar_type() == at::kLong) x = x.clamp(INT32_MIN, INT32_MAX);
   if (x.scalar_type() != at::kInt || x.device() != dev) x = x.to(dev, at::kInt);
   if (x.stride(-1) != 1 && x.size(-1) > 1) x = x.contiguous();
   return x;
