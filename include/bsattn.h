@@ -254,6 +254,7 @@ BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q,
  * multiple of page_size; without a window) says that the first prefix_len tokens of every sequence are
  * the same pages, those of sequence 0's table row: they may be read once for the whole batch.  The
  * result is that of prefix_len == 0.  Dead rows and rows without keys get o = 0 and lse = -inf.
+ * scale <= 0 selects 1/sqrt(128).
  * scratch: bsattn_paged_scratch_bytes bytes of device memory, 16-byte aligned, any content, used by
  * this call only.  counters: bsattn_paged_counters() ints of device memory, zero before their first
  * use; every call leaves them zero, and calls that may run at the same time need their own. */

@@ -378,6 +378,8 @@ def test_refusals():
             lambda: attn(q_lens=lens[:1]), lambda: attn(out=q[:1]), lambda: attn(out=q.float()),
             lambda: attn(lse_out=torch.zeros(2, 4, device=DEV)), lambda: attn(window=0),
             lambda: attn(global_blocks=1), lambda: attn(window=2, global_blocks=-1),
+            lambda: attn(scale=0.0), lambda: attn(scale=-0.1), lambda: attn(scale=float("nan")),
+            lambda: attn(scale=1e39),
             lambda: attn(window=2 ** 40), lambda: shared(24), lambda: shared(-16),
             lambda: shared(16 * (table.shape[1] + 1)), lambda: shared(2 ** 40),
             lambda: append(k=k[0]), lambda: append(k=k[:1]), lambda: append(v=q),

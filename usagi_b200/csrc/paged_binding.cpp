@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <map>
 #include <string>
 #include <utility>
@@ -305,6 +306,9 @@ PyObject* attn_impl(PyObject* const* a) {
   if (!is_none(a[9])) {
     scale = PyFloat_AsDouble(a[9]);
     if (scale == -1.0 && PyErr_Occurred()) throw Raised();
+    // The C ABI takes 0 for the default.
+    if (!(static_cast<float>(scale) > 0.0f) || std::isinf(static_cast<float>(scale)))
+      refuse(PyExc_ValueError, "scale must be positive and finite");
   }
   at::ScalarType out_dtype = call.dtype;
   if (!is_none(a[10])) {

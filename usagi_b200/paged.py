@@ -111,7 +111,7 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``global_blocks``: the rows of :func:`usagi_b200.block_sparse_attn_fwd_window`.  Returns
     ``(o, lse)`` like the prefill calls: o ``[B, Hq, Tq, 128]`` in ``out_dtype`` (default: q's),
     lse fp32 ``[B, Hq, Tq]`` (None if ``return_lse=False``); rows without a key, padding among them,
-    get o = 0, lse = -inf.
+    get o = 0, lse = -inf.  ``scale`` is positive (None: 1/sqrt(128)).
     """
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1 block, got {window}")
