@@ -222,7 +222,8 @@ typedef struct bsattn_paged_call {
                                  multiples of 8, positive where the dimension is not 1; the 128
                                  values of a token and head are contiguous                         */
   const int32_t* block_table; /* tokens n * page_size .. of sequence b: page [b * table_stride + n];
-                                 entries behind a sequence's length are not read                   */
+                                 entries behind a sequence's length are not read, none of a
+                                 sequence without live rows (prefix_len: from that token on)       */
   int64_t table_stride;
   const int32_t* seq_lens;    /* [B] tokens of each sequence, the new ones of this call included   */
   const int32_t* q_lens;      /* [B] live rows of each sequence, 0 .. Tq; NULL: Tq for all         */

@@ -1,0 +1,65 @@
+"""Edges of the paged-cache calls: sequences that take no part in a call, limits of the arguments, layouts
+that differ only where a dimension has one entry, and what a call leaves behind.  Bounds as in
+paged_reference.py; every cache has NaN in all slots that hold no token."""
+import pytest
+import torch
+
+import usagi_b200 as ub
+from usagi_b200 import _lib
+from paged_reference import Cache, attention, check_attention
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _setup():
+    ub.setup(device="cuda:0")
+    yield
+    ub.check_errors(DEV)
+
+
+def _q(B, Hq, Tq, dtype, seed, gain=2.0):
+    return (gain * torch.randn(B, Hq, Tq, 128,
+                               generator=torch.Generator().manual_seed(seed))).to(dtype)
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def _expect_page_error():
+    with pytest.raises(ub.BsattnError) as err:
+        ub.check_errors(DEV)
+    assert err.value.code == _lib.E_PAGE
+    ub.check_errors(DEV)  # cleared
+
+
+# (prefix, B, Hq, Tq, width): one row and a few by the few-row kernel, up to 32 sequences and more, several
+# tiles of rows; many rows; behind a prefix that is read once.
+IDLE = {"one_row": (0, 3, 4, 1, 1), "rows": (0, 4, 4, 3, 1), "sequences": (0, 40, 4, 1, 1),
+        "row_tiles": (0, 3, 8, 6, 1), "many_rows": (0, 3, 8, 40, 1), "wide": (0, 4, 8, 9, 2200),
+        "prefix": (2048, 66, 4, 1, 1), "prefix_rows": (2048, 70, 4, 5, 1)}
+
+
+@pytest.mark.parametrize("entry", ["none", "recycled"])
+@pytest.mark.parametrize("name,window,glob", [(n, w, g) for n in IDLE for w, g in (
+    [(None, 0)] if IDLE[n][0] else [(None, 0), (2, 0), (1, 1)])])
+def test_a_sequence_without_live_rows_is_not_read(name, window, glob, entry):
+    """q_lens[b] == 0: none of its pages is needed, so their entries may be no page at all or pages that
+    hold something else by now; its rows are padding."""
+    prefix, B, Hq, Tq, width = IDLE[name]
+    lens = [prefix + [700, 300, 1283, 129][b % 4] for b in range(B)]
+    c = Cache(lens, 2, 16, F16, 211, DEV, prefix=prefix, width_extra=width)
+    q, q_lens = _q(B, Hq, Tq, F16, 212), [0 if b % 3 == 1 else Tq for b in range(B)]
+    kp, vp, table, sl = c.to(DEV)
+    free = next(i for i in range(kp.shape[0]) if torch.isnan(kp[i]).all())
+    for b in range(1, B, 3):
+        table[b, prefix // 16:] = -1 if entry == "none" else free
+    kw = dict(prefix_len=prefix) if prefix else dict(window=window, global_blocks=glob)
+    fn = ub.shared_prefix_attn_fwd if prefix else ub.paged_attn_fwd
+    o, lse = fn(q.to(DEV), kp, vp, table, sl, q_lens=_ints(q_lens), **kw)
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c, q_lens, window or 0, glob))

@@ -71,8 +71,8 @@ struct Part {
 };
 
 // The slices of one sequence, those any live row sees, in ascending order: n_glob leading ones, then
-// those from key `lo` on.  A sequence without a key still gets one slice, so that every row is
-// written by the same path.
+// those from key `lo` on.  A sequence without a key or a live row still gets one slice, so that every
+// row is written by the same path; its length is 0 here, so nothing of it is read.
 struct Slices {
   int len;
   Rows r;
@@ -81,7 +81,7 @@ struct Slices {
 __device__ __forceinline__ Slices slices_of(const Params& p, int b) {
   const SeqLen s = seq_len(p.c, b);
   Slices t;
-  t.len = s.len;
+  t.len = s.rows > 0 ? s.len : 0;
   t.r = Rows{s.rows, s.len - s.rows};
   t.lo = p.rule.k0;
   t.n_glob = 0;

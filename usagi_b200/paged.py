@@ -15,7 +15,8 @@ The cache is plain tensors that the caller owns:
   ``[n_pages, page_size, Hkv, 128]`` cache is passed as ``pages.transpose(1, 2)``.
 * ``block_table``: int ``[B, max_pages]``, the pages of each sequence in order.  Entries behind a
   sequence's length are not read and may be anything, and so may, with a window, the entries of pages
-  that no row of the call sees.
+  that no row of the call sees, and all entries of a sequence without live rows (behind a shared prefix
+  those of its own pages).
 * ``seq_lens``: int ``[B]``, tokens of each sequence, the new ones of this call included.
 * ``q_lens``: int ``[B]`` or None, how many of the Tq rows of each sequence are live (None: all).
   Row t < q_lens[b] is the token at position ``seq_lens[b] - q_lens[b] + t``; the rows behind them are
