@@ -251,10 +251,11 @@ BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q,
 /* Attention of the live rows over the cache, the new tokens included: o [B, Hq, Tq, 128] (contiguous,
  * like q) and lse [B, Hq, Tq] (or NULL), each group of Hq / Hkv query heads on one K/V head, keys at
  * positions up to the row's own.  window > 0 keeps, for a row in block i = position / 128, the keys of
- * blocks < global_blocks and > i - window: the rows that bsattn_fwd_window computes.  prefix_len > 0 (a
- * multiple of page_size; without a window) says that the first prefix_len tokens of every sequence are
- * the same pages, those of sequence 0's table row: they may be read once for the whole batch.  The
- * result is that of prefix_len == 0.  Dead rows and rows without keys get o = 0 and lse = -inf.
+ * blocks < global_blocks and > i - window: the rows that bsattn_fwd_window computes (both up to 2^24).
+ * prefix_len > 0 (a multiple of page_size; without a window) says that the first prefix_len tokens of
+ * every sequence are the same pages, those of sequence 0's table row: they may be read once for the
+ * whole batch.  The result is that of prefix_len == 0.  Dead rows and rows without keys get o = 0 and
+ * lse = -inf.
  * scale <= 0 selects 1/sqrt(128).
  * scratch: bsattn_paged_scratch_bytes bytes of device memory, 16-byte aligned, any content, used by
  * this call only.  counters: bsattn_paged_counters() ints of device memory, zero before their first

@@ -63,3 +63,14 @@ def test_a_sequence_without_live_rows_is_not_read(name, window, glob, entry):
     o, lse = fn(q.to(DEV), kp, vp, table, sl, q_lens=_ints(q_lens), **kw)
     ub.check_errors(DEV)
     check_attention(o, lse, attention(q, c, q_lens, window or 0, glob))
+
+
+@pytest.mark.parametrize("Tq,Hq", [(1, 8), (5, 4), (200, 2)])
+@pytest.mark.parametrize("glob", [1 << 24, (1 << 24) - 1, 1 << 20])
+def test_global_blocks_up_to_the_limit(glob, Tq, Hq):
+    """More global blocks than a sequence has: every key up to the row's own."""
+    c = Cache([700, 2000, 130], 2, 32, F16, 221, DEV)
+    q = _q(3, Hq, Tq, F16, 222)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV), window=1, global_blocks=glob)
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c, None, 1, glob))

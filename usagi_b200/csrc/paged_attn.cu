@@ -544,7 +544,10 @@ int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, floa
       prefix_len > static_cast<long long>(call->max_pages) * call->page_size ||
       (prefix_len > 0 && window > 0))
     return BSATTN_E_SHAPE;
-  const Rule rule{0, window, global_blocks};
+  // More global blocks than the table holds are the same as all of them, whose keys 32 bits can count.
+  const long long cap = static_cast<long long>(call->max_pages) * call->page_size;
+  const int blocks = static_cast<int>((cap + kTileKeys - 1) / kTileKeys);
+  const Rule rule{0, window, std::min(global_blocks, blocks)};
   return launch_paged(q, c, rule, prefix_len, call->Hq, scale, call->dtype_flags, call->page_size, o,
                       lse, scratch, scratch_bytes, counters, static_cast<cudaStream_t>(call->stream));
 }
