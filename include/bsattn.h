@@ -242,8 +242,9 @@ typedef struct bsattn_paged_call {
  * rot_dim values of each row of k, and of q [B, Hq, Tq, 128] on its way to q_out (contiguous; zero in
  * padding rows), are turned: pair i = (x_i, x_{i + rot_dim/2}), or (x_2i, x_{2i+1}) when interleaved, by
  * position * inv_freq[i].  inv_freq NULL: no rotation.  Hq == 0: no q.  q_out may be q itself when q is
- * contiguous.  in_strides[9] (host) = elements between batches, heads and tokens of q, k, v.  Two rows
- * of one call must not share a slot (a page in two places of the table): parts of both could be left. */
+ * contiguous.  in_strides[9] (host) = elements between batches, heads and tokens of q, k, v: multiples
+ * of 8, also where the dimension is 1.  Two rows of one call must not share a slot (a page in two places
+ * of the table): parts of both could be left. */
 BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q, const void* k,
                                    const void* v, const int64_t* in_strides, void* q_out,
                                    const double* inv_freq, int rot_dim, int interleaved);

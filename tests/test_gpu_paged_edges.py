@@ -74,3 +74,45 @@ def test_global_blocks_up_to_the_limit(glob, Tq, Hq):
     o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV), window=1, global_blocks=glob)
     ub.check_errors(DEV)
     check_attention(o, lse, attention(q, c, None, 1, glob))
+
+
+def _odd_strides(x):
+    """x with strides of no use (1, 3, 5) in its dimensions of one entry."""
+    s = [o if n == 1 else st for n, st, o in zip(x.shape, x.stride(), (3, 5, 1, 1))]
+    return torch.as_strided(x, x.shape, s)
+
+
+@pytest.mark.parametrize("B,H,Tq", [(3, 2, 1), (1, 2, 3), (2, 1, 2), (1, 1, 1)])
+def test_strides_of_dimensions_of_one_entry_do_not_matter(B, H, Tq):
+    c = Cache([40, 33, 20][:B], H, 16, F16, 231, DEV)
+    q, k, v = [_q(B, H, Tq, F16, 232 + i).to(DEV) for i in range(3)]
+    inv = ub.rope_inv_freq(128, device=DEV)
+    a, b = c.to(DEV), c.to(DEV)
+    want = ub.paged_kv_append(*a, k, v, q=q, inv_freq=inv)
+    got = ub.paged_kv_append(*b, _odd_strides(k), _odd_strides(v), q=_odd_strides(q), inv_freq=inv)
+    assert torch.equal(got, want)
+    for x, y in zip(a[:2], b[:2]):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+    o, lse = ub.paged_attn_fwd(want, *a)
+    o2, lse2 = ub.paged_attn_fwd(_odd_strides(want), *b)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    # a token made by a transpose: its stride over the one token is 1
+    one = torch.randn(B, H, 128, 1, generator=torch.Generator().manual_seed(235)).half().to(DEV)
+    got = ub.paged_kv_append(*b, one.transpose(2, 3), one.transpose(2, 3))
+    assert got is None
+    ub.check_errors(DEV)
+
+
+@pytest.mark.parametrize("Tq,Hq", [(1, 4), (40, 16)])
+def test_strides_of_one_page_or_head_do_not_matter(Tq, Hq):
+    c = Cache([900], 1, 1024, F16, 236, DEV, extra_pages=0, width_extra=0)
+    q = _q(1, Hq, Tq, F16, 237).to(DEV)
+    kp, vp, table, lens = c.to(DEV)
+    kp, vp = _odd_strides(kp), _odd_strides(vp)
+    assert kp.stride() == (3, 5, 128, 1)
+    x = c.pages[0][c.table[0, 0].long(), :, 900 - Tq:900][None].to(DEV)
+    y = c.pages[1][c.table[0, 0].long(), :, 900 - Tq:900][None].to(DEV)
+    ub.paged_kv_append(kp, vp, table, lens, x, y)
+    o, lse = ub.paged_attn_fwd(q, kp, vp, table, lens)
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q.cpu(), c))

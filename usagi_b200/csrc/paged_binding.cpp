@@ -65,6 +65,12 @@ int64_t integer(PyObject* o, const char* name) {
   return v;
 }
 
+// Stride of a dimension; one of a single entry is never used, whatever torch holds for it.
+int64_t stride_of(const at::Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : kHeadDim; }
+// Whether rows of 128 contiguous values begin at multiples of 8.
+bool rows_of_eight(const at::Tensor& t) {
+  return t.stride(3) == 1 && ((stride_of(t, 0) | stride_of(t, 1) | stride_of(t, 2)) & 7) == 0;
+}
 bool misaligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0; }
 
 void check_call(int rc, const char* where) {
@@ -100,8 +106,7 @@ at::Tensor rows_tensor(const at::Tensor& t, const char* name, c10::Device dev, a
            std::string(name) + " must be " + shape_text(shape) + ", got " + shape_text(t.sizes()));
   if (t.scalar_type() != dtype || t.device() != dev)
     refuse(PyExc_TypeError, std::string(name) + " must have the dtype and device of the pages");
-  const at::IntArrayRef s = t.strides();
-  if (s[3] == 1 && ((s[0] | s[1] | s[2]) & 7) == 0 && !misaligned(t)) return t;
+  if (rows_of_eight(t) && !misaligned(t)) return t;
   at::Tensor x = t.contiguous();
   return misaligned(x) ? x.clone() : x;
 }
@@ -137,9 +142,7 @@ struct Call {
       refuse(PyExc_ValueError, "the cache has no pages or no heads: " + shape_text(k.sizes()));
     if (page < 16 || page > 1024 || (page & (page - 1)) != 0)
       refuse(PyExc_ValueError, "page_size must be a power of two from 16 to 1024, got " + std::to_string(page));
-    const at::IntArrayRef ks = k.strides(), vs = v.strides();
-    if (ks[3] != 1 || vs[3] != 1 || ((ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7) != 0 ||
-        misaligned(k) || misaligned(v))
+    if (!rows_of_eight(k) || !rows_of_eight(v) || misaligned(k) || misaligned(v))
       refuse(PyExc_ValueError, "k_pages and v_pages must be 16-byte aligned, with a contiguous last "
                                "dimension and strides that are multiples of 8");
     const at::Tensor& t = tensor(table_, "block_table");
@@ -153,8 +156,8 @@ struct Call {
     c.k_pages = k.data_ptr();
     c.v_pages = v.data_ptr();
     for (int i = 0; i < 3; ++i) {
-      c.page_strides[i] = ks[i];
-      c.page_strides[3 + i] = vs[i];
+      c.page_strides[i] = stride_of(k, i);
+      c.page_strides[3 + i] = stride_of(v, i);
     }
     c.block_table = static_cast<const int32_t*>(table.data_ptr());
     c.table_stride = table.stride(0);
@@ -266,9 +269,9 @@ PyObject* append_impl(PyObject* const* a) {
     call.c.dtype_flags = call.dtype == at::kBFloat16 ? BSATTN_IN_BF16 : 0;
     int64_t st[9] = {0};
     for (int i = 0; i < 3; ++i) {
-      if (Hq > 0) st[i] = q.stride(i);
-      st[3 + i] = k.stride(i);
-      st[6 + i] = v.stride(i);
+      if (Hq > 0) st[i] = stride_of(q, i);
+      st[3 + i] = stride_of(k, i);
+      st[6 + i] = stride_of(v, i);
     }
     check_call(g_append(&call.c, Hq > 0 ? q.data_ptr() : nullptr, k.data_ptr(), v.data_ptr(), st,
                         Hq > 0 ? q_out.data_ptr() : nullptr,

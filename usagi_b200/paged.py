@@ -11,8 +11,9 @@ there is none for the prefill.
 The cache is plain tensors that the caller owns:
 
 * ``k_pages``, ``v_pages``: fp16 or bf16 ``[n_pages, Hkv, page_size, 128]``, page_size a power of two
-  from 16 to 1024.  Any strides that are multiples of 8 with a contiguous last dimension: a
-  ``[n_pages, page_size, Hkv, 128]`` cache is passed as ``pages.transpose(1, 2)``.
+  from 16 to 1024.  16-byte aligned, with a contiguous last dimension and strides that are multiples of 8
+  (those of dimensions of one entry do not count): a ``[n_pages, page_size, Hkv, 128]`` cache is passed
+  as ``pages.transpose(1, 2)``.
 * ``block_table``: int ``[B, max_pages]``, the pages of each sequence in order.  Entries behind a
   sequence's length are not read and may be anything, and so may, with a window, the entries of pages
   that no row of the call sees, and all entries of a sequence without live rows (behind a shared prefix
