@@ -116,3 +116,23 @@ def test_strides_of_one_page_or_head_do_not_matter(Tq, Hq):
     o, lse = ub.paged_attn_fwd(q, kp, vp, table, lens)
     ub.check_errors(DEV)
     check_attention(o, lse, attention(q.cpu(), c))
+
+
+def test_unsigned_64_bit_metadata():
+    """As for signed: what 32 bits do not hold stays out of range, what they hold is taken."""
+    c = Cache([40, 33], 2, 16, F16, 241, DEV)
+    (kp, vp, table, lens), q = c.to(DEV), _q(2, 4, 1, F16, 242)
+    table = table.clamp(min=0)  # the entries behind the sequences
+    wide = lambda x, far=0: (x.cpu().long() + far).to(torch.uint64).to(DEV)  # noqa: E731
+    top = lambda x: (x.cpu().long() - 2 ** 63).to(torch.uint64).to(DEV)  # noqa: E731
+    o, lse = ub.paged_attn_fwd(q.to(DEV), kp, vp, wide(table), wide(lens),
+                               q_lens=wide(torch.ones(2)))
+    ub.check_errors(DEV)
+    check_attention(o, lse, attention(q, c))
+    for bad in (dict(block_table=wide(table, 2 ** 32)), dict(seq_lens=wide(lens, 2 ** 32)),
+                dict(q_lens=wide(torch.ones(2), 2 ** 32)), dict(block_table=top(table)),
+                dict(seq_lens=top(lens)), dict(q_lens=top(torch.ones(2)))):
+        kw = dict(block_table=table, seq_lens=lens, q_lens=None)
+        kw.update(bad)
+        ub.paged_attn_fwd(q.to(DEV), kp, vp, **kw)
+        _expect_page_error()

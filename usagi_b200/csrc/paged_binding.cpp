@@ -92,6 +92,7 @@ at::Tensor index_tensor(const at::Tensor& t, const char* name, c10::Device dev, 
   if (!at::isIntegralType(x.scalar_type(), false))
     refuse(PyExc_TypeError, std::string(name) + " must hold integers");
   // What 32 bits do not hold stays out of range, where the kernels find it.
+  if (x.scalar_type() == at::kUInt64) x = x.to(at::kLong);  // what passes 2^63 becomes negative
   if (x.scalar_type() == at::kLong) x = x.clamp(INT32_MIN, INT32_MAX);
   if (x.scalar_type() != at::kInt || x.device() != dev) x = x.to(dev, at::kInt);
   if (x.stride(-1) != 1 && x.size(-1) > 1) x = x.contiguous();
