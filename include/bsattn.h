@@ -211,10 +211,11 @@ BSATTN_API int bsattn_peer_copy(void* dst, const void* src, size_t bytes, void* 
  * seq_lens[b] - q_lens[b] + t; the rows behind them are padding, and a row whose position is negative
  * is dead like them.
  * A page table entry outside [0, n_pages), a length outside the table or a live row count outside
- * [0, Tq] is reported as BSATTN_E_PAGE through bsattn_check_error and never used as an address:
- * the length or count is forced into range, the entry's tokens are not written, and are read as
- * zeros.  Slots that hold no token of a sequence are never used, whatever their bits are; values that
- * are held must be finite, since one that a row's mask excludes may still enter it with weight 0. */
+ * [0, Tq] is reported as BSATTN_E_PAGE through bsattn_check_error and never used as an address.  An
+ * entry's tokens are not written, and are read as zeros; with a length or count out of range nothing of
+ * the sequence is written, and its attention takes them as forced into range.  Slots that hold no token
+ * of a sequence are never used, whatever their bits are; values that are held must be finite, since one
+ * that a row's mask excludes may still enter it with weight 0. */
 typedef struct bsattn_paged_call {
   void* k_pages;              /* fp16 or bf16 [n_pages, Hkv, page_size, 128], 16-byte aligned      */
   void* v_pages;
@@ -241,10 +242,11 @@ typedef struct bsattn_paged_call {
  * was.  With inv_freq (rot_dim / 2 doubles on the device, rot_dim a multiple of 16 up to 128) the first
  * rot_dim values of each row of k, and of q [B, Hq, Tq, 128] on its way to q_out (contiguous; zero in
  * padding rows), are turned: pair i = (x_i, x_{i + rot_dim/2}), or (x_2i, x_{2i+1}) when interleaved, by
- * position * inv_freq[i].  inv_freq NULL: no rotation.  Hq == 0: no q.  q_out may be q itself when q is
- * contiguous.  in_strides[9] (host) = elements between batches, heads and tokens of q, k, v: multiples
- * of 8, also where the dimension is 1.  Two rows of one call must not share a slot (a page in two places
- * of the table): parts of both could be left. */
+ * position * inv_freq[i].  Rows of a sequence whose length or count is out of range are padding.
+ * inv_freq NULL: no rotation.  Hq == 0: no q.  q_out may be q itself when q is contiguous.
+ * in_strides[9] (host) = elements between batches, heads and tokens of q, k, v: multiples of 8, also where
+ * the dimension is 1.  Two rows of one call must not share a slot (a page in two places of the table):
+ * parts of both could be left. */
 BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q, const void* k,
                                    const void* v, const int64_t* in_strides, void* q_out,
                                    const double* inv_freq, int rot_dim, int interleaved);

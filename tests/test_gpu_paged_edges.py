@@ -136,3 +136,34 @@ def test_unsigned_64_bit_metadata():
         kw.update(bad)
         ub.paged_attn_fwd(q.to(DEV), kp, vp, **kw)
         _expect_page_error()
+
+
+@pytest.mark.parametrize("Tq", [1, 3])
+def test_append_writes_nothing_for_a_length_or_count_out_of_range(Tq):
+    """A sequence that has outgrown its table row, or a count of rows that the call does not have: there is no
+    right slot for its tokens, so the ones that are held stay, and its rows of q are zero."""
+    c = Cache([64, 40, 30], 2, 16, F16, 251, DEV, width_extra=0)
+    kp, vp, table, lens = c.to(DEV)
+    table = torch.where(table < 0, table.flatten()[0], table)  # a page behind a sequence, if one were used
+    inv = ub.rope_inv_freq(128, device=DEV)
+    k, v = _q(3, 2, Tq, F16, 252).to(DEV), _q(3, 2, Tq, F16, 253).to(DEV)
+    q = _q(3, 4, Tq, F16, 254).to(DEV)
+    same = torch.full((3,), Tq, dtype=torch.int32, device=DEV)
+    good = [x.clone() for x in (kp, vp)]
+    want_q = ub.paged_kv_append(*good, table, lens, k, v, q=q, inv_freq=inv)
+    ub.check_errors(DEV)
+    want_q[0] = 0
+    slots = [(table[0, (64 - Tq + t) // 16].item(), (64 - Tq + t) % 16) for t in range(Tq)]
+    for x, y in zip(good, (kp, vp)):
+        for page, slot in slots:
+            x[page, :, slot] = y[page, :, slot]
+    for which, value in [("len", 65), ("len", -1), ("len", 2 ** 31 - 1), ("rows", Tq + 1), ("rows", -1),
+                         ("rows", 2 ** 31 - 1)]:
+        bad = [lens.clone(), same.clone()]
+        bad[which == "rows"][0] = value
+        a = [x.clone() for x in (kp, vp)]
+        got = ub.paged_kv_append(*a, table, bad[0], k, v, q=q, q_lens=bad[1], inv_freq=inv)
+        _expect_page_error()
+        assert torch.equal(got, want_q), (which, value)
+        for x, y in zip(a, good):
+            assert torch.equal(x.view(torch.int16), y.view(torch.int16)), (which, value)

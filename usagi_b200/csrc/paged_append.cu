@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
       b = static_cast<int>(tok / p.c.Tq);
       t = static_cast<int>(tok - static_cast<long long>(b) * p.c.Tq);
       const SeqLen s = seq_len(p.c, b);
-      if (t < s.rows) pos = s.len - s.rows + t;
+      // A forced length or count says where no token belongs: it would go over one that is held.
+      if (t < s.rows && s.ok) pos = s.len - s.rows + t;
     }
     if (f == 0) {
       int page = -1;

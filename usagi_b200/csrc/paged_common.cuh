@@ -42,6 +42,7 @@ __device__ __forceinline__ void raise(int* err, int code) { atomicCAS(err, 0, co
 // a value outside is reported and never used to form an address.
 struct SeqLen {
   int len, rows;
+  bool ok;  // neither had to be forced
 };
 __device__ __forceinline__ SeqLen seq_len(const Cache& c, int b) {
   SeqLen s;
@@ -50,7 +51,8 @@ __device__ __forceinline__ SeqLen seq_len(const Cache& c, int b) {
   const int rows = c.q_lens != nullptr ? __ldg(c.q_lens + b) : c.Tq;
   s.len = min(max(len, 0), cap);
   s.rows = min(max(rows, 0), c.Tq);
-  if (s.len != len || s.rows != rows) raise(c.err, BSATTN_E_PAGE);
+  s.ok = s.len == len && s.rows == rows;
+  if (!s.ok) raise(c.err, BSATTN_E_PAGE);
   return s;
 }
 

@@ -27,7 +27,8 @@ Slots that hold no token may hold anything.  Values that are held must be finite
 of a call sees reach the others as well, with weight 0, and 0 times NaN is NaN.
 
 A page table entry, a length or a row count out of range is found on the device, never used as an
-address, and raised by :func:`usagi_b200.check_errors` (code ``E_PAGE``).
+address, and raised by :func:`usagi_b200.check_errors` (code ``E_PAGE``).  Such an entry's tokens are
+not written; of a sequence whose length or count is out of range none are, and its rotated q is zero.
 """
 from __future__ import annotations
 
