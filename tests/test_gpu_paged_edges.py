@@ -167,3 +167,23 @@ def test_append_writes_nothing_for_a_length_or_count_out_of_range(Tq):
         assert torch.equal(got, want_q), (which, value)
         for x, y in zip(a, good):
             assert torch.equal(x.view(torch.int16), y.view(torch.int16)), (which, value)
+
+
+def test_a_call_of_much_scratch_keeps_none():
+    """Its scratch goes back when it ends, and the stream keeps no other in its place."""
+    B, prefix = 1024, 512
+    c = Cache([prefix + 1] * B, 8, 64, F16, 261, DEV, prefix=prefix, extra_pages=0, width_extra=0)
+    q, args = _q(B, 8, 1, F16, 262), c.to(DEV)
+    qd = q.to(DEV)
+    stream = torch.cuda.Stream(DEV, priority=-1)
+    stream.wait_stream(torch.cuda.current_stream(DEV))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(DEV)
+    with torch.cuda.stream(stream):
+        torch.cuda.reset_peak_memory_stats(DEV)
+        o, lse = ub.shared_prefix_attn_fwd(qd, *args, prefix_len=prefix)
+        ub.check_errors(DEV)
+    assert torch.cuda.max_memory_allocated(DEV) - before > 32 << 20  # it needs more than is ever kept
+    kept = torch.cuda.memory_allocated(DEV) - before - o.nbytes - lse.nbytes
+    assert kept < 1 << 20, kept
+    check_attention(o[:8], lse[:8], [x[:8] for x in attention(q[:8], c)])

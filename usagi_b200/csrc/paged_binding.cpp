@@ -27,7 +27,7 @@
 namespace {
 
 constexpr int64_t kHeadDim = 128;
-constexpr int64_t kKept = 32 << 20;  // bytes of scratch that a stream keeps
+constexpr int64_t kKeptAtLeast = 4 << 20, kKept = 32 << 20;  // bytes of scratch that a stream keeps
 
 decltype(&bsattn_paged_append) g_append = nullptr;
 decltype(&bsattn_paged_fwd) g_fwd = nullptr;
@@ -214,10 +214,10 @@ Room room(c10::Device dev, cudaStream_t stream, int64_t need) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     return {at::empty({need}, bytes), at::zeros({g_counters()}, ints)};
   Room& r = rooms[{dev.index(), stream}];
-  const int64_t keep = std::min(std::max<int64_t>(need, 4 << 20), kKept);
   if (!r.counters.defined()) r.counters = at::zeros({g_counters()}, ints);
-  if (!r.scratch.defined() || r.scratch.numel() < std::min(need, kKept)) r.scratch = at::empty({keep}, bytes);
   if (need > kKept) return {at::empty({need}, bytes), r.counters};
+  if (!r.scratch.defined() || r.scratch.numel() < need)
+    r.scratch = at::empty({std::max<int64_t>(need, kKeptAtLeast)}, bytes);
   return r;
 }
 
