@@ -187,3 +187,22 @@ def test_a_call_of_much_scratch_keeps_none():
     kept = torch.cuda.memory_allocated(DEV) - before - o.nbytes - lse.nbytes
     assert kept < 1 << 20, kept
     check_attention(o[:8], lse[:8], [x[:8] for x in attention(q[:8], c)])
+
+
+def test_scratch_is_kept_for_a_few_streams_only():
+    """A call of 20 MB of scratch on 32 streams: those that were used last keep theirs."""
+    c = Cache([900, 400], 2, 64, F16, 271, DEV, width_extra=100)
+    q, args = _q(2, 8, 40, F16, 272).to(DEV), c.to(DEV)
+    want = ub.paged_attn_fwd(q, *args)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(DEV)
+    streams = [torch.cuda.Stream(DEV, priority=-1) for _ in range(32)]
+    assert len({s.cuda_stream for s in streams}) > 24
+    for _ in range(2):
+        for s in streams:
+            with torch.cuda.stream(s):
+                o, lse = ub.paged_attn_fwd(q, *args)
+                ub.check_errors(DEV)
+                assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    del o, lse
+    assert torch.cuda.memory_allocated(DEV) - before <= 16 * (33 << 20)

@@ -28,6 +28,7 @@ namespace {
 
 constexpr int64_t kHeadDim = 128;
 constexpr int64_t kKeptAtLeast = 4 << 20, kKept = 32 << 20;  // bytes of scratch that a stream keeps
+constexpr size_t kStreams = 16;                              // streams that keep any, the last ones used
 
 decltype(&bsattn_paged_append) g_append = nullptr;
 decltype(&bsattn_paged_fwd) g_fwd = nullptr;
@@ -202,18 +203,34 @@ int32_t as_int32(int64_t v, const char* what) {
 }
 
 // Scratch and counters of a call.  The calls of one CUDA stream follow one another, so a stream keeps
-// its own; a captured call gets new ones, which belong to the graph (the counters zeroed by it), since
-// graphs captured on one stream may be replayed at the same time.
+// its own (what another stream takes the place of goes back to the allocator, which hands it to that same
+// stream again); a captured call gets new ones, which belong to the graph (the counters zeroed by it),
+// since graphs captured on one stream may be replayed at the same time.
 struct Room {
   at::Tensor scratch, counters;
 };
 Room room(c10::Device dev, cudaStream_t stream, int64_t need) {
-  static std::map<std::pair<int, cudaStream_t>, Room> rooms;  // under the interpreter's lock
+  struct Kept {
+    Room room;
+    uint64_t call = 0;  // the last one that used it
+  };
+  static std::map<std::pair<int, cudaStream_t>, Kept> rooms;  // under the interpreter's lock
+  static uint64_t calls = 0;
   const auto bytes = at::TensorOptions().device(dev).dtype(at::kByte);
   const auto ints = at::TensorOptions().device(dev).dtype(at::kInt);
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     return {at::empty({need}, bytes), at::zeros({g_counters()}, ints)};
-  Room& r = rooms[{dev.index(), stream}];
+  const std::pair<int, cudaStream_t> key{dev.index(), stream};
+  auto at = rooms.find(key);
+  if (at == rooms.end()) {
+    if (rooms.size() >= kStreams)
+      rooms.erase(std::min_element(rooms.begin(), rooms.end(), [](const auto& a, const auto& b) {
+        return a.second.call < b.second.call;
+      }));
+    at = rooms.emplace(key, Kept{}).first;
+  }
+  at->second.call = ++calls;
+  Room& r = at->second.room;
   if (!r.counters.defined()) r.counters = at::zeros({g_counters()}, ints);
   if (need > kKept) return {at::empty({need}, bytes), r.counters};
   if (!r.scratch.defined() || r.scratch.numel() < need)
