@@ -129,10 +129,20 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
     """Compile ``csrc/*.cu`` into ``usagi_b200/libbsattn.so`` and the binding next to it; returns the
-    library path."""
-    build_binding(force, verbose)
+    library path.  The library needs only nvcc; where the binding cannot be built (no headers of Python
+    or torch) that is printed, and the paged-cache calls of Python are missing."""
+    _build_library(force, verbose, ptxas_info)
+    try:
+        build_binding(force, verbose)
+    except (ImportError, OSError, RuntimeError) as e:
+        BINDING_PATH.unlink(missing_ok=True)  # one of other sources must not meet this library
+        print(f"usagi_b200: no paged-cache calls, their binding was not built: {e}", file=sys.stderr)
+    return LIB_PATH
+
+
+def _build_library(force: bool, verbose: bool, ptxas_info: bool) -> None:
     if not force and not needs_build():
-        return LIB_PATH
+        return
     cmd = [_nvcc(), *NVCC_FLAGS]
     if ptxas_info:
         cmd += ["-Xptxas", "-v"]
@@ -144,7 +154,6 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     digest = source_hash()
     os.replace(tmp, LIB_PATH)
     STAMP_PATH.write_text(digest + "\n")
-    return LIB_PATH
 
 
 if __name__ == "__main__":
