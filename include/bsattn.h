@@ -46,8 +46,10 @@ extern "C" {
 
 enum {
   BSATTN_OK = 0,
-  BSATTN_E_SHAPE = -1,      /* B, H, T or D out of range, T % 128 != 0, D != 128          */
-  BSATTN_E_ALIGN = -2,      /* q/k/v/o not 16-byte aligned                                  */
+  BSATTN_E_SHAPE = -1,      /* B, H, T or D out of range, T % 128 != 0, D != 128; for a paged
+                               call a size or limit below                                   */
+  BSATTN_E_ALIGN = -2,      /* q/k/v/o (paged: pages, scratch) not 16-byte aligned, or a stride
+                               that is not a multiple of 8                                  */
   BSATTN_E_NULL = -3,       /* required pointer is NULL                                     */
   BSATTN_E_WORKSPACE = -4,  /* workspace NULL or smaller than bsattn_workspace_bytes()      */
   BSATTN_E_CUDA = -5,       /* CUDA runtime error (launch, attribute, device query)         */
@@ -260,9 +262,15 @@ BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q,
  * whole batch.  The result is that of prefix_len == 0.  Dead rows and rows without keys get o = 0 and
  * lse = -inf.
  * scale <= 0 selects 1/sqrt(128).
- * scratch: bsattn_paged_scratch_bytes bytes of device memory, 16-byte aligned, any content, used by
- * this call only.  counters: bsattn_paged_counters() ints of device memory, zero before their first
- * use; every call leaves them zero, and calls that may run at the same time need their own. */
+ * scratch: bsattn_paged_scratch_bytes bytes of device memory, 16-byte aligned, any content, used by this
+ * call only.  counters: bsattn_paged_counters() ints of device memory, zero before their first use; every
+ * call leaves them zero, and calls that may run at the same time need their own.
+ * Limits: B * Hq * Tq < 2^31, max_pages * page_size <= 2^31 - 256, and the tiles that the table has room
+ * for: with n the tiles of 8 rows of G * Tq (up to 8 rows, or behind a prefix) or those of 128,
+ * B * Hkv * n * (keys / 16 + 65, or keys / 128 + 65) <= 2^30, keys = max_pages * page_size.  A table that
+ * is wider than its sequences need costs scratch, and more than 8 rows of a short cache start about 3 us
+ * sooner when the table has room for no more than 32 MB of keys and values, all heads and tiles of 8 rows
+ * counted. */
 BSATTN_API int bsattn_paged_counters(void);
 BSATTN_API int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages,
                                           int page_size, int prefix_len, size_t* bytes);
@@ -277,7 +285,8 @@ BSATTN_API const char* bsattn_strerror(int code);
  * (BSATTN_IN_BF16, bsattn_bf16_to_f16), work lists (bsattn_plan, bsattn_fwd_plan, BSATTN_E_PLAN)
  * and device-built CSR patterns (bsattn_build_csr); minor 2 the analytic window rows
  * (bsattn_fwd_window, bsattn_plan_window) and, later, the paged cache (bsattn_paged_append,
- * bsattn_paged_fwd, BSATTN_E_PAGE).  Every 100 call keeps its meaning. */
+ * bsattn_paged_fwd, BSATTN_E_PAGE).  Whether a library of version 102 has the cache is told by its symbol
+ * bsattn_paged_fwd, or by bsattn_strerror(BSATTN_E_PAGE) being more than "unknown error".  Every 100 call keeps its meaning. */
 BSATTN_API int bsattn_version(void);
 
 #ifdef __cplusplus

@@ -206,3 +206,18 @@ def test_scratch_is_kept_for_a_few_streams_only():
                 assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
     del o, lse
     assert torch.cuda.memory_allocated(DEV) - before <= 16 * (33 << 20)
+
+
+def test_a_call_past_the_limits_says_so():
+    """What the C ABI refuses reaches the user with a text that is about these calls."""
+    pages = torch.zeros(1, 32, 1024, 128, dtype=F16, device=DEV)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV).expand(256, 2048)
+    lens = torch.ones(256, dtype=torch.int32, device=DEV)
+    q = torch.zeros(256, 32, 1, 128, dtype=F16, device=DEV)
+    for kw in (dict(block_table=table), dict(block_table=table[:, :64], window=(1 << 24) + 1)):
+        with pytest.raises(ub.BsattnError, match="paged") as err:
+            ub.paged_attn_fwd(q, pages, pages, seq_lens=lens, **kw)
+        assert err.value.code == _lib.E_SHAPE and "limits" in str(err.value)
+    o, lse = ub.paged_attn_fwd(q, pages, pages, table[:, :64], lens)
+    ub.check_errors(DEV)
+    assert (o == 0).all() and (lse == 0).all()

@@ -1132,8 +1132,12 @@ int bsattn_setup(void) { return device_setup(nullptr); }
 const char* bsattn_strerror(int code) {
   switch (code) {
     case BSATTN_OK: return "ok";
-    case BSATTN_E_SHAPE: return "bad shape: need B,H >= 1, T % 128 == 0, D == 128";
-    case BSATTN_E_ALIGN: return "q/k/v/o must be 16-byte aligned";
+    case BSATTN_E_SHAPE:
+      return "bad shape: a prefill call needs B,H >= 1, T % 128 == 0, D == 128, a paged call the sizes and "
+             "limits of bsattn.h";
+    case BSATTN_E_ALIGN:
+      return "q/k/v/o (of a paged call also the pages and the scratch) must be 16-byte aligned, strides "
+             "multiples of 8";
     case BSATTN_E_NULL: return "required pointer is NULL";
     case BSATTN_E_WORKSPACE: return "workspace missing or too small";
     case BSATTN_E_CUDA: return "CUDA runtime error";

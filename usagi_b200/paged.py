@@ -18,6 +18,9 @@ The cache is plain tensors that the caller owns:
   sequence's length are not read and may be anything, and so may, with a window, the entries of pages
   that no row of the call sees, and all entries of a sequence without live rows (behind a shared prefix
   those of its own pages).
+  A table that is no wider than the sequences need is best (``block_table[:, :n]`` is read in place):
+  the room it has sizes the scratch, and decides for more than 8 rows of a K/V head whether a short
+  cache is read by the kernel that starts 3 us sooner.
 * ``seq_lens``: int ``[B]``, tokens of each sequence, the new ones of this call included.
 * ``q_lens``: int ``[B]`` or None, how many of the Tq rows of each sequence are live (None: all).
   Row t < q_lens[b] is the token at position ``seq_lens[b] - q_lens[b] + t``; the rows behind them are
