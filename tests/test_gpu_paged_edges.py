@@ -221,3 +221,31 @@ def test_a_call_past_the_limits_says_so():
     o, lse = ub.paged_attn_fwd(q, pages, pages, table[:, :64], lens)
     ub.check_errors(DEV)
     assert (o == 0).all() and (lse == 0).all()
+
+
+@pytest.mark.parametrize("Tq", [1, 32])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype,mag", [(F16, 200.0), (F16, 30000.0), (BF16, 1e10), (BF16, 1e17)])
+def test_scores_of_any_size(dtype, mag, sign, Tq):
+    """One product per score, so that 32 bits hold it to half a step; the largest score is at least 2^-8 of its
+    size ahead of the others, whose weights vanish.  o is the value of that key, lse its score."""
+    n, H, G = 700, 1, 8
+    c = Cache([n], H, 32, dtype, 281, DEV)
+    g = torch.Generator().manual_seed(282)
+    x = sign * mag * (1 + torch.randperm(64, generator=g) / 64.0)
+    x = torch.cat([x, torch.full((n - 64,), mag * (0.5 if sign > 0 else -2.1))])
+    for j in range(n):
+        c.pages[0][c.table[0, j // 32], :, j % 32] = 0
+        c.pages[0][c.table[0, j // 32], 0, j % 32, 5] = x[j].to(dtype)
+    q = torch.zeros(1, G, Tq, 128, dtype=dtype)
+    q[..., 5] = (mag * (1 + torch.rand(1, G, Tq, generator=g))).to(dtype)
+    o, lse = ub.paged_attn_fwd(q.to(DEV), *c.to(DEV))
+    ub.check_errors(DEV)
+    s = c.dense(0, n, 0)[0, :, 5]
+    top = int(s.argmax())
+    v = c.dense(0, n, 1)[0, top]
+    u = torch.finfo(dtype).eps / 2
+    assert ((o.double().cpu() - v).abs() <= 2 * u * v.abs()).all()
+    want = q[..., 5].double() * s[top] * 128 ** -0.5
+    # score, scale_log2, their product, times ln 2: half a step each, and the constants' own
+    assert ((lse.double().cpu() - want).abs() <= 8 * 2.0 ** -24 * want.abs()).all()

@@ -49,8 +49,15 @@ constexpr int kThreads = 512;
 constexpr int kSoftmaxWarp0 = 4, kEpiWarp0 = 12;
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr float kNoMax = -1e30f;        // running maximum before the first visible key
-constexpr float kNoMaxBelow = -1e29f;
+constexpr float kNoMax = -3e38f;        // running maximum before the first visible key
+constexpr float kNoMaxBelow = -2.9e38f;
+// The exponent is one FMA, score * scale - maximum, and the maximum is that product rounded, so the largest
+// exponent is what the rounding lost: from 2^28 on up to 16 and more, where P would pass what fp16 holds.
+// Past 2^27 a row's unit is therefore the next power of two above the scale, whose products are exact.
+// That makes weights steeper by less than twice where 32-bit scores lie 8 apart and are themselves off by
+// more.  (117.3 us for 2 x 512 tokens over 8,192 keys without it, 117.5 with it; rounding the products of
+// such rows first, behind a vote of the warp, 121.)
+constexpr float kFar = 134217728.0f;
 constexpr int kPolyEvery = 4;           // every 4th pair of exponentials runs on the FMA pipe
 constexpr unsigned long long kDrainNs = 100000000ull;  // floor of the teardown waits
 constexpr int kRing = 8;
@@ -533,6 +540,8 @@ __device__ void softmax_role(Smem& sh, const Params& p, int half, uint32_t tmem)
   const int wq = t >> 5;
   const uint32_t lane_addr = tmem + (static_cast<uint32_t>(wq * 32) << 16);
   const float sl2 = p.scale_log2;
+  // The power of two that is not below the scale.
+  const float far_scale = __uint_as_float((__float_as_uint(sl2) + 0x7fffffu) & 0x7f800000u);
   const int glob_end = p.rule.glob * kTileKeys;
   int tile = 0;
   for (int ii = 0;; ++ii) {
@@ -590,7 +599,9 @@ __device__ void softmax_role(Smem& sh, const Params& p, int half, uint32_t tmem)
       ptx::mbar_arrive(ptx::smem_u32(&sh.xchg[sb][wq]));
       if (!wait_warp(ptx::smem_u32(&sh.xchg[sb][wq]), (static_cast<uint32_t>(tile) >> 1) & 1u, sh, p))
         return;
-      const float m_cand = fmaxf(pmax, sh.xmax[sb][half ^ 1][t]) * sl2;
+      const float top = fmaxf(pmax, sh.xmax[sb][half ^ 1][t]);
+      float m_cand = top * sl2;
+      if (fabsf(m_cand) > kFar) m_cand = top * far_scale;
       float alpha = 1.0f;
       bool rescale = false;
       if (j == 0) {
@@ -604,7 +615,8 @@ __device__ void softmax_role(Smem& sh, const Params& p, int half, uint32_t tmem)
           m_run = m_new;
         }
       }
-      const uint64_t sc2 = ptx::pack2(sl2, sl2);
+      const float sc = fabsf(m_run) > kFar ? far_scale : sl2;
+      const uint64_t sc2 = ptx::pack2(sc, sc);
       const uint64_t nm2 = ptx::pack2(-m_run, -m_run);
       uint64_t acc0 = 0, acc1 = 0;
       uint32_t pk[32];
@@ -655,7 +667,8 @@ __device__ void softmax_role(Smem& sh, const Params& p, int half, uint32_t tmem)
       if (!wait_warp(ptx::smem_u32(&sh.o_free[ob]), ((static_cast<uint32_t>(ii) >> 1) + 1u) & 1u, sh, p))
         return;
     }
-    if (half == 0) sh.stats[ob][0][t] = m_run;
+    if (half == 0)  // back in the scale's unit
+      sh.stats[ob][0][t] = fabsf(m_run) > kFar && m_run > kNoMaxBelow ? m_run * (sl2 / far_scale) : m_run;
     sh.stats[ob][1 + half][t] = l_run;
     ptx::mbar_arrive(ptx::smem_u32(&sh.stats_rdy[ob]));
   }
