@@ -1,12 +1,15 @@
 """Edges of the paged-cache calls: sequences that take no part in a call, limits of the arguments, layouts
 that differ only where a dimension has one entry, and what a call leaves behind.  Bounds as in
 paged_reference.py; every cache has NaN in all slots that hold no token."""
+import ctypes
+
 import pytest
 import torch
 
 import usagi_b200 as ub
 from usagi_b200 import _lib
 from paged_reference import Cache, attention, check_attention
+from test_paged_args import Call
 
 pytestmark = pytest.mark.gpu
 
@@ -249,3 +252,32 @@ def test_scores_of_any_size(dtype, mag, sign, Tq):
     want = q[..., 5].double() * s[top] * 128 ** -0.5
     # score, scale_log2, their product, times ln 2: half a step each, and the constants' own
     assert ((lse.double().cpu() - want).abs() <= 8 * 2.0 ** -24 * want.abs()).all()
+
+
+def test_counts_left_behind_do_not_stay():
+    """What a call that went wrong leaves in the counters (its lengths were rewritten while it ran, say) is
+    gone for the call after the next one of the same buffer."""
+    c = Cache([20011, 3000], 1, 64, F16, 291, DEV)
+    q = _q(2, 2, 1, F16, 292).to(DEV)
+    args = c.to(DEV)
+    want, want_lse = ub.paged_attn_fwd(q, *args)
+    ub.check_errors(DEV)
+    kp, vp, table, lens = args
+    lib = _lib.load()
+    need = ctypes.c_size_t()
+    assert lib.bsattn_paged_scratch_bytes(2, 2, 1, 1, table.shape[1], 64, 0, ctypes.byref(need)) == 0
+    scratch = torch.empty(need.value, dtype=torch.uint8, device=DEV)
+    counters = torch.ones(lib.bsattn_paged_counters(), dtype=torch.int32, device=DEV)
+    ws = torch.zeros(lib.bsattn_workspace_bytes() // 4 + 1, dtype=torch.int32, device=DEV)
+    call = Call(kp.data_ptr(), vp.data_ptr(), (ctypes.c_int64 * 6)(*kp.stride()[:3], *vp.stride()[:3]),
+                table.data_ptr(), table.stride(0), lens.data_ptr(), None, table.shape[1], kp.shape[0], 64,
+                2, 2, 1, 1, _lib.OUT_F16, ws.data_ptr(), ws.numel() * 4,
+                torch.cuda.current_stream(DEV).cuda_stream)
+    for i in range(5):
+        o, lse = torch.full_like(want, float("nan")), torch.full_like(want_lse, float("nan"))
+        assert lib.bsattn_paged_fwd(ctypes.byref(call), q.data_ptr(), o.data_ptr(), lse.data_ptr(), 0, 0, 0,
+                                    0.0, scratch.data_ptr(), need.value, counters.data_ptr()) == 0
+        torch.cuda.synchronize()
+        if i > 0:
+            assert torch.equal(o, want) and torch.equal(lse, want_lse), i
+    assert (counters == 0).all() and (ws == 0).all()

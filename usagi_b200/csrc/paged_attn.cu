@@ -528,7 +528,7 @@ int bsattn_paged_scratch_bytes(int B, int Hq, int Hkv, int Tq, int max_pages, in
   return BSATTN_OK;
 }
 
-int bsattn_paged_counters(void) { return kMaxSms * kFewRows; }
+int bsattn_paged_counters(void) { return 2 * kMaxSms * kFewRows; }
 
 int bsattn_paged_fwd(const bsattn_paged_call* call, const void* q, void* o, float* lse, int window,
                      int global_blocks, int prefix_len, float scale, void* scratch,

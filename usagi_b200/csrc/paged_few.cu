@@ -26,6 +26,7 @@
 // Keys past a sequence's end are loaded as zeros, never read: a recycled page may hold anything.
 // P is rounded to the type of V, as the tensor cores take it; its sum is of the unrounded values.
 #include <algorithm>
+#include <atomic>
 
 #include "paged_few.cuh"
 #include "sm100_ptx.cuh"
@@ -59,6 +60,7 @@ struct Params {
   float* part_o;
   float* part_l;
   int* counters;
+  int* others;  // the half of them that this call does not use
 };
 
 // What a warp leaves of an item that is not its own alone: which item, and the rows' maxima and sums.
@@ -361,6 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
   if (valid(cx)) load_q(cx.b, cx.h, qn);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load_next();
+  // Every call leaves its counters zero, unless its lengths are rewritten while it runs; then a later call
+  // must not begin with what it left.  The first CTA always gets here.
+  if (cta == 0 && !p.all_partial)
+    for (int i = threadIdx.x; i < kMaxSms * R; i += kThreads) p.others[i] = 0;
   if (lane == 0) sh.part[warp][0].item = sh.part[warp][1].item = -1;
   __syncwarp();
 
@@ -660,8 +666,13 @@ int few_launch(const FewCall& c, cudaStream_t stream) {
   using namespace few;
   // The tokens of a page and head lie side by side.
   const int packed = c.c.k_tok == kHeadDim * 2 && c.c.v_tok == kHeadDim * 2;
+  // Calls take the two halves of the counters by turns, and clear the one that they do not use.
+  static std::atomic<unsigned> calls{0};
+  constexpr int kHalf = kMaxSms * kFewRows;
+  const int turn = static_cast<int>(calls.fetch_add(1, std::memory_order_relaxed) & 1u);
   const Params p{c.c,        c.rule,        c.q,    c.o,   c.lse,    c.rows,   c.row_tiles, c.scale_log2,
-                 c.out_bf16, c.all_partial, packed, c.cum, c.part_o, c.part_l, c.counters};
+                 c.out_bf16, c.all_partial, packed, c.cum, c.part_o, c.part_l,
+                 c.counters + turn * kHalf, c.counters + (1 - turn) * kHalf};
   return launch(c.in_bf16 ? few_kernel<true> : few_kernel<false>, dim3(static_cast<unsigned>(c.ctas)),
                 kThreads, sizeof(Smem), stream, p);
 }

@@ -27,7 +27,7 @@ struct FewCall {
   int* cum;
   float* part_o;
   float* part_l;
-  int* counters;           // [kMaxSms, kFewRows], zero between calls
+  int* counters;           // [2, kMaxSms, kFewRows], zero between calls
 };
 
 int few_setup();

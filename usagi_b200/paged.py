@@ -26,6 +26,8 @@ The cache is plain tensors that the caller owns:
   Row t < q_lens[b] is the token at position ``seq_lens[b] - q_lens[b] + t``; the rows behind them are
   padding.
 
+Like those of any call, the tensors of these must stay as they are until the call has run on its stream.
+
 Slots that hold no token may hold anything.  Values that are held must be finite: those that one row
 of a call sees reach the others as well, with weight 0, and 0 times NaN is NaN.
 
