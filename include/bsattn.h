@@ -266,7 +266,7 @@ BSATTN_API int bsattn_paged_append(const bsattn_paged_call* call, const void* q,
  * call only.  counters: bsattn_paged_counters() ints of device memory, zero before their first use; every
  * call leaves them zero, and calls that may run at the same time need their own.  The arrays of a call,
  * lengths and table among them, must stay as they are until it has run; the results of one whose lengths
- * change meanwhile are not defined, nor are those of the next call of the same counters.
+ * change meanwhile are not defined, and those of the next call of the same counters may not be either.
  * Limits: B * Hq * Tq < 2^31, max_pages * page_size <= 2^31 - 256, and the tiles that the table has room
  * for: with n the tiles of 8 rows of G * Tq (up to 8 rows, or behind a prefix) or those of 128,
  * B * Hkv * n * (keys / 16 + 65, or keys / 128 + 65) <= 2^30, keys = max_pages * page_size.  A table that

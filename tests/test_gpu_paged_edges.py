@@ -256,7 +256,7 @@ def test_scores_of_any_size(dtype, mag, sign, Tq):
 
 def test_counts_left_behind_do_not_stay():
     """What a call that went wrong leaves in the counters (its lengths were rewritten while it ran, say) is
-    gone for the call after the next one of the same buffer."""
+    gone for the call after the next one of the same buffer, whatever other buffers are used between."""
     c = Cache([20011, 3000], 1, 64, F16, 291, DEV)
     q = _q(2, 2, 1, F16, 292).to(DEV)
     args = c.to(DEV)
@@ -274,6 +274,7 @@ def test_counts_left_behind_do_not_stay():
                 2, 2, 1, 1, _lib.OUT_F16, ws.data_ptr(), ws.numel() * 4,
                 torch.cuda.current_stream(DEV).cuda_stream)
     for i in range(5):
+        ub.paged_attn_fwd(q, *args)
         o, lse = torch.full_like(want, float("nan")), torch.full_like(want_lse, float("nan"))
         assert lib.bsattn_paged_fwd(ctypes.byref(call), q.data_ptr(), o.data_ptr(), lse.data_ptr(), 0, 0, 0,
                                     0.0, scratch.data_ptr(), need.value, counters.data_ptr()) == 0

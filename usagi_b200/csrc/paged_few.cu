@@ -666,10 +666,12 @@ int few_launch(const FewCall& c, cudaStream_t stream) {
   using namespace few;
   // The tokens of a page and head lie side by side.
   const int packed = c.c.k_tok == kHeadDim * 2 && c.c.v_tok == kHeadDim * 2;
-  // Calls take the two halves of the counters by turns, and clear the one that they do not use.
-  static std::atomic<unsigned> calls{0};
+  // The calls of a buffer take its two halves by turns, and clear the one that they do not use.  Buffers
+  // that share a place here only take their turns in another order.
+  static std::atomic<uint8_t> turns[1024];
   constexpr int kHalf = kMaxSms * kFewRows;
-  const int turn = static_cast<int>(calls.fetch_add(1, std::memory_order_relaxed) & 1u);
+  const uint64_t place = (reinterpret_cast<uintptr_t>(c.counters) >> 4) * 0x9E3779B97F4A7C15ull >> 54;
+  const int turn = turns[place].fetch_add(1, std::memory_order_relaxed) & 1;
   const Params p{c.c,        c.rule,        c.q,    c.o,   c.lse,    c.rows,   c.row_tiles, c.scale_log2,
                  c.out_bf16, c.all_partial, packed, c.cum, c.part_o, c.part_l,
                  c.counters + turn * kHalf, c.counters + (1 - turn) * kHalf};
