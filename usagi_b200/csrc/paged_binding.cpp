@@ -67,10 +67,11 @@ int64_t integer(PyObject* o, const char* name) {
 }
 
 // Stride of a dimension; one of a single entry is never used, whatever torch holds for it.
-int64_t stride_of(const at::Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : kHeadDim; }
+int64_t stride_of(at::IntArrayRef n, at::IntArrayRef s, int i) { return n[i] > 1 ? s[i] : kHeadDim; }
 // Whether rows of 128 contiguous values begin at multiples of 8.
 bool rows_of_eight(const at::Tensor& t) {
-  return t.stride(3) == 1 && ((stride_of(t, 0) | stride_of(t, 1) | stride_of(t, 2)) & 7) == 0;
+  const at::IntArrayRef n = t.sizes(), s = t.strides();
+  return s[3] == 1 && ((stride_of(n, s, 0) | stride_of(n, s, 1) | stride_of(n, s, 2)) & 7) == 0;
 }
 bool misaligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0; }
 
@@ -157,9 +158,10 @@ struct Call {
     if (!is_none(q_lens_)) q_lens = index_tensor(tensor(q_lens_, "q_lens"), "q_lens", dev, {B});
     c.k_pages = k.data_ptr();
     c.v_pages = v.data_ptr();
+    const at::IntArrayRef n = k.sizes(), ks = k.strides(), vs = v.strides();
     for (int i = 0; i < 3; ++i) {
-      c.page_strides[i] = stride_of(k, i);
-      c.page_strides[3 + i] = stride_of(v, i);
+      c.page_strides[i] = stride_of(n, ks, i);
+      c.page_strides[3 + i] = stride_of(n, vs, i);
     }
     c.block_table = static_cast<const int32_t*>(table.data_ptr());
     c.table_stride = table.stride(0);
@@ -286,10 +288,11 @@ PyObject* append_impl(PyObject* const* a) {
     call.c.Tq = as_int32(Tq, "Tq");
     call.c.dtype_flags = call.dtype == at::kBFloat16 ? BSATTN_IN_BF16 : 0;
     int64_t st[9] = {0};
+    const at::IntArrayRef n = k.sizes(), ks = k.strides(), vs = v.strides();
     for (int i = 0; i < 3; ++i) {
-      if (Hq > 0) st[i] = stride_of(q, i);
-      st[3 + i] = stride_of(k, i);
-      st[6 + i] = stride_of(v, i);
+      if (Hq > 0) st[i] = stride_of(q.sizes(), q.strides(), i);
+      st[3 + i] = stride_of(n, ks, i);
+      st[6 + i] = stride_of(n, vs, i);
     }
     check_call(g_append(&call.c, Hq > 0 ? q.data_ptr() : nullptr, k.data_ptr(), v.data_ptr(), st,
                         Hq > 0 ? q_out.data_ptr() : nullptr,
