@@ -24,7 +24,8 @@
 //     finds its row's parts complete adds them, in the order of the line: results do not depend on
 //     timing.
 // Keys past a sequence's end are loaded as zeros, never read: a recycled page may hold anything.
-// P is rounded to the type of V, as the tensor cores take it; its sum is of the unrounded values.
+// P is rounded to the type of V (fp16: 11 bits, bf16: 8), since one MMA takes both operands in one type and
+// a V converted to fp16 would lose what lies past its range; its sum is of the unrounded values.
 #include <algorithm>
 #include <atomic>
 

@@ -25,6 +25,7 @@
 //   warps 12-15 epilogue: o = O / l, to o (a whole item) or to the partial buffer, which is laid out
 //               [32 pieces of four columns][128 rows] so that the threads of a warp, one row each,
 //               write side by side.
+// P is rounded to the type of V, as in the few-row kernel; everything else is held in 32 bits.
 // Tensor memory: S[2] at columns 0 and 128 (P overwrites S), O[2] at 256 and 384.  Every wait is
 // bounded; on expiry all roles leave, copies and MMAs in flight are drained and the call reports
 // BSATTN_E_TIMEOUT.

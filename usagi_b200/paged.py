@@ -28,6 +28,9 @@ The cache is plain tensors that the caller owns:
 
 Like those of any call, the tensors of these must stay as they are until the call has run on its stream.
 
+Scores and sums are held in 32 bits; softmax weights are rounded to the pages' type before they meet V.
+For bf16 that is coarser than the prefill calls, which take fp16 weights and a V converted to fp16.
+
 Slots that hold no token may hold anything.  Values that are held must be finite: those that one row
 of a call sees reach the others as well, with weight 0, and 0 times NaN is NaN.
 
