@@ -119,7 +119,7 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     step, more rows check drafted tokens or process a chunk of a prompt.  The new tokens' keys are
     in the cache already (:func:`paged_kv_append`); each row sees the keys up to its own position.
     ``window`` (in blocks of 128) keeps, for a row in block i, the blocks > i - window and the first
-    ``global_blocks``: the rows of :func:`usagi_b200.block_sparse_attn_fwd_window`.  Returns
+    ``global_blocks`` (both up to 2^24): the rows of :func:`usagi_b200.block_sparse_attn_fwd_window`.  Returns
     ``(o, lse)`` like the prefill calls: o ``[B, Hq, Tq, 128]`` in ``out_dtype`` (default: q's),
     lse fp32 ``[B, Hq, Tq]`` (None if ``return_lse=False``); rows without a key, padding among them,
     get o = 0, lse = -inf.  ``scale`` is positive (None: 1/sqrt(128)).
